@@ -42,6 +42,11 @@ extern "C" {
 #define KH_Q8 1
 #define KH_Q4 2
 #define KH_Q4K 3
+/* How a paged KV cache keeps its rows (kh_paged_new), beside KH_F32: half
+ * precision, or 8-bit codes, each row of a KV head with a scale of its own.
+ * Not precisions of a weight. */
+#define KH_F16 4
+#define KH_I8 5
 
 typedef struct kh_ctx kh_ctx;
 typedef struct kh_weight kh_weight;
@@ -238,6 +243,97 @@ int kh_mla_attend(kh_ctx *ctx, const kh_kv *kv, size_t layer, size_t n_head, con
 /* The same over raw device arrays: c rows 512 wide, pe rows 64 wide. */
 int kh_mla_attend_dev(kh_ctx *ctx, size_t n_head, const float *q_lat, const float *q_pe, const float *c,
                       const float *pe, size_t n_positions, float scale, float *out);
+
+/* ---- paged KV cache ----------------------------------------------------- */
+
+/* No counterpart in the reference, whose caches are one array a conversation
+ * (KvCache, model/mod.rs:612-749).  A pool of pages per layer, each holding
+ * page_size positions of every KV head, shared by any number of sequences; a
+ * sequence is a row of page numbers in the caller's table, so pages can be
+ * handed out, given back and shared by a common prefix without a copy.  Rows
+ * are kept as
+ *   KH_F32  as they are
+ *   KH_F16  half precision, rounded to nearest, times a power of two: for a
+ *           row of a head with largest magnitude amax = f 2^e, 0.5 <= f < 1,
+ *           x / 2^(e - 15) is rounded (no row overflows; exponents from -126)
+ *   KH_I8   codes -127 .. 127 times amax / 127, rounded half away from zero
+ *           as QActivation::new rounds (quant.rs:1051-1059), but over the
+ *           head's row; a scale below 2^-126 is 0
+ * and a row with a NaN or an infinity in it reads back as NaN (KH_F32: as it
+ * is), and makes the attention of the rows that see it NaN, of no others.
+ * Largest magnitude of a value the attention takes: 2^96. */
+typedef struct kh_paged kh_paged;
+
+/* New rows of some sequences, one call's worth.  Rows row_start[s] ..
+ * row_start[s + 1] - 1 are sequence s's (row_start NULL: n_rows / n_seq each),
+ * and len[s] is how many positions it holds with them: its row j is position
+ * len[s] - its rows + j, which lies in page pages[s * max_pages + position /
+ * page_size].  The arrays are on the device for _dev calls (read when the
+ * work runs, so a captured graph takes the values of each replay), else on the
+ * host.  Rows that no sequence has, before row_start[0] or behind
+ * row_start[n_seq], are left as they were.  Values in device arrays cannot be
+ * refused; they never lead out of the cache or the rows: positions below zero
+ * or past max_pages, and pages outside 0 .. n_pages - 1, are not written, are
+ * seen by no row and read as zero.  A slot given to two rows of one push holds
+ * either's elements, mixed.  max_len (0: what max_pages hold) is the longest
+ * len, for choosing how work is split alone: any value gives the same results
+ * to rounding. */
+typedef struct kh_batch {
+    size_t n_seq, n_rows;
+    const int32_t *row_start; /* [n_seq + 1] or NULL */
+    const int32_t *len;       /* [n_seq] */
+    const int32_t *pages;     /* [n_seq][max_pages] */
+    size_t max_pages, max_len;
+} kh_batch;
+
+/* n_pages pages of page_size positions (32, 64, ... 1024) per layer; head_dim a
+ * multiple of 4 up to 256 (kept as 64, 128 or 256 dims); precision KH_F32,
+ * KH_F16 or KH_I8.  Slots that no row was written to hold zeros. */
+int kh_paged_new(kh_ctx *ctx, size_t n_layer, size_t n_kv_head, size_t head_dim, int precision, size_t page_size,
+                 size_t n_pages, kh_paged **out);
+int kh_paged_free(kh_paged *kv);
+/* Positions a page, pages, and device bytes of all layers. */
+int kh_paged_info(const kh_paged *kv, size_t *page_size, size_t *n_pages, size_t *bytes);
+/* Whether a batch in host memory is sound, without a device: rows in order,
+ * no more of a sequence's than its positions, lengths within the table, pages
+ * 0 .. n_pages - 1, and with `writes` no page that two sequences write to.
+ * KH_EINVAL and the reason otherwise.  The host calls below check theirs. */
+int kh_batch_check(const kh_batch *b, size_t page_size, size_t n_pages, int writes);
+
+/* The batch's rows written to `layer`: k and v [n_rows][n_kv_head][head_dim],
+ * rows k_stride and v_stride floats apart (0: packed).  The counterpart of
+ * KvCache::push (mod.rs:666-669).  Keys are pushed rotated. */
+int kh_paged_push(kh_paged *kv, size_t layer, const kh_batch *b, const float *k, const float *v);
+int kh_paged_push_dev(kh_paged *kv, size_t layer, const kh_batch *b, const float *k, size_t k_stride, const float *v,
+                      size_t v_stride);
+/* The batch's rows read back: what the cache rounded them to (KvCache::keys,
+ * values).  A batch whose sequences have len[s] rows reads them whole. */
+int kh_paged_read(const kh_paged *kv, size_t layer, const kh_batch *b, float *k, float *v);
+int kh_paged_read_dev(const kh_paged *kv, size_t layer, const kh_batch *b, float *k, size_t k_stride, float *v,
+                      size_t v_stride);
+/* Attention of the batch's rows over the cache, their own positions (pushed
+ * before) among it: with q and out [n_rows][n_head][head_dim] (rows q_stride
+ * and out_stride floats apart, 0: packed; out is not q) and head h reading KV
+ * head h / (n_head / n_kv_head), a row at position p weights the positions t
+ * in softmax(scale * q . k_t) over 0 <= t <= p; with window > 0 over those with
+ * t > p - window or t < sinks alone, and pages in between are not read.  A row
+ * that sees nothing is zero.  scale > 0 (model::attend's is
+ * 1 / sqrt(head_dim)).  No weight is dropped for its size, unlike kh_attend's;
+ * a position's part in the result is held to 2^-32 of the largest weight times
+ * the largest |v| that the row sees.
+ *
+ * Calls of few rows over many positions are split over the positions and
+ * joined through `ws`, 16-byte aligned device memory of up to
+ * kh_paged_attend_ws bytes (less: fewer splits).  ws NULL takes the context's
+ * scratch, and none while the stream is captured: a call in a graph that should
+ * be split brings its own, one for each graph that may run at the same time. */
+int kh_paged_attend(kh_paged *kv, size_t layer, const kh_batch *b, size_t n_head, const float *q, float scale,
+                    size_t window, size_t sinks, float *out);
+int kh_paged_attend_dev(kh_paged *kv, size_t layer, const kh_batch *b, size_t n_head, const float *q, size_t q_stride,
+                        float scale, size_t window, size_t sinks, float *out, size_t out_stride, void *ws,
+                        size_t ws_bytes);
+int kh_paged_attend_ws(const kh_paged *kv, const kh_batch *b, size_t n_head, size_t window, size_t sinks,
+                       size_t *bytes);
 
 /* ---- decode glue (device pointers, asynchronous on the context's stream) */
 

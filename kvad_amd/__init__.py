@@ -25,10 +25,11 @@ import numpy as np
 
 __all__ = [
     "F32", "Q8", "Q4", "Q4K", "KvadError", "Declined", "lib", "Context", "Weight", "matvec_many",
-    "KvCache", "Spec", "attend", "LIB_PATH", "Moe", "QCache", "mla_attend", "mla_attend_dev", "Llm", "LlmSpec", "Parked", "SOFTMAX", "SIGMOID", "GREEDY", "GROUP_LIMITED", "NOAUX_TC",
+    "KvCache", "Spec", "attend", "F16", "I8", "Batch", "PagedCache", "LIB_PATH", "Moe", "QCache", "mla_attend", "mla_attend_dev", "Llm", "LlmSpec", "Parked", "SOFTMAX", "SIGMOID", "GREEDY", "GROUP_LIMITED", "NOAUX_TC",
 ]
 
 F32, Q8, Q4, Q4K = 0, 1, 2, 3
+F16, I8 = 4, 5                            # rows of a PagedCache, beside F32
 SOFTMAX, SIGMOID = 0, 1                   # Scoring, model/ffn.rs:173-177
 GREEDY, GROUP_LIMITED, NOAUX_TC = 0, 1, 2  # Select, model/ffn.rs:179-195
 OK, DECLINED = 0, 1
@@ -111,6 +112,17 @@ _SIGS = {
     "kh_attend_dev": (C.c_int, [_p, _sz, _sz, _sz, _p, _p, _p, _sz, _p]),
     "kh_attend_dev_noalloc": (C.c_int, [_p, _sz, _sz, _sz, _p, _p, _p, _sz, _p]),
     "kh_noalloc_scratch_bytes": (_sz, []),
+    "kh_paged_new": (C.c_int, [_p, _sz, _sz, _sz, C.c_int, _sz, _sz, C.POINTER(_p)]),
+    "kh_paged_free": (C.c_int, [_p]),
+    "kh_paged_info": (C.c_int, [_p, C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz)]),
+    "kh_batch_check": (C.c_int, [_p, _sz, _sz, C.c_int]),
+    "kh_paged_push": (C.c_int, [_p, _sz, _p, _p, _p]),
+    "kh_paged_push_dev": (C.c_int, [_p, _sz, _p, _p, _sz, _p, _sz]),
+    "kh_paged_read": (C.c_int, [_p, _sz, _p, _p, _p]),
+    "kh_paged_read_dev": (C.c_int, [_p, _sz, _p, _p, _sz, _p, _sz]),
+    "kh_paged_attend": (C.c_int, [_p, _sz, _p, _sz, _p, C.c_float, _sz, _sz, _p]),
+    "kh_paged_attend_dev": (C.c_int, [_p, _sz, _p, _sz, _p, _sz, C.c_float, _sz, _sz, _p, _sz, _p, _sz]),
+    "kh_paged_attend_ws": (C.c_int, [_p, _p, _sz, _sz, _sz, C.POINTER(_sz)]),
     "kh_rms_norm_dev": (C.c_int, [_p, _p, _p, _sz, _sz, C.c_float, _p]),
     "kh_rope_dev": (C.c_int, [_p, _p, _p, _sz, _p, _sz, _sz, _sz, C.c_int]),
     "kh_swiglu_dev": (C.c_int, [_p, _p, _p, _sz]),
@@ -209,7 +221,7 @@ class Context:
         their session, sessions and MoE layers before the weights they name)."""
         if self.h:
             live = list(self._objects)
-            for kind in (Parked, Llm, Moe, KvCache, Weight):
+            for kind in (Parked, Llm, Moe, KvCache, PagedCache, Weight):
                 for obj in live:
                     if isinstance(obj, kind):
                         obj.free()
@@ -553,6 +565,117 @@ def attend(ctx: Context, spec: Spec, q, cache: KvCache, layer: int, n_positions:
     _check(lib.kh_attend(ctx.h, cache.h, layer, spec.n_head, spec.n_kv_head, spec.head_dim, _ptr(q),
                          n_positions, _ptr(out)))
     return out
+
+
+class Batch(C.Structure):
+    """kh_batch: one call's new rows of some sequences and where they lie.
+
+    Device addresses for the _dev calls; `Batch.host` builds one over numpy
+    arrays for the others (and keeps them referenced)."""
+    _fields_ = [("n_seq", _sz), ("n_rows", _sz), ("row_start", _p), ("len", _p), ("pages", _p), ("max_pages", _sz),
+                ("max_len", _sz)]
+
+    def __init__(self, n_seq: int, n_rows: int, len: int, pages: int, max_pages: int, row_start: int | None = None,
+                 max_len: int = 0):
+        super().__init__(n_seq, n_rows, row_start, len, pages, max_pages, max_len)
+
+    @classmethod
+    def host(cls, lens, pages, rows=None, n_rows: int | None = None) -> "Batch":
+        """lens [n_seq], pages [n_seq, max_pages]; rows: each sequence's new
+        rows, or None for n_rows / n_seq each."""
+        i32 = lambda a: np.ascontiguousarray(a, np.int32)  # noqa: E731
+        lens, pages = i32(lens), i32(pages)
+        if pages.ndim != 2 or pages.shape[0] != lens.size:
+            raise ValueError("pages are [n_seq, max_pages]")
+        start = None if rows is None else i32(np.concatenate([[0], np.cumsum(rows)]))
+        if start is not None and start.size != lens.size + 1:
+            raise ValueError("a row count for each sequence")
+        if n_rows is None:
+            if start is None:
+                raise ValueError("rows or n_rows")
+            n_rows = int(start[-1])
+        b = cls(lens.size, n_rows, _ptr(lens), _ptr(pages), pages.shape[1], None if start is None else _ptr(start),
+                int(lens.max(initial=0)))
+        b._keep = (lens, pages, start)
+        return b
+
+    def check(self, page_size: int, n_pages: int, writes: bool = False) -> None:
+        """kh_batch_check of a host batch; needs no device."""
+        _check(lib.kh_batch_check(C.byref(self), page_size, n_pages, int(writes)))
+
+
+class PagedCache:
+    """kh_paged: a pool of KV pages per layer that sequences hold by page
+    number, rows kept as F32, F16 or I8, and the attention over them.  The
+    _dev forms take device addresses and run on the context's stream; the
+    others take a Batch.host and numpy arrays."""
+
+    def __init__(self, ctx: Context, n_layer: int, n_kv_head: int, head_dim: int, n_pages: int, page_size: int = 64,
+                 precision: int = F32):
+        h = C.c_void_p()
+        _check(lib.kh_paged_new(ctx.h, n_layer, n_kv_head, head_dim, precision, page_size, n_pages, C.byref(h)))
+        self.ctx, self.h = ctx, h
+        ctx._own(self)
+        self.n_layer, self.n_kv_head, self.head_dim, self.precision = n_layer, n_kv_head, head_dim, precision
+        size, pages, nbytes = _sz(), _sz(), _sz()
+        _check(lib.kh_paged_info(h, C.byref(size), C.byref(pages), C.byref(nbytes)))
+        self.page_size, self.n_pages, self.bytes = size.value, pages.value, nbytes.value
+
+    def free(self) -> None:
+        if self.h:
+            lib.kh_paged_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+    def _rows(self, batch: Batch, x, heads: int) -> np.ndarray:
+        x = _f32(x)
+        assert x.size == batch.n_rows * heads * self.head_dim, "paged cache shape mismatch"
+        return x
+
+    def push(self, layer: int, batch: Batch, k, v) -> None:
+        k, v = self._rows(batch, k, self.n_kv_head), self._rows(batch, v, self.n_kv_head)
+        _check(lib.kh_paged_push(self.h, layer, C.byref(batch), _ptr(k), _ptr(v)))
+
+    def push_dev(self, layer: int, batch: Batch, k_ptr: int, v_ptr: int, k_stride: int = 0, v_stride: int = 0) -> None:
+        _check(lib.kh_paged_push_dev(self.h, layer, C.byref(batch), k_ptr, k_stride, v_ptr, v_stride))
+
+    def read(self, layer: int, batch: Batch) -> tuple[np.ndarray, np.ndarray]:
+        """The batch's rows as the cache holds them: k, v [n_rows, n_kv_head, head_dim]."""
+        k, v = (np.zeros((batch.n_rows, self.n_kv_head, self.head_dim), np.float32) for _ in range(2))
+        _check(lib.kh_paged_read(self.h, layer, C.byref(batch), _ptr(k), _ptr(v)))
+        return k, v
+
+    def read_dev(self, layer: int, batch: Batch, k_ptr: int, v_ptr: int, k_stride: int = 0, v_stride: int = 0) -> None:
+        _check(lib.kh_paged_read_dev(self.h, layer, C.byref(batch), k_ptr, k_stride, v_ptr, v_stride))
+
+    def attend(self, layer: int, batch: Batch, n_head: int, q, scale: float | None = None, window: int = 0,
+               sinks: int = 0) -> np.ndarray:
+        """out [n_rows, n_head, head_dim]; scale None: 1 / sqrt(head_dim), as attend's."""
+        q = self._rows(batch, q, n_head)
+        out = np.zeros((batch.n_rows, n_head, self.head_dim), np.float32)
+        _check(lib.kh_paged_attend(self.h, layer, C.byref(batch), n_head, _ptr(q), self._scale(scale), window, sinks,
+                                   _ptr(out)))
+        return out
+
+    def attend_dev(self, layer: int, batch: Batch, n_head: int, q_ptr: int, out_ptr: int, scale: float | None = None,
+                   window: int = 0, sinks: int = 0, q_stride: int = 0, out_stride: int = 0, ws_ptr: int | None = None,
+                   ws_bytes: int = 0) -> None:
+        _check(lib.kh_paged_attend_dev(self.h, layer, C.byref(batch), n_head, q_ptr, q_stride, self._scale(scale),
+                                       window, sinks, out_ptr, out_stride, ws_ptr, ws_bytes))
+
+    def attend_ws(self, batch: Batch, n_head: int, window: int = 0, sinks: int = 0) -> int:
+        """Bytes of workspace with which attend_dev splits such a call as it would with the context's."""
+        n = _sz()
+        _check(lib.kh_paged_attend_ws(self.h, C.byref(batch), n_head, window, sinks, C.byref(n)))
+        return n.value
+
+    def _scale(self, scale: float | None) -> float:
+        return self.head_dim ** -0.5 if scale is None else scale
 
 
 def mla_attend(ctx: Context, cache: "KvCache", layer: int, n_head: int, q_lat, q_pe, n_positions: int,

@@ -1,0 +1,103 @@
+// Internal declarations of the paged KV cache (paged.hip, paged_attn.hip).
+#pragma once
+
+#include "common.hpp"
+#include "device.hpp"
+#include "paged_layout.hpp"
+
+// A pool of pages per layer (kvad_hip.h); the pages' owners are the caller's tables.
+struct kh_paged {
+    kh_ctx *ctx = nullptr;
+    size_t n_layer = 0, n_kv_head = 0, head_dim = 0;
+    int precision = 0, es = 0, d = 0;
+    int page = 0, page_shift = 0;
+    size_t n_pages = 0;
+    size_t block = 0;               // bytes of one page of one head
+    size_t bytes = 0;               // of all layers
+    std::vector<char *> layers;
+};
+
+namespace kh {
+namespace paged {
+
+// A batch as the kernels take it: device arrays, sizes checked by the host.
+struct Batch {
+    const int32_t *row_start;  // or null: `per` rows each
+    const int32_t *len;
+    const int32_t *pages;
+    int n_seq, n_rows, per, max_pages;
+};
+
+constexpr int NAN_BITS = 0x7fc00000;
+
+__device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+// First row of sequence i, and of the one behind it; within the rows whatever
+// the table says.
+__device__ __forceinline__ int first_row(const Batch &b, int i) {
+    return b.row_start ? clampi(b.row_start[i], 0, b.n_rows) : i * b.per;
+}
+__device__ __forceinline__ int rows_of(const Batch &b, int i, int first) {
+    return b.row_start ? clampi(b.row_start[i + 1], first, b.n_rows) - first : b.per;
+}
+
+// Which sequence the tile'th tile of the batch belongs to, sequence i having
+// count(i) of them: a wave takes the running sum of 64 counts at a time.
+// False past the last tile.  `tile` is the same in every lane; so are the
+// results.
+template <typename F>
+__device__ __forceinline__ bool find_seq(int n_seq, int tile, F count, int &seq, int &local, int &n) {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < n_seq; base += 64) {
+        const int i = base + lane;
+        const int c = i < n_seq ? count(i) : 0;
+        int sum = c;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int up = __shfl_up(sum, o);
+            if (lane >= o) sum += up;
+        }
+        const int all = __builtin_amdgcn_readlane(sum, 63);
+        if (tile < all) {
+            const int l = __builtin_ctzll(__ballot(sum > tile));
+            n = __builtin_amdgcn_readlane(c, l);
+            local = tile - (__builtin_amdgcn_readlane(sum, l) - n);
+            seq = base + l;
+            return true;
+        }
+        tile -= all;
+    }
+    return false;
+}
+
+// An attention call over a layer (paged_attn.hip).
+struct AttnCall {
+    const kh_paged *kv;
+    const char *pool;
+    Batch b;
+    int n_head;
+    const float *q;
+    size_t q_stride;
+    float *out;
+    size_t out_stride;
+    float scale;
+    int window, sinks;   // window INT32_MAX: none
+    size_t max_len;      // positions of the longest sequence, for the split alone
+    void *ws;
+    size_t ws_bytes;
+};
+// How a call is cut up, from its sizes alone.
+struct AttnPlan {
+    bool wide;         // a workgroup's four waves take 32 rows each (else they share 32 rows)
+    int tile_rows;     // rows x heads of a workgroup: 128 or 32
+    int tiles;         // row tiles, or a bound on them where rows are ragged
+    int per;           // tiles of each sequence where rows are not
+    int splits;        // of the positions, over workgroups
+    int split_tiles;   // 32-position tiles a split
+    size_t ws_bytes;   // of partials
+};
+AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head, size_t max_len, int window, int sinks,
+                   size_t ws_max);
+int launch_attn(kh_ctx *ctx, const AttnCall &c, const AttnPlan &p);
+
+}  // namespace paged
+}  // namespace kh

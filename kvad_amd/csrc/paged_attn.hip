@@ -1,0 +1,604 @@
+// Attention over the paged KV cache: out = softmax(scale q K^T) V for ragged
+// batches of new rows, causal, over a sequence's whole cache or through a
+// window with sinks.  One pass over the positions, the running maximum and sum
+// of each row's softmax in registers.
+//
+// The products run on the f16 matrix cores with 32-bit results.  A f32 operand
+// is cut into two f16 pieces, hi + lo, 22 bits of significand: enough that the
+// result is as near the 64-bit one as f32 arithmetic is (the operands of a row
+// share a power-of-two scale, so f16's exponents are wide enough).  Cache rows
+// of f16, and i8 codes, are one exact f16 each: two products a tile, q's or the
+// weights' pieces against them; f32 rows are two pieces and three products (lo
+// by lo is below the 22 bits).  The f32 matrix cores run at a sixteenth of the
+// f16 rate.
+//
+// A wave takes 32 rows of one KV head (query tokens x the head's group,
+// flattened: each K and V byte is read once for the whole group) and 32
+// positions at a time: S^T = K Q^T, then O^T += V^T P^T.  In the transposed
+// form a lane keeps one row's weights for the 16 positions that V's operand
+// wants of it, so the weights go from one product to the next in registers,
+// and K and V come from memory in operand order (paged_layout.hpp): there is
+// no LDS in the loop.  K of the next tile and V of this one are loaded while
+// the weights are computed.
+#include <algorithm>
+
+#include "paged.hpp"
+
+namespace kh {
+namespace paged {
+namespace {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+typedef const __attribute__((address_space(4))) int32_t const_i32;
+
+constexpr float LOW = -3.0e38f;  // a running maximum that nothing has raised
+// Weights are kept at 2^BASE times their size over the row's reference, which
+// follows the maximum only when it is SLACK powers of two behind: under 2^15,
+// f16's range, and the sums are rescaled for few tiles.
+constexpr float BASE = 8.0f, SLACK = 6.0f;
+
+struct Args {
+    const char *pool;
+    Batch b;
+    const float *q;
+    size_t q_stride;
+    float *out;
+    size_t out_stride;
+    float *part, *part_ml;  // [split][row][head]: values [D], (reference, sum)
+    size_t block;
+    int n_kv, group, hd, n_pages, page, page_shift;
+    int tiles_per, splits, split_tiles, window, sinks, vec;
+    float scale;
+};
+
+__device__ __forceinline__ float shfl32(float v) { return __shfl_xor(v, 32); }
+__device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// hi + lo of two floats.  hi is cut off, not rounded: one instruction that the
+// compiler cannot split into two conversions, whose ties need not agree, one
+// for the product and one for the remainder.  The remainder is under 2^-10 of
+// the value and exact, lo is off by 2^-22 of the value.
+__device__ __forceinline__ void split2(float a, float b, h2 &hi, h2 &lo) {
+    hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
+    lo = h2{(_Float16)__builtin_fmaf((float)hi.x, -1.0f, a), (_Float16)__builtin_fmaf((float)hi.y, -1.0f, b)};
+}
+__device__ __forceinline__ void split8(const float *x, h8 &hi, h8 &lo) {
+    h2 h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) split2(x[2 * i], x[2 * i + 1], h[i], l[i]);
+    hi = h8{h[0].x, h[0].y, h[1].x, h[1].y, h[2].x, h[2].y, h[3].x, h[3].y};
+    lo = h8{l[0].x, l[0].y, l[1].x, l[1].y, l[2].x, l[2].y, l[3].x, l[3].y};
+}
+
+// Eight biased codes as f16: the bits of 1024 + byte are 0x6400 | byte.
+__device__ __forceinline__ h8 codes8(unsigned a, unsigned b) {
+    const h2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    const h2 r0 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u)) + off;
+    const h2 r1 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u)) + off;
+    const h2 r2 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) + off;
+    const h2 r3 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) + off;
+    return h8{r0.x, r0.y, r1.x, r1.y, r2.x, r2.y, r3.x, r3.y};
+}
+
+__device__ __forceinline__ f16v mfma(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ int4 load16(dev::rsrc_t r, unsigned voff, unsigned soff) {
+    return __builtin_bit_cast(int4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
+}
+
+// The positions a wave's rows see, as a list of 32-position tiles: those of
+// the sinks, then those from the first window's start on.
+struct Range {
+    int front, from, n;  // tiles of the sinks apart from the rest; first tile of the rest; tiles in all
+    __device__ int start(int i) const { return (i < front ? i : i - front + from) * TILE; }
+};
+__device__ __forceinline__ Range range_of(int p_lo, int p_hi, int cap, int window, int sinks) {
+    Range r{0, 0, 0};
+    const int end = min(p_hi + 1, cap);
+    if (end <= 0) return r;
+    const int last = (end + TILE - 1) / TILE;
+    const int front = (min(sinks, end) + TILE - 1) / TILE;
+    const int from = window == INT32_MAX ? 0 : max(0, p_lo - window + 1) / TILE;
+    if (front < from) {
+        r.front = front;
+        r.from = from;
+    }
+    r.n = r.front + max(last - r.from, 0);
+    return r;
+}
+
+// ES bytes an element, D dims, WS waves that share 32 rows (1: each its own).
+template <int ES, int D, int WS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ES == 4 || D == 256 ? 1 : 2)))
+void attn_kernel(Args a) {
+    constexpr int NK = D * ES / 32;  // loads of a lane for K
+    constexpr int DT = D / 32;       // dim tiles of V
+    constexpr int NS = D / 16;       // products over the dims
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int n = lane & 31, h = lane >> 5;
+    int rest = blockIdx.x;
+    const int head = rest % a.n_kv;
+    rest /= a.n_kv;
+    const int split = rest % a.splits, tile = rest / a.splits;
+    constexpr int ROWS = WS == 1 ? 128 : 32;
+
+    // the workgroup's rows: sequence s, rows row0 .. of its rows x group
+    int s, local, tiles;
+    if (a.b.row_start) {
+        auto at = [&](int i) {
+            const int r = first_row(a.b, i);
+            return (rows_of(a.b, i, r) * a.group + ROWS - 1) / ROWS;
+        };
+        if (!find_seq(a.b.n_seq, tile, at, s, local, tiles)) return;
+    } else {
+        tiles = a.tiles_per;
+        s = tile / tiles;
+        local = tile - s * tiles;
+    }
+    const int seq_row = first_row(a.b, s), seq_rows = rows_of(a.b, s, seq_row);
+    // later rows see more: they go first
+    const int row0 = (tiles - 1 - local) * ROWS + (WS == 1 ? 32 * wave : 0);
+    const int nr = min(seq_rows * a.group - row0, 32);
+    if (nr <= 0) return;
+    const int first = max(a.b.len[s], 0) - seq_rows;  // position of the sequence's first row
+    const int rr = row0 + min(n, nr - 1);
+    const int j = rr / a.group, g = rr - j * a.group;
+    const int pos = first + j;
+    const int p_lo = first + row0 / a.group, p_hi = first + (row0 + nr - 1) / a.group;
+    const int cap = a.b.max_pages << a.page_shift;
+    const Range range = range_of(p_lo, p_hi, cap, a.window, a.sinks);
+    int t_at = 0, t_end = range.n;
+    if (a.splits > 1) {
+        t_at = min(split * a.split_tiles, range.n);
+        t_end = split == a.splits - 1 ? range.n : min(t_at + a.split_tiles, range.n);
+    }
+    t_at += WS == 1 ? 0 : wave;
+
+    // q's rows, scaled to under 2^15 by a power of two, in two pieces
+    h8 qh[NS], ql[NS];
+    float rowf;  // score, in powers of two, of an accumulated product
+    {
+        const float *x = a.q + (size_t)(seq_row + j) * a.q_stride + (size_t)(head * a.group + g) * a.hd;
+        float v[NS][8];
+        int amax = 0;
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            const int d0 = k_dim(ES, i, h, 0);
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const int d = d0 + 4 * c;
+                if (d < a.hd)
+                    f = a.vec ? *reinterpret_cast<const float4 *>(x + d) : make_float4(x[d], x[d + 1], x[d + 2], x[d + 3]);
+                v[i][4 * c] = f.x;
+                v[i][4 * c + 1] = f.y;
+                v[i][4 * c + 2] = f.z;
+                v[i][4 * c + 3] = f.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) amax = max(amax, __builtin_bit_cast(int, v[i][e]) & 0x7fffffff);
+        }
+        amax = max(amax, __shfl_xor(amax, 32));
+        const int e = min(max((amax >> 23) - 126 - 15, -126), 113);  // amax < 2^(e + 15)
+        const float inv = __builtin_bit_cast(float, (127 - e) << 23);
+        rowf = (a.scale * 1.44269504088896341f) * __builtin_bit_cast(float, (127 + e) << 23);
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[i][k] = v[i][k] * inv;
+            split8(v[i], qh[i], ql[i]);
+        }
+    }
+
+    f16v acc[DT];
+#pragma unroll
+    for (int i = 0; i < DT; i++) acc[i] = f16v{0.0f};
+    float ref = LOW, sum = 0.0f;  // the row's reference and this lane's part of its sum
+
+    const int P = a.page;
+    const unsigned k_lane = (unsigned)(k_load_unit(ES, 0, h) * P + tile_pos(n)) * 16;
+    const unsigned v_lane = (unsigned)(P * D * ES) + (unsigned)(v_load_unit(ES, 0, h) * D + n) * 16;
+    const unsigned s_lane = (unsigned)(2 * P * D * ES) + 64 * h;
+    // read through the scalar cache: no wait for it is a wait for K or V
+    const_i32 *table = (const_i32 *)dev::uniform_ptr(a.b.pages + (size_t)s * a.b.max_pages);
+
+    struct Where {
+        dev::rsrc_t r;
+        int start, in_page;
+        bool there;
+    };
+    auto page_of = [&](int t) { return table[range.start(t) >> a.page_shift]; };
+    auto find = [&](int t, int page) {
+        Where w;
+        w.start = range.start(t);
+        w.there = page >= 0 && page < a.n_pages;
+        if (!w.there) page = 0;  // read, and hidden from every row
+        w.in_page = w.start & (P - 1);
+        w.r = dev::rsrc(dev::uniform_ptr(a.pool + ((size_t)page * a.n_kv + head) * a.block), a.block);
+        return w;
+    };
+    int4 kraw[NK], vraw[DT * ES];
+    float4 ks[4], vs[4];
+    float k_own = 0.0f;
+    auto load_k = [&](const Where &w) {
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            const int unit = k_load_unit(ES, i, 0);
+            kraw[i] = load16(w.r, k_lane, (unsigned)(unit * P + w.in_page) * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) ks[i] = __builtin_bit_cast(float4, load16(w.r, s_lane + 16 * i, 4 * w.in_page));
+        if (ES == 4) k_own = dev::bldf(w.r, (unsigned)(2 * P * D * ES) + 4 * (w.in_page + tile_pos(n)));
+    };
+    auto load_v = [&](const Where &w) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            vs[i] = __builtin_bit_cast(float4, load16(w.r, s_lane + 16 * i, (unsigned)(4 * P + 4 * w.in_page)));
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int c = 0; c < ES; c++)
+                vraw[dt * ES + c] = load16(w.r, v_lane + (c * D + dt * 32) * 16, (unsigned)(w.in_page * D * ES));
+    };
+
+    Where here;
+    if (t_at < t_end) {
+        here = find(t_at, page_of(t_at));
+        load_k(here);
+    }
+    for (int t = t_at; t < t_end; t += WS) {
+        const int next_page = page_of(min(t + WS, t_end - 1));
+        load_v(here);
+        __builtin_amdgcn_sched_barrier(0);
+
+        // ---- scores: register i is position start + 16 h + i ----
+        f16v sc = f16v{0.0f};
+        if (ES == 1) {
+#pragma unroll
+            for (int i = 0; i < NK; i++) {
+                const h8 k0 = codes8(kraw[i].x, kraw[i].y), k1 = codes8(kraw[i].z, kraw[i].w);
+                sc = mfma(k0, qh[2 * i % NS], sc);
+                sc = mfma(k0, ql[2 * i % NS], sc);
+                sc = mfma(k1, qh[(2 * i + 1) % NS], sc);
+                sc = mfma(k1, ql[(2 * i + 1) % NS], sc);
+            }
+        } else if (ES == 2) {
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                const h8 k = __builtin_bit_cast(h8, kraw[i % NK]);
+                sc = mfma(k, qh[i], sc);
+                sc = mfma(k, ql[i], sc);
+            }
+        } else {
+            // the position's scale, a power of two, inverted
+            const float inv = __builtin_bit_cast(float, 0x7f000000 - __builtin_bit_cast(int, k_own));
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                const float4 x = __builtin_bit_cast(float4, kraw[(2 * i) % NK]), y = __builtin_bit_cast(float4, kraw[(2 * i + 1) % NK]);
+                const float f[8] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv, y.x * inv, y.y * inv, y.z * inv, y.w * inv};
+                h8 kh, kl;
+                split8(f, kh, kl);
+                sc = mfma(kh, qh[i], sc);
+                sc = mfma(kh, ql[i], sc);
+                sc = mfma(kl, qh[i], sc);
+            }
+        }
+        float st[16];
+        {
+            const float all[16] = {ks[0].x, ks[0].y, ks[0].z, ks[0].w, ks[1].x, ks[1].y, ks[1].z, ks[1].w,
+                                   ks[2].x, ks[2].y, ks[2].z, ks[2].w, ks[3].x, ks[3].y, ks[3].z, ks[3].w};
+#pragma unroll
+            for (int i = 0; i < 16; i++) st[i] = sc[i] * all[i];
+        }
+        const int start = here.start;
+        const bool edge = !here.there || start + TILE - 1 > p_lo ||
+                          (a.window != INT32_MAX && start + TILE > a.sinks && start < p_hi - a.window + 1);
+        const bool there = here.there;
+        if (t + WS < t_end) {
+            here = find(t + WS, next_page);
+            load_k(here);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+
+        // ---- weights ----
+        float sv[16] = {vs[0].x, vs[0].y, vs[0].z, vs[0].w, vs[1].x, vs[1].y, vs[1].z, vs[1].w,
+                        vs[2].x, vs[2].y, vs[2].z, vs[2].w, vs[3].x, vs[3].y, vs[3].z, vs[3].w};
+        float inv_v[ES == 4 ? 16 : 1];
+        if (ES == 4) {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                inv_v[i % (ES == 4 ? 16 : 1)] = __builtin_bit_cast(float, 0x7f000000 - __builtin_bit_cast(int, sv[i]));
+        }
+        if (edge) {
+            // positions ahead of the row, behind its window, or in no page:
+            // no weight, and their rows' scales (NaN where a row is not
+            // finite) out of everything
+            const int lo = a.window == INT32_MAX ? 0 : pos - a.window + 1;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int at = start + 16 * h + i;
+                const bool seen = there && at <= pos && (at >= lo || at < a.sinks);
+                st[i] = seen ? st[i] : -__builtin_inff();
+                sv[i] = seen ? sv[i] : 0.0f;
+            }
+        }
+        float top = st[0];
+        unsigned vtop = __builtin_bit_cast(unsigned, sv[0]);
+#pragma unroll
+        for (int i = 1; i < 16; i++) {
+            top = fmaxf(top, st[i]);
+            vtop = max(vtop, __builtin_bit_cast(unsigned, sv[i]));
+        }
+        // the reference bounds weight times V's scale
+        const float vexp = (float)min(max((int)(vtop >> 23) - 127, -90), 90);
+        const float want = __builtin_fmaf(top, rowf, vexp);
+        if (__any(want > ref + SLACK)) {
+            // each row for itself: what it gives does not hang on the rows beside it
+            const float all = fmaxf(want, shfl32(want));
+            const float next = all > ref + SLACK ? all : ref;
+            const float f = exp2_(ref - next);
+            ref = next;
+            sum = sum * f;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) acc[dt][i] = acc[dt][i] * f;
+        }
+        const float shift = BASE - ref;
+        h8 ph[2], pl[2];
+        {
+            float w[16], part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float p = exp2_(__builtin_fmaf(st[i], rowf, shift));
+                part[i & 3] = part[i & 3] + p;
+                w[i] = p * sv[i];
+            }
+            sum = sum + ((part[0] + part[1]) + (part[2] + part[3]));
+            split8(w, ph[0], pl[0]);
+            split8(w + 8, ph[1], pl[1]);
+        }
+
+        // ---- O^T += V^T P^T ----
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) {
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                if (ES == 1) {
+                    const int4 r = vraw[dt * ES];
+                    const h8 v = c ? codes8(r.z, r.w) : codes8(r.x, r.y);
+                    acc[dt] = mfma(v, ph[c], acc[dt]);
+                    acc[dt] = mfma(v, pl[c], acc[dt]);
+                } else if (ES == 2) {
+                    const h8 v = __builtin_bit_cast(h8, vraw[dt * ES + c % ES]);
+                    acc[dt] = mfma(v, ph[c], acc[dt]);
+                    acc[dt] = mfma(v, pl[c], acc[dt]);
+                } else {
+                    const float4 x = __builtin_bit_cast(float4, vraw[dt * ES + (2 * c) % ES]);
+                    const float4 y = __builtin_bit_cast(float4, vraw[dt * ES + (2 * c + 1) % ES]);
+                    float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                    // a row that is not finite leaves finite pieces here: its
+                    // scale alone says so, to the rows that see it
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        f[e] = __builtin_amdgcn_fmed3f(f[e] * inv_v[(8 * c + e) % (ES == 4 ? 16 : 1)], -65504.0f, 65504.0f);
+                    h8 vh, vl;
+                    split8(f, vh, vl);
+                    acc[dt] = mfma(vh, ph[c], acc[dt]);
+                    acc[dt] = mfma(vh, pl[c], acc[dt]);
+                    acc[dt] = mfma(vl, ph[c], acc[dt]);
+                }
+            }
+        }
+    }
+    sum = sum + shfl32(sum);
+
+    if (WS > 1) {
+        // the four waves' sums, at the largest reference, two and then one
+        constexpr int SLAB = D < 128 ? D : 128, SN = SLAB / 2;  // dims and registers a step
+        __shared__ float s_acc[2][SN * 64];
+        __shared__ float s_ref[WS][32], s_sum[WS][32];
+        if (h == 0) {
+            s_ref[wave][n] = ref;
+            s_sum[wave][n] = sum;
+        }
+        __syncthreads();
+        float all = s_ref[0][n];
+#pragma unroll
+        for (int w = 1; w < WS; w++) all = fmaxf(all, s_ref[w][n]);
+        const float f = exp2_(ref - all);
+        sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WS; w++) sum = sum + s_sum[w][n] * exp2_(s_ref[w][n] - all);
+        ref = all;
+#pragma unroll
+        for (int half = WS / 2; half >= 1; half /= 2) {
+#pragma unroll
+            for (int d0 = 0; d0 < DT; d0 += SLAB / 32) {
+                if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                    for (int k = 0; k < SN; k++) {
+                        const float v = acc[d0 + k / 16][k % 16];
+                        s_acc[wave - half][k * 64 + lane] = half == WS / 2 ? v * f : v;
+                    }
+                }
+                __syncthreads();
+                if (wave < half) {
+#pragma unroll
+                    for (int k = 0; k < SN; k++) {
+                        const float v = acc[d0 + k / 16][k % 16];
+                        acc[d0 + k / 16][k % 16] = (half == WS / 2 ? v * f : v) + s_acc[wave][k * 64 + lane];
+                    }
+                }
+                __syncthreads();
+            }
+        }
+        if (wave > 0) return;
+    }
+    if (n >= nr) return;
+
+    const size_t row = (size_t)(seq_row + j);
+    const int q_head = head * a.group + g;
+    if (a.splits > 1) {
+        const size_t at = ((size_t)split * a.b.n_rows + row) * (a.n_kv * a.group) + q_head;
+        if (h == 0) {
+            a.part_ml[2 * at] = ref;
+            a.part_ml[2 * at + 1] = sum;
+        }
+        if (sum == 0.0f) return;  // nothing seen here: the merge reads no values
+        float *o = a.part + at * D;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *reinterpret_cast<float4 *>(o + dt * 32 + 8 * i + 4 * h) =
+                    make_float4(acc[dt][4 * i], acc[dt][4 * i + 1], acc[dt][4 * i + 2], acc[dt][4 * i + 3]);
+        return;
+    }
+    float *o = a.out + row * a.out_stride + (size_t)q_head * a.hd;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int d = dt * 32 + 8 * i + 4 * h;
+            if (d >= a.hd) continue;
+            const float v[4] = {acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv, acc[dt][4 * i + 2] * inv,
+                                acc[dt][4 * i + 3] * inv};
+            if (a.vec) {
+                *reinterpret_cast<float4 *>(o + d) = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+                for (int e = 0; e < 4; e++) o[d + e] = v[e];
+            }
+        }
+}
+
+// The splits of a row and head, joined at the largest reference: a wave each.
+template <int D>
+__global__ __launch_bounds__(256) void merge_kernel(Args a) {
+    const int n_head = a.n_kv * a.group;
+    const size_t item = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (item >= (size_t)a.b.n_rows * n_head) return;
+    const int row = (int)(item / n_head);
+    // rows that no sequence has stay as they are
+    if (row < first_row(a.b, 0)) return;
+    if (a.b.row_start && row >= clampi(a.b.row_start[a.b.n_seq], 0, a.b.n_rows)) return;
+    const size_t step = (size_t)a.b.n_rows * n_head;
+    float all = LOW;
+    for (int i = lane; i < a.splits; i += 64) all = fmaxf(all, a.part_ml[2 * (i * step + item)]);
+    for (int o = 1; o < 64; o <<= 1) all = fmaxf(all, __shfl_xor(all, o));
+    constexpr int E = D / 64;
+    float acc[E] = {}, sum = 0.0f;
+    for (int i = 0; i < a.splits; i++) {
+        const size_t at = i * step + item;
+        const float l = a.part_ml[2 * at + 1];
+        if (l == 0.0f) continue;
+        const float f = exp2_(a.part_ml[2 * at] - all);
+        sum = sum + l * f;
+#pragma unroll
+        for (int e = 0; e < E; e++) acc[e] = acc[e] + a.part[at * D + E * lane + e] * f;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    float *o = a.out + (size_t)row * a.out_stride + (item - (size_t)row * n_head) * a.hd;
+#pragma unroll
+    for (int e = 0; e < E; e++)
+        if (E * lane + e < a.hd) o[E * lane + e] = acc[e] * inv;
+}
+
+template <int ES, int D>
+int launch(const Args &a, const AttnPlan &p, unsigned blocks, size_t items, hipStream_t stream) {
+    if (p.wide) attn_kernel<ES, D, 1><<<blocks, 256, 0, stream>>>(a);
+    else attn_kernel<ES, D, 4><<<blocks, 256, 0, stream>>>(a);
+    KH_HIP(hipGetLastError());
+    if (p.splits > 1) {
+        merge_kernel<D><<<(unsigned)((items + 3) / 4), 256, 0, stream>>>(a);
+        KH_HIP(hipGetLastError());
+    }
+    return KH_OK;
+}
+
+template <int ES>
+int launch_d(int d, const Args &a, const AttnPlan &p, unsigned blocks, size_t items, hipStream_t s) {
+    if (d == 64) return launch<ES, 64>(a, p, blocks, items, s);
+    if (d == 128) return launch<ES, 128>(a, p, blocks, items, s);
+    return launch<ES, 256>(a, p, blocks, items, s);
+}
+
+size_t up_to(size_t n, size_t m) { return (n + m - 1) / m; }
+
+}  // namespace
+
+AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head, size_t max_len, int window, int sinks,
+                   size_t ws_max) {
+    AttnPlan p{};
+    const size_t group = (size_t)n_head / kv->n_kv_head;
+    auto tiles = [&](size_t rows) {
+        return b.row_start ? (size_t)b.n_rows * group / rows + b.n_seq : b.n_seq * up_to((size_t)b.per * group, rows);
+    };
+    // 128 rows a workgroup where that alone is two workgroups a CU
+    p.wide = tiles(128) * kv->n_kv_head >= 2 * (size_t)cu_count;
+    p.tile_rows = p.wide ? 128 : 32;
+    p.tiles = (int)tiles(p.tile_rows);
+    p.per = b.row_start ? 0 : (int)up_to((size_t)b.per * group, p.tile_rows);
+    // positions a tile of rows goes over, at most
+    size_t span = max_len;
+    if (window != INT32_MAX) span = std::min(span, (size_t)window + p.tile_rows / group + sinks + 2 * TILE);
+    const size_t pos_tiles = up_to(span, TILE);
+    const size_t blocks = (size_t)p.tiles * kv->n_kv_head;
+    p.splits = 1;
+    p.split_tiles = (int)pos_tiles;
+    if (!p.wide) {
+        // enough workgroups for two a CU twice over, 16 tiles to each at least
+        const size_t want = up_to(4 * (size_t)cu_count, blocks);
+        const size_t most = std::max<size_t>(1, pos_tiles / 16);
+        size_t splits = std::min(std::min(want, most), (size_t)1024);
+        const size_t each = 4 * (size_t)b.n_rows * n_head * (kv->d + 2);
+        if (ws_max / each < splits) splits = ws_max / each;
+        if (splits > 1) {
+            p.split_tiles = (int)up_to(pos_tiles, splits);
+            p.splits = (int)up_to(pos_tiles, p.split_tiles);
+            p.ws_bytes = p.splits > 1 ? each * p.splits : 0;
+        }
+    }
+    return p;
+}
+
+int launch_attn(kh_ctx *ctx, const AttnCall &c, const AttnPlan &p) {
+    const kh_paged *kv = c.kv;
+    Args a{};
+    a.pool = c.pool;
+    a.b = c.b;
+    a.q = c.q;
+    a.q_stride = c.q_stride;
+    a.out = c.out;
+    a.out_stride = c.out_stride;
+    const size_t items = (size_t)c.b.n_rows * c.n_head;
+    a.part = static_cast<float *>(c.ws);
+    a.part_ml = a.part ? a.part + (size_t)p.splits * items * kv->d : nullptr;
+    a.block = kv->block;
+    a.n_kv = (int)kv->n_kv_head;
+    a.group = c.n_head / a.n_kv;
+    a.hd = (int)kv->head_dim;
+    a.n_pages = (int)kv->n_pages;
+    a.page = kv->page;
+    a.page_shift = kv->page_shift;
+    a.tiles_per = p.per;
+    a.splits = p.splits;
+    a.split_tiles = p.split_tiles;
+    a.window = c.window;
+    a.sinks = c.sinks;
+    a.scale = c.scale;
+    auto vec = [](const void *x, size_t stride) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && stride % 4 == 0; };
+    a.vec = vec(c.q, c.q_stride) && vec(c.out, c.out_stride);
+    const unsigned blocks = (unsigned)((size_t)p.tiles * kv->n_kv_head * p.splits);
+    if (kv->es == 4) return launch_d<4>(kv->d, a, p, blocks, items, ctx->stream);
+    if (kv->es == 2) return launch_d<2>(kv->d, a, p, blocks, items, ctx->stream);
+    return launch_d<1>(kv->d, a, p, blocks, items, ctx->stream);
+}
+
+}  // namespace paged
+}  // namespace kh
