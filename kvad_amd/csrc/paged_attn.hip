@@ -31,6 +31,7 @@ namespace {
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));  // rows may start at any float
 
 typedef const __attribute__((address_space(4))) int32_t const_i32;
 
@@ -50,7 +51,7 @@ struct Args {
     float *part, *part_ml;  // [split][row][head]: values [D], (reference, sum)
     size_t block;
     int n_kv, group, hd, n_pages, page, page_shift;
-    int tiles_per, splits, split_tiles, window, sinks, vec;
+    int tiles_per, splits, split_tiles, window, sinks;
     float scale;
 };
 
@@ -62,8 +63,10 @@ __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(
 // for the product and one for the remainder.  The remainder is under 2^-10 of
 // the value and exact, lo is off by 2^-22 of the value.
 __device__ __forceinline__ void split2(float a, float b, h2 &hi, h2 &lo) {
+    float minus = -1.0f;
+    asm("" : "+s"(minus));  // known, the product would become a conversion and a subtraction
     hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
-    lo = h2{(_Float16)__builtin_fmaf((float)hi.x, -1.0f, a), (_Float16)__builtin_fmaf((float)hi.y, -1.0f, b)};
+    lo = h2{(_Float16)__builtin_fmaf((float)hi.x, minus, a), (_Float16)__builtin_fmaf((float)hi.y, minus, b)};
 }
 __device__ __forceinline__ void split8(const float *x, h8 &hi, h8 &lo) {
     h2 h[4], l[4];
@@ -169,14 +172,10 @@ void attn_kernel(Args a) {
             const int d0 = k_dim(ES, i, h, 0);
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 const int d = d0 + 4 * c;
-                if (d < a.hd)
-                    f = a.vec ? *reinterpret_cast<const float4 *>(x + d) : make_float4(x[d], x[d + 1], x[d + 2], x[d + 3]);
-                v[i][4 * c] = f.x;
-                v[i][4 * c + 1] = f.y;
-                v[i][4 * c + 2] = f.z;
-                v[i][4 * c + 3] = f.w;
+                const float4u f = *reinterpret_cast<const float4u *>(x + min(d, a.hd - 4));
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[i][4 * c + e] = d < a.hd ? f[e] : 0.0f;
             }
 #pragma unroll
             for (int e = 0; e < 8; e++) amax = max(amax, __builtin_bit_cast(int, v[i][e]) & 0x7fffffff);
@@ -223,14 +222,16 @@ void attn_kernel(Args a) {
     int4 kraw[NK], vraw[DT * ES];
     float4 ks[4], vs[4];
     float k_own = 0.0f;
+    auto load_ks = [&](const Where &w) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) ks[i] = __builtin_bit_cast(float4, load16(w.r, s_lane + 16 * i, 4 * w.in_page));
+    };
     auto load_k = [&](const Where &w) {
 #pragma unroll
         for (int i = 0; i < NK; i++) {
             const int unit = k_load_unit(ES, i, 0);
             kraw[i] = load16(w.r, k_lane, (unsigned)(unit * P + w.in_page) * 16);
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++) ks[i] = __builtin_bit_cast(float4, load16(w.r, s_lane + 16 * i, 4 * w.in_page));
         if (ES == 4) k_own = dev::bldf(w.r, (unsigned)(2 * P * D * ES) + 4 * (w.in_page + tile_pos(n)));
     };
     auto load_v = [&](const Where &w) {
@@ -248,9 +249,12 @@ void attn_kernel(Args a) {
     if (t_at < t_end) {
         here = find(t_at, page_of(t_at));
         load_k(here);
+        load_ks(here);
     }
     for (int t = t_at; t < t_end; t += WS) {
-        const int next_page = page_of(min(t + WS, t_end - 1));
+        // the next tile (this one again behind the last: the loads in flight
+        // are the same at every wait, and none waits for more than its own)
+        const int next_t = min(t + WS, t_end - 1), next_page = page_of(next_t);
         load_v(here);
         __builtin_amdgcn_sched_barrier(0);
 
@@ -286,6 +290,13 @@ void attn_kernel(Args a) {
                 sc = mfma(kl, qh[i], sc);
             }
         }
+        const int start = here.start;
+        const bool edge = !here.there || start + TILE - 1 > p_lo ||
+                          (a.window != INT32_MAX && start + TILE > a.sinks && start < p_hi - a.window + 1);
+        const bool there = here.there;
+        here = find(next_t, next_page);
+        load_k(here);
+        __builtin_amdgcn_sched_barrier(0);
         float st[16];
         {
             const float all[16] = {ks[0].x, ks[0].y, ks[0].z, ks[0].w, ks[1].x, ks[1].y, ks[1].z, ks[1].w,
@@ -293,15 +304,8 @@ void attn_kernel(Args a) {
 #pragma unroll
             for (int i = 0; i < 16; i++) st[i] = sc[i] * all[i];
         }
-        const int start = here.start;
-        const bool edge = !here.there || start + TILE - 1 > p_lo ||
-                          (a.window != INT32_MAX && start + TILE > a.sinks && start < p_hi - a.window + 1);
-        const bool there = here.there;
-        if (t + WS < t_end) {
-            here = find(t + WS, next_page);
-            load_k(here);
-        }
         __builtin_amdgcn_sched_barrier(0);
+        load_ks(here);
 
         // ---- weights ----
         float sv[16] = {vs[0].x, vs[0].y, vs[0].z, vs[0].w, vs[1].x, vs[1].y, vs[1].z, vs[1].w,
@@ -466,41 +470,66 @@ void attn_kernel(Args a) {
         for (int i = 0; i < 4; i++) {
             const int d = dt * 32 + 8 * i + 4 * h;
             if (d >= a.hd) continue;
-            const float v[4] = {acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv, acc[dt][4 * i + 2] * inv,
-                                acc[dt][4 * i + 3] * inv};
-            if (a.vec) {
-                *reinterpret_cast<float4 *>(o + d) = make_float4(v[0], v[1], v[2], v[3]);
-            } else {
-                for (int e = 0; e < 4; e++) o[d + e] = v[e];
-            }
+            *reinterpret_cast<float4u *>(o + d) = float4u{acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv,
+                                                          acc[dt][4 * i + 2] * inv, acc[dt][4 * i + 3] * inv};
         }
 }
 
-// The splits of a row and head, joined at the largest reference: a wave each.
-template <int D>
+// The splits of a row and head, joined at the largest reference, by WM waves:
+// one, or four that take every fourth split where there are many.
+template <int D, int WM>
 __global__ __launch_bounds__(256) void merge_kernel(Args a) {
     const int n_head = a.n_kv * a.group;
-    const size_t item = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const size_t item = WM == 1 ? (size_t)blockIdx.x * 4 + wave : blockIdx.x;
     if (item >= (size_t)a.b.n_rows * n_head) return;
     const int row = (int)(item / n_head);
     // rows that no sequence has stay as they are
     if (row < first_row(a.b, 0)) return;
     if (a.b.row_start && row >= clampi(a.b.row_start[a.b.n_seq], 0, a.b.n_rows)) return;
     const size_t step = (size_t)a.b.n_rows * n_head;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + item;
     float all = LOW;
-    for (int i = lane; i < a.splits; i += 64) all = fmaxf(all, a.part_ml[2 * (i * step + item)]);
+    for (int i = lane; i < a.splits; i += 64) all = fmaxf(all, ml[i * step].x);
     for (int o = 1; o < 64; o <<= 1) all = fmaxf(all, __shfl_xor(all, o));
     constexpr int E = D / 64;
-    float acc[E] = {}, sum = 0.0f;
-    for (int i = 0; i < a.splits; i++) {
-        const size_t at = i * step + item;
-        const float l = a.part_ml[2 * at + 1];
-        if (l == 0.0f) continue;
-        const float f = exp2_(a.part_ml[2 * at] - all);
-        sum = sum + l * f;
+    typedef float fe __attribute__((ext_vector_type(E)));
+    fe acc = {};
+    float sum = 0.0f;
+    for (int base = 0; base < a.splits; base += 64) {
+        // a lane keeps a split's weight; a split that saw nothing has no values
+        const int i = base + lane;
+        const float2 m = i < a.splits ? ml[i * step] : make_float2(LOW, 0.0f);
+        const float f = m.y == 0.0f ? 0.0f : exp2_(m.x - all);
+        sum = sum + (m.y == 0.0f ? 0.0f : m.y * f);
+        const unsigned long long has = __ballot(m.y != 0.0f);
+        const float *from = a.part + ((size_t)base * step + item) * D + E * lane;
+        const int n = min(a.splits - base, 64);
+        constexpr int AT_ONCE = 4;
+        for (int k = WM == 1 ? 0 : wave; k < n; k += WM * AT_ONCE) {
+            fe v[AT_ONCE];
 #pragma unroll
-        for (int e = 0; e < E; e++) acc[e] = acc[e] + a.part[at * D + E * lane + e] * f;
+            for (int u = 0; u < AT_ONCE; u++) {
+                const int j = k + u * WM;
+                v[u] = fe{};
+                if (j < n && (has >> j & 1)) v[u] = *reinterpret_cast<const fe *>(from + (size_t)j * step * D);
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++) {
+                const int j = min(k + u * WM, 63);
+                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), j));
+                acc = acc + v[u] * w;
+            }
+        }
+    }
+    for (int o = 1; o < 64; o <<= 1) sum = sum + __shfl_xor(sum, o);
+    if (WM > 1) {
+        __shared__ float s_acc[WM][D];
+        *reinterpret_cast<fe *>(&s_acc[wave][E * lane]) = acc;
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int w = 1; w < WM; w++) acc = acc + *reinterpret_cast<const fe *>(&s_acc[w][E * lane]);
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     float *o = a.out + (size_t)row * a.out_stride + (item - (size_t)row * n_head) * a.hd;
@@ -515,7 +544,8 @@ int launch(const Args &a, const AttnPlan &p, unsigned blocks, size_t items, hipS
     else attn_kernel<ES, D, 4><<<blocks, 256, 0, stream>>>(a);
     KH_HIP(hipGetLastError());
     if (p.splits > 1) {
-        merge_kernel<D><<<(unsigned)((items + 3) / 4), 256, 0, stream>>>(a);
+        if (p.splits > 8) merge_kernel<D, 4><<<(unsigned)items, 256, 0, stream>>>(a);
+        else merge_kernel<D, 1><<<(unsigned)((items + 3) / 4), 256, 0, stream>>>(a);
         KH_HIP(hipGetLastError());
     }
     return KH_OK;
@@ -592,8 +622,6 @@ int launch_attn(kh_ctx *ctx, const AttnCall &c, const AttnPlan &p) {
     a.window = c.window;
     a.sinks = c.sinks;
     a.scale = c.scale;
-    auto vec = [](const void *x, size_t stride) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && stride % 4 == 0; };
-    a.vec = vec(c.q, c.q_stride) && vec(c.out, c.out_stride);
     const unsigned blocks = (unsigned)((size_t)p.tiles * kv->n_kv_head * p.splits);
     if (kv->es == 4) return launch_d<4>(kv->d, a, p, blocks, items, ctx->stream);
     if (kv->es == 2) return launch_d<2>(kv->d, a, p, blocks, items, ctx->stream);
