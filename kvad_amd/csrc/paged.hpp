@@ -87,8 +87,7 @@ struct AttnCall {
 };
 // How a call is cut up, from its sizes alone.
 struct AttnPlan {
-    bool wide;         // a workgroup's four waves take 32 rows each (else they share 32 rows)
-    int tile_rows;     // rows x heads of a workgroup: 128 or 32
+    int tile_rows;     // rows x group of a workgroup: 8, 16, 32 or 128
     int tiles;         // row tiles, or a bound on them where rows are ragged
     int per;           // tiles of each sequence where rows are not
     int splits;        // of the positions, over workgroups

@@ -12,14 +12,18 @@
 // by lo is below the 22 bits).  The f32 matrix cores run at a sixteenth of the
 // f16 rate.
 //
-// A wave takes 32 rows of one KV head (query tokens x the head's group,
-// flattened: each K and V byte is read once for the whole group) and 32
-// positions at a time: S^T = K Q^T, then O^T += V^T P^T.  In the transposed
-// form a lane keeps one row's weights for the 16 positions that V's operand
-// wants of it, so the weights go from one product to the next in registers,
-// and K and V come from memory in operand order (paged_layout.hpp): there is
-// no LDS in the loop.  K of the next tile and V of this one are loaded while
-// the weights are computed.
+// A wave takes rows of one KV head (query tokens x the head's group, flattened:
+// each K and V byte is read once for the whole group) and 32 positions at a
+// time: S^T = K Q^T, then O^T += V^T P^T.  In the transposed form a lane keeps
+// one row's weights for the positions that V's operand wants of it, so the
+// weights go from one product to the next in registers, and K and V come from
+// memory in operand order (paged_layout.hpp): there is no LDS in the loop.  K of
+// the next tile and V of this one are loaded while the weights are computed.
+//
+// Two forms of the wave's work.  many_rows: 32 rows on 32x32x16 products, each
+// piece a product of its own.  few_rows: 8 or 16 rows on 16x16x32 products; with
+// 8, the pieces are the two halves of the 16 columns, so that one product does
+// both, and their sums meet in the scores (by a lane move) and at the end.
 #include <algorithm>
 
 #include "paged.hpp"
@@ -30,6 +34,7 @@ namespace {
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4v __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));  // rows may start at any float
 
@@ -55,7 +60,9 @@ struct Args {
     float scale;
 };
 
-__device__ __forceinline__ float shfl32(float v) { return __shfl_xor(v, 32); }
+__device__ __forceinline__ float shfl(float v, int x) { return __shfl_xor(v, x); }
+// the value 8 lanes on, in each row of 16
+__device__ __forceinline__ float other_half(float v) { return dev::dppf<0x128>(v); }
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 
 // hi + lo of two floats.  hi is cut off, not rounded: one instruction that the
@@ -87,7 +94,12 @@ __device__ __forceinline__ h8 codes8(unsigned a, unsigned b) {
 }
 
 __device__ __forceinline__ f16v mfma(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f4v mfma(h8 a, h8 b, f4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
+typedef unsigned u2v __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u2v load8(dev::rsrc_t r, unsigned voff, unsigned soff) {
+    return __builtin_bit_cast(u2v, __builtin_amdgcn_raw_buffer_load_b64(r, voff, soff, 0));
+}
 __device__ __forceinline__ int4 load16(dev::rsrc_t r, unsigned voff, unsigned soff) {
     return __builtin_bit_cast(int4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
 }
@@ -113,77 +125,184 @@ __device__ __forceinline__ Range range_of(int p_lo, int p_hi, int cap, int windo
     return r;
 }
 
-// ES bytes an element, D dims, WS waves that share 32 rows (1: each its own).
+// A wave's rows: those of sequence `seq` from row0 on (rows x group), nr of them
+// or more; its positions' tiles from t_at up to t_end, every WS'th.
+struct Job {
+    int seq, head, split, seq_row, first, row0, nr;
+    int p_lo, p_hi, t_at, t_end;
+    Range range;
+};
+
+__device__ __forceinline__ void find_range(const Args &a, Job &w) {
+    w.p_lo = w.first + w.row0 / a.group;
+    w.p_hi = w.first + (w.row0 + w.nr - 1) / a.group;
+    w.range = range_of(w.p_lo, w.p_hi, a.b.max_pages << a.page_shift, a.window, a.sinks);
+    w.t_at = 0;
+    w.t_end = w.range.n;
+    if (a.splits > 1) {
+        w.t_at = min(w.split * a.split_tiles, w.range.n);
+        // the last takes what is left: a longer sequence than max_len said
+        if (w.split < a.splits - 1) w.t_end = min(w.t_at + a.split_tiles, w.range.n);
+    }
+}
+
+// A tile's block and place.
+struct Where {
+    dev::rsrc_t r;
+    int start, in_page;
+    bool there;
+};
+struct Table {
+    const_i32 *pages;
+    __device__ Table(const Args &a, int seq)
+        // read through the scalar cache: no wait for it is a wait for K or V
+        : pages((const_i32 *)dev::uniform_ptr(a.b.pages + (size_t)seq * a.b.max_pages)) {}
+    __device__ __forceinline__ int page_of(const Args &a, const Job &w, int t) const {
+        return pages[w.range.start(t) >> a.page_shift];
+    }
+    __device__ __forceinline__ Where find(const Args &a, const Job &w, int t, int page) const {
+        Where x;
+        x.start = w.range.start(t);
+        x.there = page >= 0 && page < a.n_pages;
+        if (!x.there) page = 0;  // read, and hidden from every row
+        x.in_page = x.start & (a.page - 1);
+        x.r = dev::rsrc(dev::uniform_ptr(a.pool + ((size_t)page * a.n_kv + w.head) * a.block), a.block);
+        return x;
+    }
+};
+
+// The row of the flattened row `rr`, and where its query and its output start.
+struct Row {
+    int j, g, pos;
+    __device__ Row(const Args &a, const Job &w, int rr) {
+        j = rr / a.group;
+        g = rr - j * a.group;
+        pos = w.first + j;
+    }
+    __device__ const float *query(const Args &a, const Job &w) const {
+        return a.q + (size_t)(w.seq_row + j) * a.q_stride + (size_t)(w.head * a.group + g) * a.hd;
+    }
+};
+
+// Eight of a query's dims for each of NS products, the first of product s at
+// dim0(s); zeros past head_dim.  Returns the largest magnitude's bits.
+template <int NS, typename F>
+__device__ __forceinline__ int load_q(const float *x, int hd, F dim0, float (&v)[NS][8]) {
+    int amax = 0;
+#pragma unroll
+    for (int i = 0; i < NS; i++) {
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const int d = dim0(i) + 4 * c;
+            const float4u f = *reinterpret_cast<const float4u *>(x + min(d, hd - 4));
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[i][4 * c + e] = d < hd ? f[e] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) amax = max(amax, __builtin_bit_cast(int, v[i][e]) & 0x7fffffff);
+    }
+    return amax;
+}
+// The power of two that brings a query under 2^15, inverted, and the score, in
+// powers of two, of an accumulated product of 1.
+__device__ __forceinline__ float q_scale(int amax, float scale, float &rowf) {
+    const int e = min(max((amax >> 23) - 126 - 15, -126), 113);
+    rowf = (scale * 1.44269504088896341f) * __builtin_bit_cast(float, (127 + e) << 23);
+    return __builtin_bit_cast(float, (127 - e) << 23);
+}
+// 1 / 2^k from 2^k
+__device__ __forceinline__ float inv_pow2(float s) { return __builtin_bit_cast(float, 0x7f000000 - __builtin_bit_cast(int, s)); }
+
+// The exponent of the largest of V's scales, within what the weights can take.
+__device__ __forceinline__ float scale_exp(unsigned bits) { return (float)min(max((int)(bits >> 23) - 127, -90), 90); }
+
+// The sums of four waves over the same rows, column `col` of `cols` a lane, at
+// the largest reference: two and two and then one, through lds.  Wave 0 has them.
+template <int N>
+__device__ __forceinline__ void join_waves(float (&o)[N], float &ref, float &sum, int wave, int lane, int col, bool tells,
+                                           float *lds) {
+    constexpr int SN = N < 64 ? N : 64;  // registers a step
+    float(*s_ref)[32] = reinterpret_cast<float(*)[32]>(lds), (*s_sum)[32] = s_ref + 4;
+    float *s_acc = lds + 256;
+    if (tells) {
+        s_ref[wave][col] = ref;
+        s_sum[wave][col] = sum;
+    }
+    __syncthreads();
+    float all = s_ref[0][col];
+#pragma unroll
+    for (int w = 1; w < 4; w++) all = fmaxf(all, s_ref[w][col]);
+    const float f = exp2_(ref - all);
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) sum = sum + s_sum[w][col] * exp2_(s_ref[w][col] - all);
+    ref = all;
+#pragma unroll
+    for (int k = 0; k < N; k++) o[k] = o[k] * f;
+#pragma unroll
+    for (int half = 2; half >= 1; half /= 2) {
+#pragma unroll
+        for (int k0 = 0; k0 < N; k0 += SN) {
+            if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                for (int k = 0; k < SN; k++) s_acc[((wave - half) * SN + k) * 64 + lane] = o[k0 + k];
+            }
+            __syncthreads();
+            if (wave < half) {
+#pragma unroll
+                for (int k = 0; k < SN; k++) o[k0 + k] = o[k0 + k] + s_acc[(wave * SN + k) * 64 + lane];
+            }
+            __syncthreads();
+        }
+    }
+}
+// its LDS, in floats
+template <int N>
+constexpr int join_floats() { return 256 + 2 * (N < 64 ? N : 64) * 64; }
+
+// A lane's part of a row's result, four dims from dim(c) on in o[4 c ..]: into
+// the output, or beside the other splits'.
+template <int N, typename F>
+__device__ __forceinline__ void put_row(const Args &a, const Job &w, const Row &row, const float (&o)[N], float ref,
+                                        float sum, bool tells, int stored, F dim) {
+    const size_t r = (size_t)(w.seq_row + row.j);
+    const int q_head = w.head * a.group + row.g;
+    if (a.splits > 1) {
+        const size_t at = ((size_t)w.split * a.b.n_rows + r) * (a.n_kv * a.group) + q_head;
+        if (tells) reinterpret_cast<float2 *>(a.part_ml)[at] = make_float2(ref, sum);
+        if (sum == 0.0f) return;  // nothing seen here: the merge reads no values
+        float *to = a.part + at * stored;
+#pragma unroll
+        for (int c = 0; c < N / 4; c++)
+            *reinterpret_cast<float4 *>(to + dim(c)) = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+        return;
+    }
+    float *to = a.out + r * a.out_stride + (size_t)q_head * a.hd;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int c = 0; c < N / 4; c++)
+        if (dim(c) < a.hd)
+            *reinterpret_cast<float4u *>(to + dim(c)) =
+                float4u{o[4 * c] * inv, o[4 * c + 1] * inv, o[4 * c + 2] * inv, o[4 * c + 3] * inv};
+}
+
+// 32 rows; WS waves share them (1: each has its own).
 template <int ES, int D, int WS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ES == 4 || D == 256 ? 1 : 2)))
-void attn_kernel(Args a) {
+__device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float *lds) {
     constexpr int NK = D * ES / 32;  // loads of a lane for K
     constexpr int DT = D / 32;       // dim tiles of V
     constexpr int NS = D / 16;       // products over the dims
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int n = lane & 31, h = lane >> 5;
-    int rest = blockIdx.x;
-    const int head = rest % a.n_kv;
-    rest /= a.n_kv;
-    const int split = rest % a.splits, tile = rest / a.splits;
-    constexpr int ROWS = WS == 1 ? 128 : 32;
+    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+    find_range(a, w);
+    const Row row(a, w, w.row0 + min(n, w.nr - 1));
 
-    // the workgroup's rows: sequence s, rows row0 .. of its rows x group
-    int s, local, tiles;
-    if (a.b.row_start) {
-        auto at = [&](int i) {
-            const int r = first_row(a.b, i);
-            return (rows_of(a.b, i, r) * a.group + ROWS - 1) / ROWS;
-        };
-        if (!find_seq(a.b.n_seq, tile, at, s, local, tiles)) return;
-    } else {
-        tiles = a.tiles_per;
-        s = tile / tiles;
-        local = tile - s * tiles;
-    }
-    const int seq_row = first_row(a.b, s), seq_rows = rows_of(a.b, s, seq_row);
-    // later rows see more: they go first
-    const int row0 = (tiles - 1 - local) * ROWS + (WS == 1 ? 32 * wave : 0);
-    const int nr = min(seq_rows * a.group - row0, 32);
-    if (nr <= 0) return;
-    const int first = max(a.b.len[s], 0) - seq_rows;  // position of the sequence's first row
-    const int rr = row0 + min(n, nr - 1);
-    const int j = rr / a.group, g = rr - j * a.group;
-    const int pos = first + j;
-    const int p_lo = first + row0 / a.group, p_hi = first + (row0 + nr - 1) / a.group;
-    const int cap = a.b.max_pages << a.page_shift;
-    const Range range = range_of(p_lo, p_hi, cap, a.window, a.sinks);
-    int t_at = 0, t_end = range.n;
-    if (a.splits > 1) {
-        t_at = min(split * a.split_tiles, range.n);
-        t_end = split == a.splits - 1 ? range.n : min(t_at + a.split_tiles, range.n);
-    }
-    t_at += WS == 1 ? 0 : wave;
-
-    // q's rows, scaled to under 2^15 by a power of two, in two pieces
     h8 qh[NS], ql[NS];
-    float rowf;  // score, in powers of two, of an accumulated product
+    float rowf;
     {
-        const float *x = a.q + (size_t)(seq_row + j) * a.q_stride + (size_t)(head * a.group + g) * a.hd;
         float v[NS][8];
-        int amax = 0;
-#pragma unroll
-        for (int i = 0; i < NS; i++) {
-            const int d0 = k_dim(ES, i, h, 0);
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const int d = d0 + 4 * c;
-                const float4u f = *reinterpret_cast<const float4u *>(x + min(d, a.hd - 4));
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[i][4 * c + e] = d < a.hd ? f[e] : 0.0f;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; e++) amax = max(amax, __builtin_bit_cast(int, v[i][e]) & 0x7fffffff);
-        }
+        int amax = load_q<NS>(row.query(a, w), a.hd, [&](int i) { return k_dim(ES, i, h, 0); }, v);
         amax = max(amax, __shfl_xor(amax, 32));
-        const int e = min(max((amax >> 23) - 126 - 15, -126), 113);  // amax < 2^(e + 15)
-        const float inv = __builtin_bit_cast(float, (127 - e) << 23);
-        rowf = (a.scale * 1.44269504088896341f) * __builtin_bit_cast(float, (127 + e) << 23);
+        const float inv = q_scale(amax, a.scale, rowf);
 #pragma unroll
         for (int i = 0; i < NS; i++) {
 #pragma unroll
@@ -201,60 +320,44 @@ void attn_kernel(Args a) {
     const unsigned k_lane = (unsigned)(k_load_unit(ES, 0, h) * P + tile_pos(n)) * 16;
     const unsigned v_lane = (unsigned)(P * D * ES) + (unsigned)(v_load_unit(ES, 0, h) * D + n) * 16;
     const unsigned s_lane = (unsigned)(2 * P * D * ES) + 64 * h;
-    // read through the scalar cache: no wait for it is a wait for K or V
-    const_i32 *table = (const_i32 *)dev::uniform_ptr(a.b.pages + (size_t)s * a.b.max_pages);
-
-    struct Where {
-        dev::rsrc_t r;
-        int start, in_page;
-        bool there;
-    };
-    auto page_of = [&](int t) { return table[range.start(t) >> a.page_shift]; };
-    auto find = [&](int t, int page) {
-        Where w;
-        w.start = range.start(t);
-        w.there = page >= 0 && page < a.n_pages;
-        if (!w.there) page = 0;  // read, and hidden from every row
-        w.in_page = w.start & (P - 1);
-        w.r = dev::rsrc(dev::uniform_ptr(a.pool + ((size_t)page * a.n_kv + head) * a.block), a.block);
-        return w;
-    };
+    const Table table(a, w.seq);
     int4 kraw[NK], vraw[DT * ES];
     float4 ks[4], vs[4];
     float k_own = 0.0f;
-    auto load_ks = [&](const Where &w) {
+    auto load_ks = [&](const Where &x) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) ks[i] = __builtin_bit_cast(float4, load16(w.r, s_lane + 16 * i, 4 * w.in_page));
+        for (int i = 0; i < 4; i++) ks[i] = __builtin_bit_cast(float4, load16(x.r, s_lane + 16 * i, 4 * x.in_page));
     };
-    auto load_k = [&](const Where &w) {
+    auto load_k = [&](const Where &x) {
 #pragma unroll
         for (int i = 0; i < NK; i++) {
             const int unit = k_load_unit(ES, i, 0);
-            kraw[i] = load16(w.r, k_lane, (unsigned)(unit * P + w.in_page) * 16);
+            kraw[i] = load16(x.r, k_lane, (unsigned)(unit * P + x.in_page) * 16);
         }
-        if (ES == 4) k_own = dev::bldf(w.r, (unsigned)(2 * P * D * ES) + 4 * (w.in_page + tile_pos(n)));
+        if (ES == 4) k_own = dev::bldf(x.r, (unsigned)(2 * P * D * ES) + 4 * (x.in_page + tile_pos(n)));
     };
-    auto load_v = [&](const Where &w) {
+    auto load_v = [&](const Where &x) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            vs[i] = __builtin_bit_cast(float4, load16(w.r, s_lane + 16 * i, (unsigned)(4 * P + 4 * w.in_page)));
+            vs[i] = __builtin_bit_cast(float4, load16(x.r, s_lane + 16 * i, (unsigned)(4 * P + 4 * x.in_page)));
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
             for (int c = 0; c < ES; c++)
-                vraw[dt * ES + c] = load16(w.r, v_lane + (c * D + dt * 32) * 16, (unsigned)(w.in_page * D * ES));
+                vraw[dt * ES + c] = load16(x.r, v_lane + (c * D + dt * 32) * 16, (unsigned)(x.in_page * D * ES));
     };
 
+    const int t_at = w.t_at + (WS == 1 ? 0 : wave), t_end = w.t_end;
     Where here;
     if (t_at < t_end) {
-        here = find(t_at, page_of(t_at));
+        here = table.find(a, w, t_at, table.page_of(a, w, t_at));
         load_k(here);
         load_ks(here);
     }
     for (int t = t_at; t < t_end; t += WS) {
         // the next tile (this one again behind the last: the loads in flight
         // are the same at every wait, and none waits for more than its own)
-        const int next_t = min(t + WS, t_end - 1), next_page = page_of(next_t);
+        const int next_t = min(t + WS, t_end - 1), next_page = table.page_of(a, w, next_t);
         load_v(here);
         __builtin_amdgcn_sched_barrier(0);
 
@@ -277,8 +380,7 @@ void attn_kernel(Args a) {
                 sc = mfma(k, ql[i], sc);
             }
         } else {
-            // the position's scale, a power of two, inverted
-            const float inv = __builtin_bit_cast(float, 0x7f000000 - __builtin_bit_cast(int, k_own));
+            const float inv = inv_pow2(k_own);
 #pragma unroll
             for (int i = 0; i < NS; i++) {
                 const float4 x = __builtin_bit_cast(float4, kraw[(2 * i) % NK]), y = __builtin_bit_cast(float4, kraw[(2 * i + 1) % NK]);
@@ -291,10 +393,10 @@ void attn_kernel(Args a) {
             }
         }
         const int start = here.start;
-        const bool edge = !here.there || start + TILE - 1 > p_lo ||
-                          (a.window != INT32_MAX && start + TILE > a.sinks && start < p_hi - a.window + 1);
         const bool there = here.there;
-        here = find(next_t, next_page);
+        const bool edge = !there || start + TILE - 1 > w.p_lo ||
+                          (a.window != INT32_MAX && start + TILE > a.sinks && start < w.p_hi - a.window + 1);
+        here = table.find(a, w, next_t, next_page);
         load_k(here);
         __builtin_amdgcn_sched_barrier(0);
         float st[16];
@@ -313,18 +415,17 @@ void attn_kernel(Args a) {
         float inv_v[ES == 4 ? 16 : 1];
         if (ES == 4) {
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-                inv_v[i % (ES == 4 ? 16 : 1)] = __builtin_bit_cast(float, 0x7f000000 - __builtin_bit_cast(int, sv[i]));
+            for (int i = 0; i < 16; i++) inv_v[i % (ES == 4 ? 16 : 1)] = inv_pow2(sv[i]);
         }
         if (edge) {
             // positions ahead of the row, behind its window, or in no page:
             // no weight, and their rows' scales (NaN where a row is not
             // finite) out of everything
-            const int lo = a.window == INT32_MAX ? 0 : pos - a.window + 1;
+            const int lo = a.window == INT32_MAX ? 0 : row.pos - a.window + 1;
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const int at = start + 16 * h + i;
-                const bool seen = there && at <= pos && (at >= lo || at < a.sinks);
+                const bool seen = there && at <= row.pos && (at >= lo || at < a.sinks);
                 st[i] = seen ? st[i] : -__builtin_inff();
                 sv[i] = seen ? sv[i] : 0.0f;
             }
@@ -337,11 +438,10 @@ void attn_kernel(Args a) {
             vtop = max(vtop, __builtin_bit_cast(unsigned, sv[i]));
         }
         // the reference bounds weight times V's scale
-        const float vexp = (float)min(max((int)(vtop >> 23) - 127, -90), 90);
-        const float want = __builtin_fmaf(top, rowf, vexp);
+        const float want = __builtin_fmaf(top, rowf, scale_exp(vtop));
         if (__any(want > ref + SLACK)) {
             // each row for itself: what it gives does not hang on the rows beside it
-            const float all = fmaxf(want, shfl32(want));
+            const float all = fmaxf(want, shfl(want, 32));
             const float next = all > ref + SLACK ? all : ref;
             const float f = exp2_(ref - next);
             ref = next;
@@ -354,16 +454,16 @@ void attn_kernel(Args a) {
         const float shift = BASE - ref;
         h8 ph[2], pl[2];
         {
-            float w[16], part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float x[16], part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const float p = exp2_(__builtin_fmaf(st[i], rowf, shift));
                 part[i & 3] = part[i & 3] + p;
-                w[i] = p * sv[i];
+                x[i] = p * sv[i];
             }
             sum = sum + ((part[0] + part[1]) + (part[2] + part[3]));
-            split8(w, ph[0], pl[0]);
-            split8(w + 8, ph[1], pl[1]);
+            split8(x, ph[0], pl[0]);
+            split8(x + 8, ph[1], pl[1]);
         }
 
         // ---- O^T += V^T P^T ----
@@ -398,81 +498,301 @@ void attn_kernel(Args a) {
             }
         }
     }
-    sum = sum + shfl32(sum);
-
+    sum = sum + shfl(sum, 32);
+    float o[D / 2];
+#pragma unroll
+    for (int k = 0; k < D / 2; k++) o[k] = acc[k / 16][k % 16];
     if (WS > 1) {
-        // the four waves' sums, at the largest reference, two and then one
-        constexpr int SLAB = D < 128 ? D : 128, SN = SLAB / 2;  // dims and registers a step
-        __shared__ float s_acc[2][SN * 64];
-        __shared__ float s_ref[WS][32], s_sum[WS][32];
-        if (h == 0) {
-            s_ref[wave][n] = ref;
-            s_sum[wave][n] = sum;
-        }
-        __syncthreads();
-        float all = s_ref[0][n];
-#pragma unroll
-        for (int w = 1; w < WS; w++) all = fmaxf(all, s_ref[w][n]);
-        const float f = exp2_(ref - all);
-        sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WS; w++) sum = sum + s_sum[w][n] * exp2_(s_ref[w][n] - all);
-        ref = all;
-#pragma unroll
-        for (int half = WS / 2; half >= 1; half /= 2) {
-#pragma unroll
-            for (int d0 = 0; d0 < DT; d0 += SLAB / 32) {
-                if (wave >= half && wave < 2 * half) {
-#pragma unroll
-                    for (int k = 0; k < SN; k++) {
-                        const float v = acc[d0 + k / 16][k % 16];
-                        s_acc[wave - half][k * 64 + lane] = half == WS / 2 ? v * f : v;
-                    }
-                }
-                __syncthreads();
-                if (wave < half) {
-#pragma unroll
-                    for (int k = 0; k < SN; k++) {
-                        const float v = acc[d0 + k / 16][k % 16];
-                        acc[d0 + k / 16][k % 16] = (half == WS / 2 ? v * f : v) + s_acc[wave][k * 64 + lane];
-                    }
-                }
-                __syncthreads();
-            }
-        }
+        join_waves(o, ref, sum, wave, lane, n, h == 0, lds);
         if (wave > 0) return;
     }
-    if (n >= nr) return;
+    if (n >= w.nr) return;
+    put_row(a, w, row, o, ref, sum, h == 0, D, [&](int c) { return 32 * (c >> 2) + 8 * (c & 3) + 4 * h; });
+}
 
-    const size_t row = (size_t)(seq_row + j);
-    const int q_head = head * a.group + g;
-    if (a.splits > 1) {
-        const size_t at = ((size_t)split * a.b.n_rows + row) * (a.n_kv * a.group) + q_head;
-        if (h == 0) {
-            a.part_ml[2 * at] = ref;
-            a.part_ml[2 * at + 1] = sum;
+// ROWS rows, 8 or 16, shared by the workgroup's four waves.
+template <int ES, int D, int ROWS>
+__device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float *lds) {
+    constexpr bool PACKED = ROWS == 8;  // columns 0 .. 7 the high pieces, 8 .. 15 the low ones
+    constexpr int NK = D * ES / 64;     // loads of a lane for K, a block of 16 positions
+    constexpr int DB = D / 16;          // dim blocks of V
+    constexpr int NS = D / 32;          // products over the dims
+    constexpr int NV = ES == 4 ? 2 : 1; // loads of a lane for V, a dim block
+    const int lane = threadIdx.x & 63, n = lane & 15, z = lane >> 4;
+    const bool low = PACKED && n >= 8;
+    find_range(a, w);
+    const Row row(a, w, w.row0 + min(n & (ROWS - 1), w.nr - 1));
+
+    h8 qh[NS], ql[PACKED ? 1 : NS];
+    float rowf;
+    {
+        float v[NS][8];
+        int amax = load_q<NS>(row.query(a, w), a.hd, [&](int i) { return few_k_dim(ES, i, z, 0); }, v);
+        amax = max(amax, __shfl_xor(amax, 16));
+        amax = max(amax, __shfl_xor(amax, 32));
+        const float inv = q_scale(amax, a.scale, rowf);
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[i][k] = v[i][k] * inv;
+            h8 hi, lo;
+            split8(v[i], hi, lo);
+            qh[i] = low ? lo : hi;
+            if (!PACKED) ql[i % (PACKED ? 1 : NS)] = lo;
         }
-        if (sum == 0.0f) return;  // nothing seen here: the merge reads no values
-        float *o = a.part + at * D;
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                *reinterpret_cast<float4 *>(o + dt * 32 + 8 * i + 4 * h) =
-                    make_float4(acc[dt][4 * i], acc[dt][4 * i + 1], acc[dt][4 * i + 2], acc[dt][4 * i + 3]);
-        return;
     }
-    float *o = a.out + row * a.out_stride + (size_t)q_head * a.hd;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+
+    f4v acc[DB];
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++)
+    for (int i = 0; i < DB; i++) acc[i] = f4v{0.0f};
+    float ref = LOW, sum = 0.0f;
+
+    const int P = a.page;
+    const unsigned k_lane = (unsigned)(few_k_unit(ES, 0, z) * P + few_pos(n, 0)) * 16;
+    const unsigned v_lane = (unsigned)(P * D * ES) + 16 * n + few_v_off(ES, D, 0, z);
+    const unsigned s_lane = (unsigned)(2 * P * D * ES) + 32 * z;
+    const Table table(a, w.seq);
+    int4 kraw[2 * NK];
+    int4 vraw[ES == 1 ? 1 : DB * NV];
+    u2v vraw8[ES == 1 ? DB : 1];
+    float4 ks[2], vs[2];
+    float k_own[2] = {0.0f, 0.0f};
+    auto load_ks = [&](const Where &x) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int d = dt * 32 + 8 * i + 4 * h;
-            if (d >= a.hd) continue;
-            *reinterpret_cast<float4u *>(o + d) = float4u{acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv,
-                                                          acc[dt][4 * i + 2] * inv, acc[dt][4 * i + 3] * inv};
+        for (int i = 0; i < 2; i++) ks[i] = __builtin_bit_cast(float4, load16(x.r, s_lane + 16 * i, 4 * x.in_page));
+    };
+    auto load_k = [&](const Where &x) {
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+#pragma unroll
+            for (int i = 0; i < NK; i++) {
+                const int unit = few_k_unit(ES, i, 0);
+                kraw[b * NK + i] = load16(x.r, k_lane + 64 * b, (unsigned)(unit * P + x.in_page) * 16);
+            }
+            if (ES == 4) k_own[b] = dev::bldf(x.r, (unsigned)(2 * P * D * ES) + 4 * (x.in_page + few_pos(n, b)));
         }
+    };
+    auto load_v = [&](const Where &x) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            vs[i] = __builtin_bit_cast(float4, load16(x.r, s_lane + 16 * i, (unsigned)(4 * P + 4 * x.in_page)));
+#pragma unroll
+        for (int db = 0; db < DB; db++) {
+            if (ES == 1) {
+                vraw8[db % (ES == 1 ? DB : 1)] = load8(x.r, v_lane + 256 * db, (unsigned)(x.in_page * D * ES));
+            } else {
+#pragma unroll
+                for (int c = 0; c < NV; c++)
+                    vraw[(db * NV + c) % (ES == 1 ? 1 : DB * NV)] = load16(x.r, v_lane + 256 * db + c * D * 16, (unsigned)(x.in_page * D * ES));
+            }
+        }
+    };
+
+    const int t_at = w.t_at + wave, t_end = w.t_end;
+    Where here;
+    if (t_at < t_end) {
+        here = table.find(a, w, t_at, table.page_of(a, w, t_at));
+        load_k(here);
+        load_ks(here);
+    }
+    for (int t = t_at; t < t_end; t += 4) {
+        const int next_t = min(t + 4, t_end - 1), next_page = table.page_of(a, w, next_t);
+        load_v(here);
+        __builtin_amdgcn_sched_barrier(0);
+
+        // ---- scores: register 4 b + i is position start + 8 z + 4 b + i ----
+        f4v sc[2] = {f4v{0.0f}, f4v{0.0f}};
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            if (ES == 1) {
+#pragma unroll
+                for (int i = 0; i < NK; i++) {
+                    const int4 r = kraw[b * NK + i];
+                    const h8 k0 = codes8(r.x, r.y), k1 = codes8(r.z, r.w);
+                    sc[b] = mfma(k0, qh[2 * i % NS], sc[b]);
+                    if (!PACKED) sc[b] = mfma(k0, ql[2 * i % (PACKED ? 1 : NS)], sc[b]);
+                    sc[b] = mfma(k1, qh[(2 * i + 1) % NS], sc[b]);
+                    if (!PACKED) sc[b] = mfma(k1, ql[(2 * i + 1) % (PACKED ? 1 : NS)], sc[b]);
+                }
+            } else {
+                const float inv = ES == 4 ? inv_pow2(k_own[b]) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < NS; i++) {
+                    h8 kh, kl;
+                    if (ES == 2) {
+                        kh = __builtin_bit_cast(h8, kraw[(b * NK + i) % (2 * NK)]);
+                    } else {
+                        const float4 x = __builtin_bit_cast(float4, kraw[(b * NK + 2 * i) % (2 * NK)]);
+                        const float4 y = __builtin_bit_cast(float4, kraw[(b * NK + 2 * i + 1) % (2 * NK)]);
+                        const float f[8] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv, y.x * inv, y.y * inv, y.z * inv, y.w * inv};
+                        split8(f, kh, kl);
+                    }
+                    sc[b] = mfma(kh, qh[i], sc[b]);
+                    if (!PACKED) sc[b] = mfma(kh, ql[i % (PACKED ? 1 : NS)], sc[b]);
+                    if (ES == 4) sc[b] = mfma(kl, qh[i], sc[b]);
+                }
+            }
+        }
+        const int start = here.start;
+        const bool there = here.there;
+        const bool edge = !there || start + TILE - 1 > w.p_lo ||
+                          (a.window != INT32_MAX && start + TILE > a.sinks && start < w.p_hi - a.window + 1);
+        here = table.find(a, w, next_t, next_page);
+        load_k(here);
+        __builtin_amdgcn_sched_barrier(0);
+        float st[8];
+        {
+            const float all[8] = {ks[0].x, ks[0].y, ks[0].z, ks[0].w, ks[1].x, ks[1].y, ks[1].z, ks[1].w};
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                float s = sc[i >> 2][i & 3];
+                if (PACKED) s = s + other_half(s);
+                st[i] = s * all[i];
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load_ks(here);
+
+        // ---- weights ----
+        float sv[8] = {vs[0].x, vs[0].y, vs[0].z, vs[0].w, vs[1].x, vs[1].y, vs[1].z, vs[1].w};
+        float inv_v[ES == 4 ? 8 : 1];
+        if (ES == 4) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) inv_v[i % (ES == 4 ? 8 : 1)] = inv_pow2(sv[i]);
+        }
+        if (edge) {
+            const int lo = a.window == INT32_MAX ? 0 : row.pos - a.window + 1;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int at = start + 8 * z + i;
+                const bool seen = there && at <= row.pos && (at >= lo || at < a.sinks);
+                st[i] = seen ? st[i] : -__builtin_inff();
+                sv[i] = seen ? sv[i] : 0.0f;
+            }
+        }
+        float top = st[0];
+        unsigned vtop = __builtin_bit_cast(unsigned, sv[0]);
+#pragma unroll
+        for (int i = 1; i < 8; i++) {
+            top = fmaxf(top, st[i]);
+            vtop = max(vtop, __builtin_bit_cast(unsigned, sv[i]));
+        }
+        const float want = __builtin_fmaf(top, rowf, scale_exp(vtop));
+        if (__any(want > ref + SLACK)) {
+            float all = fmaxf(want, shfl(want, 16));
+            all = fmaxf(all, shfl(all, 32));
+            const float next = all > ref + SLACK ? all : ref;
+            const float f = exp2_(ref - next);
+            ref = next;
+            sum = sum * f;
+#pragma unroll
+            for (int db = 0; db < DB; db++) acc[db] = acc[db] * f;
+        }
+        const float shift = BASE - ref;
+        h8 ph, pl;
+        {
+            float x[8], part[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float p = exp2_(__builtin_fmaf(st[i], rowf, shift));
+                part[i & 1] = part[i & 1] + p;
+                x[i] = p * sv[i];
+            }
+            sum = sum + (part[0] + part[1]);
+            split8(x, ph, pl);
+            if (low) ph = pl;
+        }
+
+        // ---- O^T += V^T P^T ----
+#pragma unroll
+        for (int db = 0; db < DB; db++) {
+            h8 vh, vl;
+            if (ES == 1) {
+                const u2v r = vraw8[db % (ES == 1 ? DB : 1)];
+                vh = codes8(r.x, r.y);
+            } else if (ES == 2) {
+                vh = __builtin_bit_cast(h8, vraw[db % (ES == 1 ? 1 : DB * NV)]);
+            } else {
+                const float4 x = __builtin_bit_cast(float4, vraw[(2 * db) % (ES == 1 ? 1 : DB * NV)]);
+                const float4 y = __builtin_bit_cast(float4, vraw[(2 * db + 1) % (ES == 1 ? 1 : DB * NV)]);
+                float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    f[e] = __builtin_amdgcn_fmed3f(f[e] * inv_v[e % (ES == 4 ? 8 : 1)], -65504.0f, 65504.0f);
+                split8(f, vh, vl);
+            }
+            acc[db] = mfma(vh, ph, acc[db]);
+            if (!PACKED) acc[db] = mfma(vh, pl, acc[db]);
+            if (ES == 4) acc[db] = mfma(vl, ph, acc[db]);
+        }
+    }
+    sum = sum + shfl(sum, 16);
+    sum = sum + shfl(sum, 32);
+    float o[D / 4];
+#pragma unroll
+    for (int k = 0; k < D / 4; k++) {
+        o[k] = acc[k / 4][k % 4];
+        if (PACKED) o[k] = o[k] + other_half(o[k]);
+    }
+    join_waves(o, ref, sum, wave, lane, n, z == 0, lds);
+    if (wave > 0 || n >= w.nr) return;
+    put_row(a, w, row, o, ref, sum, z == 0, D, [&](int c) { return 16 * c + 4 * z; });
+}
+
+constexpr int FEW = 8;  // rows (x group) of a sequence that few_rows takes beside longer ones
+
+// Waves a SIMD by the registers that the loop holds: many_rows' 32 columns, or
+// few_rows' query, sums, K, V and the rest.
+constexpr int waves_for(int es, int d, int rows) {
+    if (rows > 16) return es == 4 || d == 256 ? 1 : 2;
+    const int regs = d / 8 * (rows / 8) + d / 4 + d * es / 4 + 60;
+    return regs <= 128 ? 4 : regs <= 172 ? 3 : regs <= 250 ? 2 : 1;
+}
+
+// ROWS 8 or 16: every sequence has at most so many rows.  32 or 128: any
+// number; a workgroup's waves share 32 rows, or take 32 of 128 each, and a
+// sequence of FEW rows or less goes to few_rows.
+template <int ES, int D, int ROWS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(waves_for(ES, D, ROWS))))
+void attn_kernel(Args a) {
+    constexpr int REGS = ROWS == 32 ? D / 2 : D / 4;  // of a lane, that join_waves takes
+    __shared__ __attribute__((aligned(16))) float lds[join_floats<REGS>()];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Job w;
+    int rest = blockIdx.x;
+    w.head = rest % a.n_kv;
+    rest /= a.n_kv;
+    w.split = rest % a.splits;
+    const int tile = rest / a.splits;
+    int local, tiles;
+    if (a.b.row_start) {
+        auto at = [&](int i) {
+            const int r = first_row(a.b, i);
+            return (rows_of(a.b, i, r) * a.group + ROWS - 1) / ROWS;
+        };
+        if (!find_seq(a.b.n_seq, tile, at, w.seq, local, tiles)) return;
+    } else {
+        tiles = a.tiles_per;
+        w.seq = tile / tiles;
+        local = tile - w.seq * tiles;
+    }
+    w.seq_row = first_row(a.b, w.seq);
+    const int seq_rows = rows_of(a.b, w.seq, w.seq_row);
+    w.first = max(a.b.len[w.seq], 0) - seq_rows;
+    // later rows see more: they go first
+    w.row0 = (tiles - 1 - local) * ROWS;
+    w.nr = min(seq_rows * a.group - w.row0, ROWS);
+    if constexpr (ROWS <= 16) {
+        few_rows<ES, D, ROWS>(a, w, wave, lds);
+    } else if (seq_rows * a.group <= FEW) {
+        few_rows<ES, D, FEW>(a, w, wave, lds);
+    } else if constexpr (ROWS == 32) {
+        many_rows<ES, D, 4>(a, w, wave, lds);
+    } else {
+        w.row0 += 32 * wave;
+        w.nr = min(w.nr - 32 * wave, 32);
+        if (w.nr > 0) many_rows<ES, D, 1>(a, w, wave, nullptr);
+    }
 }
 
 // The splits of a row and head, joined at the largest reference, by WM waves:
@@ -540,8 +860,10 @@ __global__ __launch_bounds__(256) void merge_kernel(Args a) {
 
 template <int ES, int D>
 int launch(const Args &a, const AttnPlan &p, unsigned blocks, size_t items, hipStream_t stream) {
-    if (p.wide) attn_kernel<ES, D, 1><<<blocks, 256, 0, stream>>>(a);
-    else attn_kernel<ES, D, 4><<<blocks, 256, 0, stream>>>(a);
+    if (p.tile_rows == 8) attn_kernel<ES, D, 8><<<blocks, 256, 0, stream>>>(a);
+    else if (p.tile_rows == 16) attn_kernel<ES, D, 16><<<blocks, 256, 0, stream>>>(a);
+    else if (p.tile_rows == 32) attn_kernel<ES, D, 32><<<blocks, 256, 0, stream>>>(a);
+    else attn_kernel<ES, D, 128><<<blocks, 256, 0, stream>>>(a);
     KH_HIP(hipGetLastError());
     if (p.splits > 1) {
         if (p.splits > 8) merge_kernel<D, 4><<<(unsigned)items, 256, 0, stream>>>(a);
@@ -569,9 +891,10 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
     auto tiles = [&](size_t rows) {
         return b.row_start ? (size_t)b.n_rows * group / rows + b.n_seq : b.n_seq * up_to((size_t)b.per * group, rows);
     };
-    // 128 rows a workgroup where that alone is two workgroups a CU
-    p.wide = tiles(128) * kv->n_kv_head >= 2 * (size_t)cu_count;
-    p.tile_rows = p.wide ? 128 : 32;
+    // few_rows where no sequence has more rows than it takes; else 128 rows a
+    // workgroup where that alone is two workgroups a CU, 32 where it is not
+    const size_t rows = b.row_start ? SIZE_MAX : (size_t)b.per * group;
+    p.tile_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : tiles(128) * kv->n_kv_head >= 2 * (size_t)cu_count ? 128 : 32;
     p.tiles = (int)tiles(p.tile_rows);
     p.per = b.row_start ? 0 : (int)up_to((size_t)b.per * group, p.tile_rows);
     // positions a tile of rows goes over, at most
@@ -581,10 +904,12 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
     const size_t blocks = (size_t)p.tiles * kv->n_kv_head;
     p.splits = 1;
     p.split_tiles = (int)pos_tiles;
-    if (!p.wide) {
-        // enough workgroups for two a CU twice over, 16 tiles to each at least
-        const size_t want = up_to(4 * (size_t)cu_count, blocks);
-        const size_t most = std::max<size_t>(1, pos_tiles / 16);
+    if (p.tile_rows < 128) {
+        // workgroups for two a CU (four of few_rows', which hold fewer
+        // registers), 8 tiles to each at least
+        static const int per_cu = env_int("KVAD_PAGED_PER_CU", 0), least = env_int("KVAD_PAGED_LEAST", 8);
+        const size_t want = up_to((per_cu ? per_cu : p.tile_rows <= 16 ? 4 : 2) * (size_t)cu_count, blocks);
+        const size_t most = std::max<size_t>(1, pos_tiles / least);
         size_t splits = std::min(std::min(want, most), (size_t)1024);
         const size_t each = 4 * (size_t)b.n_rows * n_head * (kv->d + 2);
         if (ws_max / each < splits) splits = ws_max / each;

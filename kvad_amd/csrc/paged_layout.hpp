@@ -61,5 +61,23 @@ KH_HD int k_dim(int es, int s, int h, int e) {
 // positions 16 h + U c + 0 .. U - 1 of the lane's dim.
 KH_HD int v_load_unit(int es, int c, int h) { return es * h + c; }
 
+// The same for the 16x16x32 product, which few rows take: lanes in quarters,
+// result register i of a lane in quarter z is row 4 z + i, and the tile's
+// positions are two blocks of 16.  Row m of block b is given position
+// few_pos(m, b): registers 4 b + i of quarter z are positions 8 z + 4 b + i, and
+// V's operand wants positions 8 z .. 8 z + 7 of that quarter.
+KH_HD int few_pos(int m, int b) { return 8 * (m >> 2) + 4 * b + (m & 3); }
+// K: load j (of d * es / 64) of a lane in quarter z; a product takes 32 dims, 8
+// a quarter.
+KH_HD int few_k_unit(int es, int j, int z) { return es == 4 ? 8 * (j >> 1) + 2 * z + (j & 1) : 4 * j + z; }
+KH_HD int few_k_dim(int es, int s, int z, int e) {
+    return es == 1 ? 64 * (s >> 1) + 16 * z + 8 * (s & 1) + e : 32 * s + 8 * z + e;
+}
+// V: the byte offset, from the tile's first unit of the dim, of positions
+// 8 z + 4 c .. (f32, two loads), 8 z .. (f16, one; i8, one of half a unit).
+KH_HD int few_v_off(int es, int d, int c, int z) {
+    return es == 4 ? (2 * z + c) * d * 16 : es == 2 ? z * d * 16 : (z >> 1) * d * 16 + 8 * (z & 1);
+}
+
 }  // namespace paged
 }  // namespace kh

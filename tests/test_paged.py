@@ -59,6 +59,29 @@ int main() {
                 MUST((size_t)off + 16 <= block);
                 for (int e = 0; e < U; e++) MUST(off + e * es == v_off(es, d, page, in_page + 16 * h + c * U + e, dt * 32 + n));
             }
+            // the 16x16x32 product's: row r16 of each block, quarter z
+            const int r16 = lane & 15, z = lane >> 4;
+            for (int b = 0; b < 2; b++) {
+                for (int i = 0; i < 4; i++) MUST(few_pos(4 * z + i, b) == 8 * z + 4 * b + i);
+                for (int j = 0; j < d * es / 64; j++) {
+                    const int off = (few_k_unit(es, 0, z) * page + few_pos(r16, b)) * 16 + (few_k_unit(es, j, 0) * page + in_page) * 16;
+                    MUST((size_t)off + 16 <= block);
+                    for (int e = 0; e < U; e++) {
+                        const int dim = few_k_dim(es, (j * U + e) / 8, z, (j * U + e) % 8);
+                        MUST(dim >= 0 && dim < d && off + e * es == k_off(es, page, in_page + few_pos(r16, b), dim));
+                    }
+                }
+            }
+            for (int db = 0; db < d / 16; db++) for (int c = 0; c < (es == 4 ? 2 : 1); c++) {
+                const int off = page * d * es + in_page * d * es + r16 * 16 + db * 256 + few_v_off(es, d, c, z);
+                const int bytes = es == 1 ? 8 : 16;
+                MUST((size_t)off + bytes <= block && off % bytes == 0);
+                for (int e = 0; e < bytes / es; e++) MUST(off + e * es == v_off(es, d, page, in_page + 8 * z + 4 * c + e, db * 16 + r16));
+            }
+            for (int i = 0; i < 2; i++) {
+                const int ks = 2 * page * d * es + 32 * z + 16 * i + 4 * in_page;
+                MUST(ks == k_scale_off(es, d, page, in_page + 8 * z + 4 * i) && (size_t)ks + 4 * page + 16 <= block);
+            }
             for (int i = 0; i < 4; i++) {
                 const int ks = 2 * page * d * es + 64 * h + 16 * i + 4 * in_page;
                 MUST(ks == k_scale_off(es, d, page, in_page + 16 * h + 4 * i));
