@@ -296,21 +296,6 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
     find_range(a, w);
     const Row row(a, w, w.row0 + min(n, w.nr - 1));
 
-    h8 qh[NS], ql[NS];
-    float rowf;
-    {
-        float v[NS][8];
-        int amax = load_q<NS>(row.query(a, w), a.hd, [&](int i) { return k_dim(ES, i, h, 0); }, v);
-        amax = max(amax, __shfl_xor(amax, 32));
-        const float inv = q_scale(amax, a.scale, rowf);
-#pragma unroll
-        for (int i = 0; i < NS; i++) {
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[i][k] = v[i][k] * inv;
-            split8(v[i], qh[i], ql[i]);
-        }
-    }
-
     f16v acc[DT];
 #pragma unroll
     for (int i = 0; i < DT; i++) acc[i] = f16v{0.0f};
@@ -348,12 +333,28 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
     };
 
     const int t_at = w.t_at + (WS == 1 ? 0 : wave), t_end = w.t_end;
-    Where here;
+    Where here;  // its K ahead of the query: one trip to memory, not two
     if (t_at < t_end) {
         here = table.find(a, w, t_at, table.page_of(a, w, t_at));
         load_k(here);
         load_ks(here);
     }
+
+    h8 qh[NS], ql[NS];
+    float rowf;
+    {
+        float v[NS][8];
+        int amax = load_q<NS>(row.query(a, w), a.hd, [&](int i) { return k_dim(ES, i, h, 0); }, v);
+        amax = max(amax, __shfl_xor(amax, 32));
+        const float inv = q_scale(amax, a.scale, rowf);
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[i][k] = v[i][k] * inv;
+            split8(v[i], qh[i], ql[i]);
+        }
+    }
+
     for (int t = t_at; t < t_end; t += WS) {
         // the next tile (this one again behind the last: the loads in flight
         // are the same at every wait, and none waits for more than its own)
@@ -523,25 +524,6 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
     find_range(a, w);
     const Row row(a, w, w.row0 + min(n & (ROWS - 1), w.nr - 1));
 
-    h8 qh[NS], ql[PACKED ? 1 : NS];
-    float rowf;
-    {
-        float v[NS][8];
-        int amax = load_q<NS>(row.query(a, w), a.hd, [&](int i) { return few_k_dim(ES, i, z, 0); }, v);
-        amax = max(amax, __shfl_xor(amax, 16));
-        amax = max(amax, __shfl_xor(amax, 32));
-        const float inv = q_scale(amax, a.scale, rowf);
-#pragma unroll
-        for (int i = 0; i < NS; i++) {
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[i][k] = v[i][k] * inv;
-            h8 hi, lo;
-            split8(v[i], hi, lo);
-            qh[i] = low ? lo : hi;
-            if (!PACKED) ql[i % (PACKED ? 1 : NS)] = lo;
-        }
-    }
-
     f4v acc[DB];
 #pragma unroll
     for (int i = 0; i < DB; i++) acc[i] = f4v{0.0f};
@@ -595,6 +577,26 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
         load_k(here);
         load_ks(here);
     }
+
+    h8 qh[NS], ql[PACKED ? 1 : NS];
+    float rowf;
+    {
+        float v[NS][8];
+        int amax = load_q<NS>(row.query(a, w), a.hd, [&](int i) { return few_k_dim(ES, i, z, 0); }, v);
+        amax = max(amax, __shfl_xor(amax, 16));
+        amax = max(amax, __shfl_xor(amax, 32));
+        const float inv = q_scale(amax, a.scale, rowf);
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[i][k] = v[i][k] * inv;
+            h8 hi, lo;
+            split8(v[i], hi, lo);
+            qh[i] = low ? lo : hi;
+            if (!PACKED) ql[i % (PACKED ? 1 : NS)] = lo;
+        }
+    }
+
     for (int t = t_at; t < t_end; t += 4) {
         const int next_t = min(t + 4, t_end - 1), next_page = table.page_of(a, w, next_t);
         load_v(here);
@@ -739,6 +741,9 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
     put_row(a, w, row, o, ref, sum, z == 0, D, [&](int c) { return 16 * c + 4 * z; });
 }
 
+// Bytes of a row of K up to which many_rows fits the registers; wider rows (f32,
+// 256 dims) are taken 16 at a time, however many there are.
+constexpr int MANY_MAX = 512;
 constexpr int FEW = 8;  // rows (x group) of a sequence that few_rows takes beside longer ones
 
 // Waves a SIMD by the registers that the loop holds: many_rows' 32 columns, or
@@ -749,9 +754,8 @@ constexpr int waves_for(int es, int d, int rows) {
     return regs <= 128 ? 4 : regs <= 172 ? 3 : regs <= 250 ? 2 : 1;
 }
 
-// ROWS 8 or 16: every sequence has at most so many rows.  32 or 128: any
-// number; a workgroup's waves share 32 rows, or take 32 of 128 each, and a
-// sequence of FEW rows or less goes to few_rows.
+// A workgroup takes ROWS rows: its waves share 8, 16 or 32, or take 32 of 128
+// each; with 32 and 128 a sequence of FEW rows or less goes to few_rows.
 template <int ES, int D, int ROWS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(waves_for(ES, D, ROWS))))
 void attn_kernel(Args a) {
@@ -810,37 +814,33 @@ __global__ __launch_bounds__(256) void merge_kernel(Args a) {
     const size_t step = (size_t)a.b.n_rows * n_head;
     const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + item;
     float all = LOW;
-    for (int i = lane; i < a.splits; i += 64) all = fmaxf(all, ml[i * step].x);
+    for (int i = lane; i < a.splits; i += 64) all = fmaxf(all, ml[i * step].x);  // of those that saw nothing LOW
     for (int o = 1; o < 64; o <<= 1) all = fmaxf(all, __shfl_xor(all, o));
-    constexpr int E = D / 64;
+    constexpr int E = D / 64, AT_ONCE = WM == 1 ? 8 : 16;  // loads in flight
     typedef float fe __attribute__((ext_vector_type(E)));
     fe acc = {};
     float sum = 0.0f;
     for (int base = 0; base < a.splits; base += 64) {
-        // a lane keeps a split's weight; a split that saw nothing has no values
-        const int i = base + lane;
+        const int n = min(a.splits - base, 64), i = base + lane;
         const float2 m = i < a.splits ? ml[i * step] : make_float2(LOW, 0.0f);
-        const float f = m.y == 0.0f ? 0.0f : exp2_(m.x - all);
-        sum = sum + (m.y == 0.0f ? 0.0f : m.y * f);
-        const unsigned long long has = __ballot(m.y != 0.0f);
         const float *from = a.part + ((size_t)base * step + item) * D + E * lane;
-        const int n = min(a.splits - base, 64);
-        constexpr int AT_ONCE = 4;
         for (int k = WM == 1 ? 0 : wave; k < n; k += WM * AT_ONCE) {
             fe v[AT_ONCE];
 #pragma unroll
-            for (int u = 0; u < AT_ONCE; u++) {
-                const int j = k + u * WM;
-                v[u] = fe{};
-                if (j < n && (has >> j & 1)) v[u] = *reinterpret_cast<const fe *>(from + (size_t)j * step * D);
-            }
+            for (int u = 0; u < AT_ONCE; u++)
+                v[u] = *reinterpret_cast<const fe *>(from + (size_t)min(k + u * WM, n - 1) * step * D);
+            // a lane keeps a split's weight; a split that saw nothing has no
+            // values, and what was read in their place counts for nothing
+            const float f = m.y == 0.0f ? 0.0f : exp2_(m.x - all);
+            const unsigned long long has = __ballot(m.y != 0.0f);
 #pragma unroll
             for (int u = 0; u < AT_ONCE; u++) {
-                const int j = min(k + u * WM, 63);
-                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), j));
-                acc = acc + v[u] * w;
+                const int j = k + u * WM;
+                if (j < n && (has >> j & 1))
+                    acc = acc + v[u] * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), j));
             }
         }
+        sum = sum + (m.y == 0.0f ? 0.0f : m.y * exp2_(m.x - all));
     }
     for (int o = 1; o < 64; o <<= 1) sum = sum + __shfl_xor(sum, o);
     if (WM > 1) {
@@ -862,8 +862,10 @@ template <int ES, int D>
 int launch(const Args &a, const AttnPlan &p, unsigned blocks, size_t items, hipStream_t stream) {
     if (p.tile_rows == 8) attn_kernel<ES, D, 8><<<blocks, 256, 0, stream>>>(a);
     else if (p.tile_rows == 16) attn_kernel<ES, D, 16><<<blocks, 256, 0, stream>>>(a);
-    else if (p.tile_rows == 32) attn_kernel<ES, D, 32><<<blocks, 256, 0, stream>>>(a);
-    else attn_kernel<ES, D, 128><<<blocks, 256, 0, stream>>>(a);
+    else if constexpr (ES * D <= MANY_MAX) {
+        if (p.tile_rows == 32) attn_kernel<ES, D, 32><<<blocks, 256, 0, stream>>>(a);
+        else attn_kernel<ES, D, 128><<<blocks, 256, 0, stream>>>(a);
+    }
     KH_HIP(hipGetLastError());
     if (p.splits > 1) {
         if (p.splits > 8) merge_kernel<D, 4><<<(unsigned)items, 256, 0, stream>>>(a);
@@ -894,7 +896,7 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
     // few_rows where no sequence has more rows than it takes; else 128 rows a
     // workgroup where that alone is two workgroups a CU, 32 where it is not
     const size_t rows = b.row_start ? SIZE_MAX : (size_t)b.per * group;
-    p.tile_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : tiles(128) * kv->n_kv_head >= 2 * (size_t)cu_count ? 128 : 32;
+    p.tile_rows = rows <= 8 ? 8 : rows <= 16 || kv->es * kv->d > MANY_MAX ? 16 : tiles(128) * kv->n_kv_head >= 2 * (size_t)cu_count ? 128 : 32;
     p.tiles = (int)tiles(p.tile_rows);
     p.per = b.row_start ? 0 : (int)up_to((size_t)b.per * group, p.tile_rows);
     // positions a tile of rows goes over, at most
@@ -905,10 +907,11 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
     p.splits = 1;
     p.split_tiles = (int)pos_tiles;
     if (p.tile_rows < 128) {
-        // workgroups for two a CU (four of few_rows', which hold fewer
-        // registers), 8 tiles to each at least
-        static const int per_cu = env_int("KVAD_PAGED_PER_CU", 0), least = env_int("KVAD_PAGED_LEAST", 8);
-        const size_t want = up_to((per_cu ? per_cu : p.tile_rows <= 16 ? 4 : 2) * (size_t)cu_count, blocks);
+        // A workgroup for each CU, if it gets that many tiles as take as long
+        // as joining the splits does (a launch, 4 us): 16, or fewer large ones.
+        static const int per_cu = env_int("KVAD_PAGED_PER_CU", 1), lst = env_int("KVAD_PAGED_LEAST", 0);
+        const size_t least = lst ? lst : std::min(std::max(2048 / (kv->es * kv->d), 4), 16);
+        const size_t want = up_to(per_cu * (size_t)cu_count, blocks);
         const size_t most = std::max<size_t>(1, pos_tiles / least);
         size_t splits = std::min(std::min(want, most), (size_t)1024);
         const size_t each = 4 * (size_t)b.n_rows * n_head * (kv->d + 2);
