@@ -4,7 +4,7 @@
 //
 // Both kernels move each byte once and are bound by HBM, or by the launch for
 // a few rows.  A workgroup takes the 32 positions of one layout tile, one KV
-// head, K or V: a cache unit of V runs over positions and a row over dims, so
+// head, K and V: a cache unit of V runs over positions and a row over dims, so
 // the tile is turned in LDS, and both sides go in whole lines: rows of
 // head_dim floats, and 16-byte units 32 to 256 in a run.
 #include <cmath>
@@ -24,33 +24,30 @@ struct MoveArgs {
     float *k, *v;              // rows in (push) or out (read)
     size_t k_stride, v_stride;
     size_t block;
-    int n_kv, hd, n_pages, page, page_shift, per, vec;
+    int n_kv, hd, n_pages, page, page_shift;
 };
 
 // A workgroup's tile: sequence, positions p0 .. p0 + 31 (the new rows' run
 // may start or end within), row of the run's first position.
 struct Tile {
-    int seq, p0, first, n, row0;
+    int p0, first, n, row0;
     char *block;   // null: a page out of range, or positions no table holds
 };
 
 __device__ __forceinline__ int tiles_of(int first, int n) { return n ? ((first + n - 1) >> 5) - (first >> 5) + 1 : 0; }
 
 __device__ __forceinline__ bool find_tile(const MoveArgs &a, int tile, int head, Tile &t) {
-    int local, count;
-    const Batch &b = a.b;
-    auto at = [&](int i) {
-        const int r = first_row(b, i), n = rows_of(b, i, r);
-        return tiles_of(max(b.len[i], 0) - n, n);
-    };
-    if (!find_seq(b.n_seq, tile, at, t.seq, local, count)) return false;
-    t.row0 = first_row(b, t.seq);
-    t.n = rows_of(b, t.seq, t.row0);
-    t.first = max(b.len[t.seq], 0) - t.n;
+    int seq, local, count;
+    Seq s;
+    auto tiles = [](const Seq &q) { return tiles_of(q.len - q.n, q.n); };
+    if (!find_seq(a.b, tile, tiles, seq, s, local, count)) return false;
+    t.row0 = s.row0;
+    t.n = s.n;
+    t.first = s.len - s.n;
     t.p0 = ((t.first >> 5) + local) * TILE;
     t.block = nullptr;
-    if (t.p0 >= 0 && (t.p0 >> a.page_shift) < b.max_pages) {
-        const int page = b.pages[(size_t)t.seq * b.max_pages + (t.p0 >> a.page_shift)];
+    if (t.p0 >= 0 && (t.p0 >> a.page_shift) < a.b.max_pages) {
+        const int page = a.b.pages[(size_t)seq * a.b.max_pages + (t.p0 >> a.page_shift)];
         if (page >= 0 && page < a.n_pages) t.block = a.pool + ((size_t)page * a.n_kv + head) * a.block;
     }
     return true;
@@ -100,6 +97,14 @@ __device__ __forceinline__ float value_of(const char *p) {
     return (float)((int)*reinterpret_cast<const uint8_t *>(p) - 128);
 }
 
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));  // rows may start at any float
+
+template <int ES>
+__device__ __forceinline__ unsigned get(const char *p) {
+    if (ES == 4) return *reinterpret_cast<const unsigned *>(p);
+    if (ES == 2) return *reinterpret_cast<const unsigned short *>(p);
+    return *reinterpret_cast<const uint8_t *>(p);
+}
 template <int ES>
 __device__ __forceinline__ void put(char *p, unsigned code) {
     if (ES == 4) *reinterpret_cast<unsigned *>(p) = code;
@@ -107,139 +112,136 @@ __device__ __forceinline__ void put(char *p, unsigned code) {
     if (ES == 1) *reinterpret_cast<uint8_t *>(p) = (uint8_t)code;
 }
 
+// A tile's rows of K and V, in flight together: the way to the tile (the batch's
+// arrays, then the page) is a few trips to memory, and both go it once.
 template <int ES, int D>
 __global__ __launch_bounds__(256) void push_kernel(MoveArgs a) {
     constexpr int U = 16 / ES, ROW = D * ES + 16;  // a row of codes in LDS, off the banks' period
-    __shared__ __attribute__((aligned(16))) char s_codes[TILE * ROW];
-    const int what = blockIdx.x & 1, rest = blockIdx.x >> 1;
-    const int head = rest % a.n_kv;
+    __shared__ __attribute__((aligned(16))) char s_codes[2][TILE * ROW];
+    const int head = blockIdx.x % a.n_kv;
     Tile t;
-    if (!find_tile(a, rest / a.n_kv, head, t) || !t.block) return;
-    const float *src = what ? a.v : a.k;
-    const size_t stride = what ? a.v_stride : a.k_stride;
+    if (!find_tile(a, blockIdx.x / a.n_kv, head, t) || !t.block) return;
     const int r = threadIdx.x >> 3, c = threadIdx.x & 7;
     const int row = t.p0 + r - t.first;  // of the sequence's new rows
     const bool mine = row >= 0 && row < t.n;
-    const float *x = src + (size_t)(t.row0 + (mine ? row : 0)) * stride + (size_t)head * a.hd;
-    float4 f[D / 32];
-    int amax = 0;
+    const size_t at = (size_t)(t.row0 + (mine ? row : 0));
+    const float *x[2] = {a.k + at * a.k_stride + (size_t)head * a.hd, a.v + at * a.v_stride + (size_t)head * a.hd};
+    float4u f[2][D / 32];
 #pragma unroll
-    for (int j = 0; j < D / 32; j++) {
-        const int d = 4 * c + 32 * j;
-        f[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (mine && d < a.hd)
-            f[j] = a.vec ? *reinterpret_cast<const float4 *>(x + d) : make_float4(x[d], x[d + 1], x[d + 2], x[d + 3]);
-        // magnitudes compare as their bits do, NaN above infinity
-        const float m[4] = {f[j].x, f[j].y, f[j].z, f[j].w};
-        for (int i = 0; i < 4; i++) amax = max(amax, __builtin_bit_cast(int, m[i]) & 0x7fffffff);
-    }
-    for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor(amax, o));
-    float inv;
-    const float scale = scale_of<ES>(amax, inv);
-    const bool finite = amax < 0x7f800000;
+    for (int what = 0; what < 2; what++)
+#pragma unroll
+        for (int j = 0; j < D / 32; j++) {
+            const int d = 4 * c + 32 * j;
+            f[what][j] = float4u{0.0f, 0.0f, 0.0f, 0.0f};
+            if (mine && d < a.hd) f[what][j] = *reinterpret_cast<const float4u *>(x[what] + d);
+        }
     const int in_page = t.p0 & (a.page - 1);
-    if (mine && c == 0) {
-        const int off = what ? v_scale_off(ES, D, a.page, in_page + r) : k_scale_off(ES, D, a.page, in_page + r);
-        *reinterpret_cast<float *>(t.block + off) = scale;
-    }
 #pragma unroll
-    for (int j = 0; j < D / 32; j++) {
-        char *p = s_codes + r * ROW + (4 * c + 32 * j) * ES;
-        put<ES>(p, code_of<ES>(f[j].x, inv, finite));
-        put<ES>(p + ES, code_of<ES>(f[j].y, inv, finite));
-        put<ES>(p + 2 * ES, code_of<ES>(f[j].z, inv, finite));
-        put<ES>(p + 3 * ES, code_of<ES>(f[j].w, inv, finite));
+    for (int what = 0; what < 2; what++) {
+        int amax = 0;
+#pragma unroll
+        for (int j = 0; j < D / 32; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)  // magnitudes compare as their bits do, NaN above infinity
+                amax = max(amax, __builtin_bit_cast(int, (float)f[what][j][e]) & 0x7fffffff);
+        for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor(amax, o));
+        float inv;
+        const float scale = scale_of<ES>(amax, inv);
+        const bool finite = amax < 0x7f800000;
+        if (mine && c == 0) {
+            const int off = what ? v_scale_off(ES, D, a.page, in_page + r) : k_scale_off(ES, D, a.page, in_page + r);
+            *reinterpret_cast<float *>(t.block + off) = scale;
+        }
+#pragma unroll
+        for (int j = 0; j < D / 32; j++) {
+            char *p = s_codes[what] + r * ROW + (4 * c + 32 * j) * ES;
+            unsigned w[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = code_of<ES>(f[what][j][e], inv, finite);
+            if (ES == 4) *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (ES == 2) *reinterpret_cast<uint2 *>(p) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+            if (ES == 1) *reinterpret_cast<unsigned *>(p) = w[0] | w[1] << 8 | w[2] << 16 | w[3] << 24;
+        }
     }
     __syncthreads();
     const int lo = max(t.first - t.p0, 0), hi = min(t.first + t.n - t.p0, TILE);  // the tile's new positions
-    if (!what) {
-        for (int i = threadIdx.x; i < TILE * D / U; i += 256) {
-            const int pos = i & 31, unit = i >> 5;
-            if (pos >= lo && pos < hi)
-                *reinterpret_cast<int4 *>(t.block + k_off(ES, a.page, in_page + pos, unit * U)) =
-                    *reinterpret_cast<const int4 *>(s_codes + pos * ROW + unit * 16);
-        }
-        return;
+    for (int i = threadIdx.x; i < TILE * D / U; i += 256) {
+        const int pos = i & 31, unit = i >> 5;
+        if (pos >= lo && pos < hi)
+            *reinterpret_cast<int4 *>(t.block + k_off(ES, a.page, in_page + pos, unit * U)) =
+                *reinterpret_cast<const int4 *>(s_codes[0] + pos * ROW + unit * 16);
     }
     for (int i = threadIdx.x; i < TILE / U * D; i += 256) {
         const int dim = i % D, p = i / D * U;  // the unit's first position
         char *dst = t.block + v_off(ES, D, a.page, in_page + p, dim);
-        const char *from = s_codes + p * ROW + dim * ES;
+        const char *from = s_codes[1] + p * ROW + dim * ES;
         if (p >= lo && p + U <= hi) {
             unsigned w[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int e = 0; e < U; e++) {
-                unsigned code;
-                if (ES == 4) code = *reinterpret_cast<const unsigned *>(from + e * ROW);
-                else if (ES == 2) code = *reinterpret_cast<const unsigned short *>(from + e * ROW);
-                else code = *reinterpret_cast<const uint8_t *>(from + e * ROW);
-                w[e * ES / 4] |= code << (e * ES % 4 * 8);
-            }
+            for (int e = 0; e < U; e++) w[e * ES / 4] |= get<ES>(from + e * ROW) << (e * ES % 4 * 8);
             *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
             // a run that starts or ends within the unit: its own elements
             // alone, the others may be another call's
-            for (int e = max(lo - p, 0); e < min(hi - p, U); e++) {
-                if (ES == 4) put<4>(dst + e * ES, *reinterpret_cast<const unsigned *>(from + e * ROW));
-                if (ES == 2) put<2>(dst + e * ES, *reinterpret_cast<const unsigned short *>(from + e * ROW));
-                if (ES == 1) put<1>(dst + e * ES, *reinterpret_cast<const uint8_t *>(from + e * ROW));
-            }
+            for (int e = max(lo - p, 0); e < min(hi - p, U); e++) put<ES>(dst + e * ES, get<ES>(from + e * ROW));
         }
     }
 }
 
 template <int ES, int D>
 __global__ __launch_bounds__(256) void read_kernel(MoveArgs a) {
-    constexpr int U = 16 / ES, ROW = D * ES + 16;
-    __shared__ __attribute__((aligned(16))) char s_codes[TILE * ROW];
-    __shared__ float s_scale[TILE];
-    const int what = blockIdx.x & 1, rest = blockIdx.x >> 1;
-    const int head = rest % a.n_kv;
+    constexpr int U = 16 / ES, ROW = D * ES + 16, N = TILE * D / U / 256 ? TILE * D / U / 256 : 1;
+    __shared__ __attribute__((aligned(16))) char s_codes[2][TILE * ROW];
+    __shared__ float s_scale[2][TILE];
+    const int head = blockIdx.x % a.n_kv;
     Tile t;
-    if (!find_tile(a, rest / a.n_kv, head, t)) return;
+    if (!find_tile(a, blockIdx.x / a.n_kv, head, t)) return;
     const int in_page = t.p0 & (a.page - 1);
     if (t.block) {
-        if (threadIdx.x < TILE) {
-            const int off = what ? v_scale_off(ES, D, a.page, in_page) : k_scale_off(ES, D, a.page, in_page);
-            s_scale[threadIdx.x] = reinterpret_cast<const float *>(t.block + off)[threadIdx.x];
-        }
-        for (int i = threadIdx.x; i < TILE * D / U; i += 256) {
-            if (!what) {
-                const int pos = i & 31, unit = i >> 5;
-                *reinterpret_cast<int4 *>(s_codes + pos * ROW + unit * 16) =
-                    *reinterpret_cast<const int4 *>(t.block + k_off(ES, a.page, in_page + pos, unit * U));
-            } else {
-                const int dim = i % D, p = i / D * U;
-                const uint4 u = *reinterpret_cast<const uint4 *>(t.block + v_off(ES, D, a.page, in_page + p, dim));
-                const unsigned w[4] = {u.x, u.y, u.z, u.w};
-                char *to = s_codes + p * ROW + dim * ES;
+        int4 u[2][N];
+        const bool some = TILE * D / U >= 256 || threadIdx.x < TILE * D / U;
 #pragma unroll
-                for (int e = 0; e < U; e++) put<ES>(to + e * ROW, w[e * ES / 4] >> (e * ES % 4 * 8));
-            }
+        for (int j = 0; j < N; j++) {
+            const int i = threadIdx.x + 256 * j, pos = i & 31, unit = i >> 5, dim = i % D, p = i / D * U;
+            if (!some) break;
+            u[0][j] = *reinterpret_cast<const int4 *>(t.block + k_off(ES, a.page, in_page + pos, unit * U));
+            u[1][j] = *reinterpret_cast<const int4 *>(t.block + v_off(ES, D, a.page, in_page + p, dim));
+        }
+        if (threadIdx.x < 2 * TILE) {
+            const int what = threadIdx.x >> 5, pos = threadIdx.x & 31;
+            const int off = what ? v_scale_off(ES, D, a.page, in_page + pos) : k_scale_off(ES, D, a.page, in_page + pos);
+            s_scale[what][pos] = *reinterpret_cast<const float *>(t.block + off);
+        }
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const int i = threadIdx.x + 256 * j, pos = i & 31, unit = i >> 5, dim = i % D, p = i / D * U;
+            if (!some) break;
+            *reinterpret_cast<int4 *>(s_codes[0] + pos * ROW + unit * 16) = u[0][j];
+            const unsigned w[4] = {(unsigned)u[1][j].x, (unsigned)u[1][j].y, (unsigned)u[1][j].z, (unsigned)u[1][j].w};
+#pragma unroll
+            for (int e = 0; e < U; e++) put<ES>(s_codes[1] + (p + e) * ROW + dim * ES, w[e * ES / 4] >> (e * ES % 4 * 8));
         }
     }
     __syncthreads();
-    float *dst = what ? a.v : a.k;
-    const size_t stride = what ? a.v_stride : a.k_stride;
-    const int chunks = a.hd / 4;
-    for (int i = threadIdx.x; i < TILE * chunks; i += 256) {
-        const int pos = i / chunks, d = 4 * (i - pos * chunks);
-        const int row = t.p0 + pos - t.first;
-        if (row < 0 || row >= t.n) continue;
-        float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (t.block) {
-            const char *p = s_codes + pos * ROW + d * ES;
-            const float s = s_scale[pos];
-            for (int e = 0; e < 4; e++) {
-                f[e] = value_of<ES>(p + e * ES);
-                if (ES != 4) f[e] = f[e] * s;  // f32 rows are kept as they came
+    // a run of 8 lanes takes a row, 32 dims a step
+    const int r = threadIdx.x >> 3, c = threadIdx.x & 7, row = t.p0 + r - t.first;
+    if (row < 0 || row >= t.n) return;
+#pragma unroll
+    for (int what = 0; what < 2; what++) {
+        float *y = (what ? a.v + (size_t)(t.row0 + row) * a.v_stride : a.k + (size_t)(t.row0 + row) * a.k_stride) +
+                   (size_t)head * a.hd;
+        const float s = t.block ? s_scale[what][r] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < D / 32; j++) {
+            const int d = 4 * c + 32 * j;
+            if (d >= a.hd) break;
+            float4u f = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (t.block) {
+                const char *p = s_codes[what] + r * ROW + d * ES;
+#pragma unroll
+                for (int e = 0; e < 4; e++) f[e] = ES == 4 ? value_of<ES>(p + e * ES) : value_of<ES>(p + e * ES) * s;
             }
-        }
-        float *y = dst + (size_t)(t.row0 + row) * stride + (size_t)head * a.hd + d;
-        if (a.vec) {
-            *reinterpret_cast<float4 *>(y) = make_float4(f[0], f[1], f[2], f[3]);
-        } else {
-            for (int e = 0; e < 4; e++) y[e] = f[e];
+            *reinterpret_cast<float4u *>(y + d) = f;
         }
     }
 }
@@ -257,7 +259,6 @@ void launch_move_d(bool push, int d, const MoveArgs &a, unsigned blocks, hipStre
     else launch_move<ES, 256>(push, a, blocks, stream);
 }
 
-bool aligned16(const void *p, size_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 4 == 0; }
 bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
 // Grid dimensions are counted in threads, in 32 bits.
@@ -302,11 +303,10 @@ int move(const kh_paged *kv, size_t layer, const kh_batch *b, float *k, size_t k
     a.n_pages = (int)kv->n_pages;
     a.page = kv->page;
     a.page_shift = kv->page_shift;
-    a.vec = aligned16(k, a.k_stride) && aligned16(v, a.v_stride);
     // n rows lie in at most n / 32 + 2 tiles, and in at most n
     const size_t bound = b->n_rows / TILE + 2 * b->n_seq;
     const size_t tiles = bound < b->n_rows ? bound : b->n_rows;
-    const size_t blocks = tiles * kv->n_kv_head * 2;
+    const size_t blocks = tiles * kv->n_kv_head;
     if (blocks > MAX_BLOCKS) return fail(KH_EINVAL, "kh_paged: too many rows for one launch");
     hipStream_t s = kv->ctx->stream;
     if (kv->es == 4) launch_move_d<4>(push, kv->d, a, (unsigned)blocks, s);

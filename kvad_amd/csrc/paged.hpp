@@ -41,16 +41,30 @@ __device__ __forceinline__ int rows_of(const Batch &b, int i, int first) {
     return b.row_start ? clampi(b.row_start[i + 1], first, b.n_rows) - first : b.per;
 }
 
-// Which sequence the tile'th tile of the batch belongs to, sequence i having
-// count(i) of them: a wave takes the running sum of 64 counts at a time.
-// False past the last tile.  `tile` is the same in every lane; so are the
-// results.
+// A sequence's rows and length, as a lane of find_seq holds them.
+struct Seq {
+    int row0, n, len;
+    __device__ __forceinline__ void load(const Batch &b, int i) {
+        row0 = first_row(b, i);
+        n = rows_of(b, i, row0);
+        len = max(b.len[i], 0);
+    }
+    __device__ __forceinline__ Seq of_lane(int l) const {
+        return Seq{__builtin_amdgcn_readlane(row0, l), __builtin_amdgcn_readlane(n, l), __builtin_amdgcn_readlane(len, l)};
+    }
+};
+
+// Which sequence the tile'th tile of the batch belongs to, a sequence s having
+// count(s) of them: a wave takes the running sum of 64 counts at a time.  False
+// past the last tile.  `tile` is the same in every lane; so are the results:
+// the sequence's number, the tile's among its own, how many those are.
 template <typename F>
-__device__ __forceinline__ bool find_seq(int n_seq, int tile, F count, int &seq, int &local, int &n) {
+__device__ __forceinline__ bool find_seq(const Batch &b, int tile, F count, int &seq, Seq &s, int &local, int &n) {
     const int lane = threadIdx.x & 63;
-    for (int base = 0; base < n_seq; base += 64) {
-        const int i = base + lane;
-        const int c = i < n_seq ? count(i) : 0;
+    for (int base = 0; base < b.n_seq; base += 64) {
+        Seq mine{0, 0, 0};
+        if (base + lane < b.n_seq) mine.load(b, base + lane);
+        const int c = count(mine);
         int sum = c;
         for (int o = 1; o < 64; o <<= 1) {
             const int up = __shfl_up(sum, o);
@@ -62,6 +76,7 @@ __device__ __forceinline__ bool find_seq(int n_seq, int tile, F count, int &seq,
             n = __builtin_amdgcn_readlane(c, l);
             local = tile - (__builtin_amdgcn_readlane(sum, l) - n);
             seq = base + l;
+            s = mine.of_lane(l);
             return true;
         }
         tile -= all;

@@ -768,21 +768,20 @@ void attn_kernel(Args a) {
     rest /= a.n_kv;
     w.split = rest % a.splits;
     const int tile = rest / a.splits;
+    Seq seq;
     int local, tiles;
     if (a.b.row_start) {
-        auto at = [&](int i) {
-            const int r = first_row(a.b, i);
-            return (rows_of(a.b, i, r) * a.group + ROWS - 1) / ROWS;
-        };
-        if (!find_seq(a.b.n_seq, tile, at, w.seq, local, tiles)) return;
+        auto count = [&](const Seq &q) { return (q.n * a.group + ROWS - 1) / ROWS; };
+        if (!find_seq(a.b, tile, count, w.seq, seq, local, tiles)) return;
     } else {
         tiles = a.tiles_per;
         w.seq = tile / tiles;
         local = tile - w.seq * tiles;
+        seq.load(a.b, w.seq);
     }
-    w.seq_row = first_row(a.b, w.seq);
-    const int seq_rows = rows_of(a.b, w.seq, w.seq_row);
-    w.first = max(a.b.len[w.seq], 0) - seq_rows;
+    w.seq_row = seq.row0;
+    const int seq_rows = seq.n;
+    w.first = seq.len - seq_rows;
     // later rows see more: they go first
     w.row0 = (tiles - 1 - local) * ROWS;
     w.nr = min(seq_rows * a.group - w.row0, ROWS);
