@@ -265,20 +265,21 @@ bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0;
 constexpr size_t MAX_BLOCKS = ((size_t)1 << 32) / 256 - 1;
 constexpr size_t MAX_POSITIONS = (size_t)1 << 30;
 
+int refuse(const char *what, const char *why) { return fail(KH_EINVAL, std::string(what) + ": " + why); }
+
 // What can be checked of a batch without reading its arrays.
 int check_batch(const kh_paged *kv, size_t layer, const kh_batch *b, const char *what) {
-    const std::string w = what;
-    if (!kv || !b) return fail(KH_EINVAL, w + ": null argument");
-    if (layer >= kv->n_layer) return fail(KH_EINVAL, w + ": no such layer");
+    if (!kv || !b) return refuse(what, "null argument");
+    if (layer >= kv->n_layer) return refuse(what, "no such layer");
     if (b->n_rows == 0) return KH_OK;
-    if (b->n_seq == 0) return fail(KH_EINVAL, w + ": rows, but no sequences");
-    if (!b->len || !b->pages || b->max_pages == 0) return fail(KH_EINVAL, w + ": a batch needs lengths and pages");
+    if (b->n_seq == 0) return refuse(what, "rows, but no sequences");
+    if (!b->len || !b->pages || b->max_pages == 0) return refuse(what, "a batch needs lengths and pages");
     if (!aligned4(b->len) || !aligned4(b->pages) || !aligned4(b->row_start))
-        return fail(KH_EINVAL, w + ": the batch's arrays are of 32-bit integers");
+        return refuse(what, "the batch's arrays are of 32-bit integers");
     if (!b->row_start && b->n_rows % b->n_seq)
-        return fail(KH_EINVAL, w + ": without row_start every sequence has as many rows");
+        return refuse(what, "without row_start every sequence has as many rows");
     if (b->n_rows > MAX_POSITIONS || b->n_seq > MAX_POSITIONS || b->max_pages > MAX_POSITIONS / kv->page)
-        return fail(KH_EINVAL, w + ": more than 2^30 rows, sequences or positions of a sequence");
+        return refuse(what, "more than 2^30 rows, sequences or positions of a sequence");
     return KH_OK;
 }
 
@@ -319,11 +320,11 @@ int move(const kh_paged *kv, size_t layer, const kh_batch *b, float *k, size_t k
 int check_move(const kh_paged *kv, size_t layer, const kh_batch *b, const float *k, size_t k_stride, const float *v,
                size_t v_stride, const char *what) {
     if (int rc = check_batch(kv, layer, b, what)) return rc;
-    if (b->n_rows && (!k || !v)) return fail(KH_EINVAL, std::string(what) + ": null argument");
-    if (!aligned4(k) || !aligned4(v)) return fail(KH_EINVAL, std::string(what) + ": rows are of 32-bit floats");
+    if (b->n_rows && (!k || !v)) return refuse(what, "null argument");
+    if (!aligned4(k) || !aligned4(v)) return refuse(what, "rows are of 32-bit floats");
     const size_t width = kv->n_kv_head * kv->head_dim;
     if ((k_stride && k_stride < width) || (v_stride && v_stride < width))
-        return fail(KH_EINVAL, std::string(what) + ": a stride is less than a row");
+        return refuse(what, "a stride is less than a row");
     return KH_OK;
 }
 
@@ -570,19 +571,18 @@ namespace {
 
 int check_attend(const kh_paged *kv, size_t layer, const kh_batch *b, size_t n_head, const float *q, size_t q_stride,
                  float scale, const float *out, size_t out_stride, const char *what) {
-    const std::string w = what;
     if (int rc = check_batch(kv, layer, b, what)) return rc;
     if (n_head == 0 || n_head > 65536 || n_head % kv->n_kv_head)
-        return fail(KH_EINVAL, w + ": n_head is a multiple of the cache's KV heads, at most 65536");
-    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(KH_EINVAL, w + ": scale is positive and finite");
+        return refuse(what, "n_head is a multiple of the cache's KV heads, at most 65536");
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return refuse(what, "scale is positive and finite");
     if (b->n_rows == 0) return KH_OK;
-    if (!q || !out) return fail(KH_EINVAL, w + ": null argument");
-    if (!aligned4(q) || !aligned4(out)) return fail(KH_EINVAL, w + ": rows are of 32-bit floats");
+    if (!q || !out) return refuse(what, "null argument");
+    if (!aligned4(q) || !aligned4(out)) return refuse(what, "rows are of 32-bit floats");
     const size_t width = n_head * kv->head_dim;
     if ((q_stride && q_stride < width) || (out_stride && out_stride < width))
-        return fail(KH_EINVAL, w + ": a stride is less than a row");
+        return refuse(what, "a stride is less than a row");
     if (b->n_rows * (n_head / kv->n_kv_head) > MAX_POSITIONS)
-        return fail(KH_EINVAL, w + ": more than 2^30 rows of a KV head");
+        return refuse(what, "more than 2^30 rows of a KV head");
     return KH_OK;
 }
 

@@ -906,12 +906,16 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
     p.splits = 1;
     p.split_tiles = (int)pos_tiles;
     if (p.tile_rows < 128) {
-        // A workgroup for each CU, if it gets that many tiles as take as long
-        // as joining the splits does (a launch, 4 us): 16, or fewer large ones.
-        static const int per_cu = env_int("KVAD_PAGED_PER_CU", 1), lst = env_int("KVAD_PAGED_LEAST", 0);
+        // few_rows, bound by memory: a workgroup for each CU.  many_rows, bound
+        // by its arithmetic, of which one wave keeps half a SIMD busy: two, and
+        // none more, which would wait for a place.  Each gets as many tiles as
+        // take as long as joining the splits does (a launch, 4 us): 16, or
+        // fewer large ones.
+        static const int knob = env_int("KVAD_PAGED_PER_CU", 0), lst = env_int("KVAD_PAGED_LEAST", 0);
         const size_t least = lst ? lst : std::min(std::max(2048 / (kv->es * kv->d), 4), 16);
-        const size_t want = up_to(per_cu * (size_t)cu_count, blocks);
-        const size_t most = std::max<size_t>(1, pos_tiles / least);
+        const size_t cus = (size_t)cu_count;
+        const size_t want = knob ? up_to(knob * cus, blocks) : p.tile_rows <= 16 ? up_to(cus, blocks) : 2 * cus / blocks;
+        const size_t most = pos_tiles / least;
         size_t splits = std::min(std::min(want, most), (size_t)1024);
         const size_t each = 4 * (size_t)b.n_rows * n_head * (kv->d + 2);
         if (ws_max / each < splits) splits = ws_max / each;
