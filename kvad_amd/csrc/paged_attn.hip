@@ -25,6 +25,7 @@
 // 8, the pieces are the two halves of the 16 columns, so that one product does
 // both, and their sums meet in the scores (by a lane move) and at the end.
 #include <algorithm>
+#include <utility>
 
 #include "paged.hpp"
 
@@ -61,6 +62,35 @@ struct Args {
 };
 
 __device__ __forceinline__ float shfl(float v, int x) { return __shfl_xor(v, x); }
+// lane I's value, in each row of 16.  Not where lanes are switched off: one that
+// is gives zero.
+template <int I>
+__device__ __forceinline__ float of_lane(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x150 + I, 0xf, 0xf, true));
+}
+// the largest of each row of 16, in all of its lanes
+__device__ __forceinline__ unsigned row_max(unsigned v) {
+    v = max(v, (unsigned)dev::dpp<dev::DPP_XOR1>((int)v));
+    v = max(v, (unsigned)dev::dpp<dev::DPP_XOR2>((int)v));
+    v = max(v, (unsigned)dev::dpp<dev::DPP_HALF_MIRROR>((int)v));
+    return max(v, (unsigned)dev::dpp<dev::DPP_MIRROR>((int)v));
+}
+// f(0), f(1), ... f(N - 1), each with its number as a constant
+template <typename F, int... I>
+__device__ __forceinline__ void each_(F f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F f) {
+    each_(f, std::make_integer_sequence<int, N>{});
+}
+// A row of V that is not finite, by its scale: no part of any sum, and NaN as
+// a score, so that only rows that see it are NaN.
+__device__ __forceinline__ void only_finite(float &v_scale, float &k_scale) {
+    const bool finite = (__builtin_bit_cast(int, v_scale) & 0x7fffffff) < 0x7f800000;
+    k_scale = finite ? k_scale : __builtin_bit_cast(float, NAN_BITS);
+    v_scale = finite ? v_scale : 0.0f;
+}
 // the value 8 lanes on, in each row of 16
 __device__ __forceinline__ float other_half(float v) { return dev::dppf<0x128>(v); }
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
@@ -99,6 +129,9 @@ __device__ __forceinline__ f4v mfma(h8 a, h8 b, f4v c) { return __builtin_amdgcn
 typedef unsigned u2v __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ u2v load8(dev::rsrc_t r, unsigned voff, unsigned soff) {
     return __builtin_bit_cast(u2v, __builtin_amdgcn_raw_buffer_load_b64(r, voff, soff, 0));
+}
+__device__ __forceinline__ float load4(dev::rsrc_t r, unsigned voff, unsigned soff) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, voff, soff, 0));
 }
 __device__ __forceinline__ int4 load16(dev::rsrc_t r, unsigned voff, unsigned soff) {
     return __builtin_bit_cast(int4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
@@ -304,14 +337,15 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
     const int P = a.page;
     const unsigned k_lane = (unsigned)(k_load_unit(ES, 0, h) * P + tile_pos(n)) * 16;
     const unsigned v_lane = (unsigned)(P * D * ES) + (unsigned)(v_load_unit(ES, 0, h) * D + n) * 16;
-    const unsigned s_lane = (unsigned)(2 * P * D * ES) + 64 * h;
+    // scales: a lane holds position 16 h + lane % 16's, and takes the others of
+    // its half from the lanes beside it
+    const unsigned s_lane = (unsigned)(2 * P * D * ES) + 4 * (16 * h + (lane & 15));
     const Table table(a, w.seq);
     int4 kraw[NK], vraw[DT * ES];
-    float4 ks[4], vs[4];
-    float k_own = 0.0f;
-    auto load_ks = [&](const Where &x) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) ks[i] = __builtin_bit_cast(float4, load16(x.r, s_lane + 16 * i, 4 * x.in_page));
+    float ks, vs, k_own = 0.0f;
+    auto load_s = [&](const Where &x) {
+        ks = load4(x.r, s_lane, 4 * x.in_page);
+        vs = load4(x.r, s_lane, 4 * P + 4 * x.in_page);
     };
     auto load_k = [&](const Where &x) {
 #pragma unroll
@@ -322,9 +356,6 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
         if (ES == 4) k_own = dev::bldf(x.r, (unsigned)(2 * P * D * ES) + 4 * (x.in_page + tile_pos(n)));
     };
     auto load_v = [&](const Where &x) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            vs[i] = __builtin_bit_cast(float4, load16(x.r, s_lane + 16 * i, (unsigned)(4 * P + 4 * x.in_page)));
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -337,7 +368,7 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
     if (t_at < t_end) {
         here = table.find(a, w, t_at, table.page_of(a, w, t_at));
         load_k(here);
-        load_ks(here);
+        load_s(here);
     }
 
     h8 qh[NS], ql[NS];
@@ -400,44 +431,33 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
         here = table.find(a, w, next_t, next_page);
         load_k(here);
         __builtin_amdgcn_sched_barrier(0);
+        only_finite(vs, ks);
         float st[16];
-        {
-            const float all[16] = {ks[0].x, ks[0].y, ks[0].z, ks[0].w, ks[1].x, ks[1].y, ks[1].z, ks[1].w,
-                                   ks[2].x, ks[2].y, ks[2].z, ks[2].w, ks[3].x, ks[3].y, ks[3].z, ks[3].w};
-#pragma unroll
-            for (int i = 0; i < 16; i++) st[i] = sc[i] * all[i];
-        }
+        each<16>([&](auto i) { st[i] = sc[i.value] * of_lane<i>(ks); });
+        const float sv = vs, v_inv = ES == 4 ? inv_pow2(vs) : 0.0f;
         __builtin_amdgcn_sched_barrier(0);
-        load_ks(here);
+        load_s(here);
 
         // ---- weights ----
-        float sv[16] = {vs[0].x, vs[0].y, vs[0].z, vs[0].w, vs[1].x, vs[1].y, vs[1].z, vs[1].w,
-                        vs[2].x, vs[2].y, vs[2].z, vs[2].w, vs[3].x, vs[3].y, vs[3].z, vs[3].w};
-        float inv_v[ES == 4 ? 16 : 1];
-        if (ES == 4) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) inv_v[i % (ES == 4 ? 16 : 1)] = inv_pow2(sv[i]);
-        }
+        unsigned vtop;
         if (edge) {
             // positions ahead of the row, behind its window, or in no page:
-            // no weight, and their rows' scales (NaN where a row is not
-            // finite) out of everything
+            // no weight, and no say in the reference
             const int lo = a.window == INT32_MAX ? 0 : row.pos - a.window + 1;
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
+            vtop = 0;
+            each<16>([&](auto i) {
                 const int at = start + 16 * h + i;
-                const bool seen = there && at <= row.pos && (at >= lo || at < a.sinks);
+                const bool seen = there & (at <= row.pos) & ((at >= lo) | (at < a.sinks));
+                const unsigned bits = __builtin_bit_cast(unsigned, of_lane<i>(sv));  // with every lane at work
                 st[i] = seen ? st[i] : -__builtin_inff();
-                sv[i] = seen ? sv[i] : 0.0f;
-            }
+                vtop = max(vtop, seen ? bits : 0u);
+            });
+        } else {
+            vtop = row_max(__builtin_bit_cast(unsigned, sv));
         }
         float top = st[0];
-        unsigned vtop = __builtin_bit_cast(unsigned, sv[0]);
 #pragma unroll
-        for (int i = 1; i < 16; i++) {
-            top = fmaxf(top, st[i]);
-            vtop = max(vtop, __builtin_bit_cast(unsigned, sv[i]));
-        }
+        for (int i = 1; i < 16; i++) top = fmaxf(top, st[i]);
         // the reference bounds weight times V's scale
         const float want = __builtin_fmaf(top, rowf, scale_exp(vtop));
         if (__any(want > ref + SLACK)) {
@@ -456,48 +476,42 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
         h8 ph[2], pl[2];
         {
             float x[16], part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
+            each<16>([&](auto i) {
                 const float p = exp2_(__builtin_fmaf(st[i], rowf, shift));
                 part[i & 3] = part[i & 3] + p;
-                x[i] = p * sv[i];
-            }
+                x[i] = p * of_lane<i>(sv);
+            });
             sum = sum + ((part[0] + part[1]) + (part[2] + part[3]));
             split8(x, ph[0], pl[0]);
             split8(x + 8, ph[1], pl[1]);
         }
 
         // ---- O^T += V^T P^T ----
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++) {
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                if (ES == 1) {
-                    const int4 r = vraw[dt * ES];
-                    const h8 v = c ? codes8(r.z, r.w) : codes8(r.x, r.y);
-                    acc[dt] = mfma(v, ph[c], acc[dt]);
-                    acc[dt] = mfma(v, pl[c], acc[dt]);
-                } else if (ES == 2) {
-                    const h8 v = __builtin_bit_cast(h8, vraw[dt * ES + c % ES]);
-                    acc[dt] = mfma(v, ph[c], acc[dt]);
-                    acc[dt] = mfma(v, pl[c], acc[dt]);
-                } else {
-                    const float4 x = __builtin_bit_cast(float4, vraw[dt * ES + (2 * c) % ES]);
-                    const float4 y = __builtin_bit_cast(float4, vraw[dt * ES + (2 * c + 1) % ES]);
-                    float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-                    // a row that is not finite leaves finite pieces here: its
-                    // scale alone says so, to the rows that see it
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        f[e] = __builtin_amdgcn_fmed3f(f[e] * inv_v[(8 * c + e) % (ES == 4 ? 16 : 1)], -65504.0f, 65504.0f);
-                    h8 vh, vl;
-                    split8(f, vh, vl);
-                    acc[dt] = mfma(vh, ph[c], acc[dt]);
-                    acc[dt] = mfma(vh, pl[c], acc[dt]);
-                    acc[dt] = mfma(vl, ph[c], acc[dt]);
-                }
+        each<DT * 2>([&](auto k) {
+            constexpr int dt = k / 2, c = k % 2;
+            if constexpr (ES == 1) {
+                const int4 r = vraw[dt];
+                const h8 v = c ? codes8(r.z, r.w) : codes8(r.x, r.y);
+                acc[dt] = mfma(v, ph[c], acc[dt]);
+                acc[dt] = mfma(v, pl[c], acc[dt]);
+            } else if constexpr (ES == 2) {
+                const h8 v = __builtin_bit_cast(h8, vraw[dt * ES + c]);
+                acc[dt] = mfma(v, ph[c], acc[dt]);
+                acc[dt] = mfma(v, pl[c], acc[dt]);
+            } else {
+                const f4v x = __builtin_bit_cast(f4v, vraw[dt * ES + 2 * c]), y = __builtin_bit_cast(f4v, vraw[dt * ES + 2 * c + 1]);
+                // a row that is not finite leaves finite pieces here
+                float f[8];
+                each<8>([&](auto e) {
+                    f[e] = __builtin_amdgcn_fmed3f((e < 4 ? x[e & 3] : y[e & 3]) * of_lane<8 * c + e>(v_inv), -65504.0f, 65504.0f);
+                });
+                h8 vh, vl;
+                split8(f, vh, vl);
+                acc[dt] = mfma(vh, ph[c], acc[dt]);
+                acc[dt] = mfma(vh, pl[c], acc[dt]);
+                acc[dt] = mfma(vl, ph[c], acc[dt]);
             }
-        }
+        });
     }
     sum = sum + shfl(sum, 32);
     float o[D / 2];
@@ -532,16 +546,15 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
     const int P = a.page;
     const unsigned k_lane = (unsigned)(few_k_unit(ES, 0, z) * P + few_pos(n, 0)) * 16;
     const unsigned v_lane = (unsigned)(P * D * ES) + 16 * n + few_v_off(ES, D, 0, z);
-    const unsigned s_lane = (unsigned)(2 * P * D * ES) + 32 * z;
+    const unsigned s_lane = (unsigned)(2 * P * D * ES) + 4 * (8 * z + (lane & 7));  // scales: position 8 z + lane % 8's
     const Table table(a, w.seq);
     int4 kraw[2 * NK];
     int4 vraw[ES == 1 ? 1 : DB * NV];
     u2v vraw8[ES == 1 ? DB : 1];
-    float4 ks[2], vs[2];
-    float k_own[2] = {0.0f, 0.0f};
-    auto load_ks = [&](const Where &x) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) ks[i] = __builtin_bit_cast(float4, load16(x.r, s_lane + 16 * i, 4 * x.in_page));
+    float ks, vs, k_own[2] = {0.0f, 0.0f};
+    auto load_s = [&](const Where &x) {
+        ks = load4(x.r, s_lane, 4 * x.in_page);
+        vs = load4(x.r, s_lane, 4 * P + 4 * x.in_page);
     };
     auto load_k = [&](const Where &x) {
 #pragma unroll
@@ -555,9 +568,6 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
         }
     };
     auto load_v = [&](const Where &x) {
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            vs[i] = __builtin_bit_cast(float4, load16(x.r, s_lane + 16 * i, (unsigned)(4 * P + 4 * x.in_page)));
 #pragma unroll
         for (int db = 0; db < DB; db++) {
             if (ES == 1) {
@@ -575,7 +585,7 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
     if (t_at < t_end) {
         here = table.find(a, w, t_at, table.page_of(a, w, t_at));
         load_k(here);
-        load_ks(here);
+        load_s(here);
     }
 
     h8 qh[NS], ql[PACKED ? 1 : NS];
@@ -642,43 +652,35 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
         here = table.find(a, w, next_t, next_page);
         load_k(here);
         __builtin_amdgcn_sched_barrier(0);
+        only_finite(vs, ks);
         float st[8];
-        {
-            const float all[8] = {ks[0].x, ks[0].y, ks[0].z, ks[0].w, ks[1].x, ks[1].y, ks[1].z, ks[1].w};
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                float s = sc[i >> 2][i & 3];
-                if (PACKED) s = s + other_half(s);
-                st[i] = s * all[i];
-            }
-        }
+        each<8>([&](auto i) {
+            float s = sc[i >> 2][i.value & 3];
+            if (PACKED) s = s + other_half(s);
+            st[i] = s * of_lane<i>(ks);
+        });
+        const float sv = vs, v_inv = ES == 4 ? inv_pow2(vs) : 0.0f;
         __builtin_amdgcn_sched_barrier(0);
-        load_ks(here);
+        load_s(here);
 
         // ---- weights ----
-        float sv[8] = {vs[0].x, vs[0].y, vs[0].z, vs[0].w, vs[1].x, vs[1].y, vs[1].z, vs[1].w};
-        float inv_v[ES == 4 ? 8 : 1];
-        if (ES == 4) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) inv_v[i % (ES == 4 ? 8 : 1)] = inv_pow2(sv[i]);
-        }
+        unsigned vtop;
         if (edge) {
             const int lo = a.window == INT32_MAX ? 0 : row.pos - a.window + 1;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
+            vtop = 0;
+            each<8>([&](auto i) {
                 const int at = start + 8 * z + i;
-                const bool seen = there && at <= row.pos && (at >= lo || at < a.sinks);
+                const bool seen = there & (at <= row.pos) & ((at >= lo) | (at < a.sinks));
+                const unsigned bits = __builtin_bit_cast(unsigned, of_lane<i>(sv));  // with every lane at work
                 st[i] = seen ? st[i] : -__builtin_inff();
-                sv[i] = seen ? sv[i] : 0.0f;
-            }
+                vtop = max(vtop, seen ? bits : 0u);
+            });
+        } else {
+            vtop = row_max(__builtin_bit_cast(unsigned, sv));
         }
         float top = st[0];
-        unsigned vtop = __builtin_bit_cast(unsigned, sv[0]);
 #pragma unroll
-        for (int i = 1; i < 8; i++) {
-            top = fmaxf(top, st[i]);
-            vtop = max(vtop, __builtin_bit_cast(unsigned, sv[i]));
-        }
+        for (int i = 1; i < 8; i++) top = fmaxf(top, st[i]);
         const float want = __builtin_fmaf(top, rowf, scale_exp(vtop));
         if (__any(want > ref + SLACK)) {
             float all = fmaxf(want, shfl(want, 16));
@@ -694,12 +696,11 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
         h8 ph, pl;
         {
             float x[8], part[2] = {0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
+            each<8>([&](auto i) {
                 const float p = exp2_(__builtin_fmaf(st[i], rowf, shift));
                 part[i & 1] = part[i & 1] + p;
-                x[i] = p * sv[i];
-            }
+                x[i] = p * of_lane<i>(sv);
+            });
             sum = sum + (part[0] + part[1]);
             split8(x, ph, pl);
             if (low) ph = pl;
@@ -715,12 +716,12 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
             } else if (ES == 2) {
                 vh = __builtin_bit_cast(h8, vraw[db % (ES == 1 ? 1 : DB * NV)]);
             } else {
-                const float4 x = __builtin_bit_cast(float4, vraw[(2 * db) % (ES == 1 ? 1 : DB * NV)]);
-                const float4 y = __builtin_bit_cast(float4, vraw[(2 * db + 1) % (ES == 1 ? 1 : DB * NV)]);
-                float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    f[e] = __builtin_amdgcn_fmed3f(f[e] * inv_v[e % (ES == 4 ? 8 : 1)], -65504.0f, 65504.0f);
+                const f4v x = __builtin_bit_cast(f4v, vraw[(2 * db) % (ES == 1 ? 1 : DB * NV)]);
+                const f4v y = __builtin_bit_cast(f4v, vraw[(2 * db + 1) % (ES == 1 ? 1 : DB * NV)]);
+                float f[8];
+                each<8>([&](auto e) {
+                    f[e] = __builtin_amdgcn_fmed3f((e < 4 ? x[e & 3] : y[e & 3]) * of_lane<e>(v_inv), -65504.0f, 65504.0f);
+                });
                 split8(f, vh, vl);
             }
             acc[db] = mfma(vh, ph, acc[db]);
