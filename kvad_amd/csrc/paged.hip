@@ -626,7 +626,7 @@ int attend(AttnCall &c, void *ws, size_t ws_bytes) {
         }
     }
     const size_t blocks = (size_t)p.tiles * c.kv->n_kv_head * p.splits;
-    if (blocks > MAX_BLOCKS || (size_t)c.b.n_rows * c.n_head > MAX_BLOCKS)
+    if (blocks > MAX_BLOCKS || (p.splits > 1 && (size_t)c.b.n_rows * c.n_head > MAX_BLOCKS))
         return fail(KH_EINVAL, "kh_paged_attend: too many rows for one launch");
     return launch_attn(ctx, c, p);
 }

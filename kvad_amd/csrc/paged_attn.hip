@@ -893,31 +893,46 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
     auto tiles = [&](size_t rows) {
         return b.row_start ? (size_t)b.n_rows * group / rows + b.n_seq : b.n_seq * up_to((size_t)b.per * group, rows);
     };
-    // few_rows where no sequence has more rows than it takes; else 128 rows a
-    // workgroup where that alone is two workgroups a CU, 32 where it is not
-    const size_t rows = b.row_start ? SIZE_MAX : (size_t)b.per * group;
-    p.tile_rows = rows <= 8 ? 8 : rows <= 16 || kv->es * kv->d > MANY_MAX ? 16 : tiles(128) * kv->n_kv_head >= 2 * (size_t)cu_count ? 128 : 32;
+    // positions a tile of rows goes over, at most, in tiles
+    auto over = [&](size_t rows) {
+        size_t span = max_len;
+        if (window != INT32_MAX) span = std::min(span, (size_t)window + rows / group + sinks + 2 * TILE);
+        return up_to(span, TILE);
+    };
+    // few_rows where no sequence has more rows than it takes, where many_rows
+    // does not fit the registers, and for small calls: up to 16 tiles a CU its
+    // way in and out is shorter (100 new tokens of 32 heads of 128, f16: 5.9 us
+    // against 8.5; 100 behind 3000, i8: 31 against 28).  Else 128 rows a
+    // workgroup where that alone fills the device (a 6000-token prompt, f16:
+    // 646 us against 694 with 32), 32 where it does not.
+    const size_t rows = b.row_start ? SIZE_MAX : (size_t)b.per * group, cus = (size_t)cu_count;
+    const size_t resident = cus * waves_for(kv->es, kv->d, 32);  // many_rows' workgroups
+    const bool small = tiles(16) * kv->n_kv_head * over(16) <= 16 * cus;
+    p.tile_rows = rows <= 8                                            ? 8
+                  : rows <= 16 || small || kv->es * kv->d > MANY_MAX ? 16
+                  : tiles(128) * kv->n_kv_head >= resident           ? 128
+                                                                     : 32;
+    // for experiments, and for tests of each form: any form does any call
+    const int form = env_int("KVAD_PAGED_TILE", 0);
+    if (form == 8 || form == 16 || ((form == 32 || form == 128) && kv->es * kv->d <= MANY_MAX)) p.tile_rows = form;
     p.tiles = (int)tiles(p.tile_rows);
     p.per = b.row_start ? 0 : (int)up_to((size_t)b.per * group, p.tile_rows);
-    // positions a tile of rows goes over, at most
-    size_t span = max_len;
-    if (window != INT32_MAX) span = std::min(span, (size_t)window + p.tile_rows / group + sinks + 2 * TILE);
-    const size_t pos_tiles = up_to(span, TILE);
+    const size_t pos_tiles = over(p.tile_rows);
     const size_t blocks = (size_t)p.tiles * kv->n_kv_head;
     p.splits = 1;
     p.split_tiles = (int)pos_tiles;
     if (p.tile_rows < 128) {
         // few_rows, bound by memory: a workgroup for each CU.  many_rows, bound
-        // by its arithmetic, of which one wave keeps half a SIMD busy: two, and
-        // none more, which would wait for a place.  Each gets as many tiles as
+        // by its arithmetic, of which one wave keeps half a SIMD busy: as many
+        // as are at work at once, and none that would wait for a place.  Each gets as many tiles as
         // take as long as joining the splits does (a launch, 4 us): 16, or
         // fewer large ones.
-        static const int knob = env_int("KVAD_PAGED_PER_CU", 0), lst = env_int("KVAD_PAGED_LEAST", 0);
-        const size_t least = lst ? lst : std::min(std::max(2048 / (kv->es * kv->d), 4), 16);
-        const size_t cus = (size_t)cu_count;
-        const size_t want = knob ? up_to(knob * cus, blocks) : p.tile_rows <= 16 ? up_to(cus, blocks) : 2 * cus / blocks;
+        const size_t least = std::min(std::max(2048 / (kv->es * kv->d), 4), 16);
+        const size_t want = p.tile_rows <= 16 ? up_to(cus, blocks) : resident / blocks;
         const size_t most = pos_tiles / least;
-        size_t splits = std::min(std::min(want, most), (size_t)1024);
+        const int forced = env_int("KVAD_PAGED_SPLITS", 0);
+        size_t splits = forced > 0 ? std::min((size_t)forced, pos_tiles) : std::min(want, most);
+        splits = std::min(splits, (size_t)1024);
         const size_t each = 4 * (size_t)b.n_rows * n_head * (kv->d + 2);
         if (ws_max / each < splits) splits = ws_max / each;
         if (splits > 1) {

@@ -134,6 +134,14 @@ class Pool:
         return got
 
 
+@pytest.fixture(params=["rule", "8", "16", "32", "128"])
+def form(request, monkeypatch):
+    """Each form of the attention kernel, by the rows a workgroup takes."""
+    if request.param != "rule":
+        monkeypatch.setenv("KVAD_PAGED_TILE", request.param)
+    return request.param
+
+
 # ---- rows ----------------------------------------------------------------------
 
 @pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
@@ -224,7 +232,7 @@ def test_single_tokens(ctx, precision, H, kv, hd):
 @pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
 @pytest.mark.parametrize("H, kv, hd", [(14, 2, 64), (32, 8, 128), (6, 2, 256), (5, 5, 20)])
 @pytest.mark.parametrize("held, rows", [(0, 1), (0, 45), (130, 17), (31, 2), (500, 33)])
-def test_chunks(ctx, precision, H, kv, hd, held, rows):
+def test_chunks(ctx, form, precision, H, kv, hd, held, rows):
     p = Pool(ctx, np.random.default_rng(held + rows), precision, kv, hd, 32, [held + rows, held + rows])
     p.push([held, held])
     p.push([rows, rows])
@@ -232,7 +240,7 @@ def test_chunks(ctx, precision, H, kv, hd, held, rows):
 
 
 @pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
-def test_ragged_batches(ctx, precision):
+def test_ragged_batches(ctx, form, precision):
     # more sequences than a wave has lanes, some without rows, some without
     # positions
     rng = np.random.default_rng(11)
@@ -286,7 +294,7 @@ WINDOWS = [(1, 0), (1, 1), (7, 0), (32, 4), (33, 31), (64, 32), (100, 33), (64, 
 
 @pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
 @pytest.mark.parametrize("window, sinks", WINDOWS)
-def test_windows(ctx, precision, window, sinks):
+def test_windows(ctx, form, precision, window, sinks):
     p = Pool(ctx, np.random.default_rng(window + sinks), precision, 2, 64, 32, [420, 30, 1, 333])
     p.push([400, 0, 0, 332])
     p.push([20, 30, 1, 1])
@@ -303,19 +311,24 @@ def test_long_window_prompt(ctx, precision):
 
 
 @pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
-@pytest.mark.parametrize("held", [2000, 8001])
-def test_long_caches_split_over_the_positions(ctx, precision, held):
+@pytest.mark.parametrize("held, splits", [(2000, 0), (8001, 0), (2000, 2), (2000, 7), (2000, 63), (8001, 251), (40, 2)])
+def test_long_caches_split_over_the_positions(ctx, form, monkeypatch, precision, held, splits):
+    # a join of few splits by a wave, of many by four, of more than a wave has
+    # lanes; splits that see nothing
+    if splits:
+        monkeypatch.setenv("KVAD_PAGED_SPLITS", str(splits))
     p = Pool(ctx, np.random.default_rng(held), precision, 2, 128, 128, [held + 3, 700, 40])
     p.push([held, 697, 0])
     p.push([3, 3, 40])
     b = p.batch([3, 3, 40])
-    assert p.cache.attend_ws(b, 8) > 0
+    assert form == "128" or p.cache.attend_ws(b, 8) > 0
     p.check([3, 3, 40], 8)
     p.check([3, 3, 40], 8, window=1500, sinks=4)
+    p.check([1, 0, 2], 8, window=33, sinks=1)
 
 
 @pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
-def test_scores_that_spread(ctx, precision):
+def test_scores_that_spread(ctx, form, precision):
     # the maximum rises from tile to tile, by far more than a sum can keep;
     # and a first position that takes nearly all the weight
     rng = np.random.default_rng(13)
@@ -330,7 +343,7 @@ def test_scores_that_spread(ctx, precision):
 
 
 @pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
-def test_values_of_many_sizes(ctx, precision):
+def test_values_of_many_sizes(ctx, form, precision):
     # V's rows from 1e-12 to 1e12: the reference follows their scales; the
     # large ones are hidden from the early rows, which stay exact
     rng = np.random.default_rng(17)
@@ -340,7 +353,7 @@ def test_values_of_many_sizes(ctx, precision):
     p.check([300], 2)
 
 
-def test_rows_of_zeros(ctx):
+def test_rows_of_zeros(ctx, form):
     for precision in PRECISIONS:
         p = Pool(ctx, np.random.default_rng(1), precision, 1, 64, 32, [70])
         p.push([70], k=np.zeros((70, 1, 64), np.float32), v=p.rows(70))
@@ -354,7 +367,7 @@ def test_rows_of_zeros(ctx):
 
 @pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, np.finfo(np.float32).min])
-def test_what_is_hidden_changes_nothing(ctx, precision, bad):
+def test_what_is_hidden_changes_nothing(ctx, form, precision, bad):
     # the same rows over pages that hold such values behind the sequence's end,
     # ahead of a row in its own chunk, and between the sinks and the window
     rng = np.random.default_rng(19)
@@ -387,7 +400,7 @@ def test_what_is_hidden_changes_nothing(ctx, precision, bad):
 
 
 @pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
-def test_what_is_not_finite_reaches_the_rows_that_see_it(ctx, precision):
+def test_what_is_not_finite_reaches_the_rows_that_see_it(ctx, form, precision):
     p = Pool(ctx, np.random.default_rng(23), precision, 2, 64, 32, [90])
     v = p.rows(90)
     v[60, 1, 5] = np.nan
@@ -414,7 +427,7 @@ def device_batch(lens, pages, rows=None, n_rows=None, starts=None, max_len=0):
     return b
 
 
-def test_rows_outside_the_sequences_are_left_alone(ctx):
+def test_rows_outside_the_sequences_are_left_alone(ctx, form):
     import torch
 
     p = Pool(ctx, np.random.default_rng(29), "f16", 2, 64, 32, [3000, 50])
@@ -434,7 +447,7 @@ def test_rows_outside_the_sequences_are_left_alone(ctx):
         p.check([2, 3], 4, q=q.cpu().numpy()[2:7], got=out.cpu().numpy()[2:7], window=window)
 
 
-def test_lengths_and_pages_that_lead_nowhere(ctx):
+def test_lengths_and_pages_that_lead_nowhere(ctx, form):
     # values the host cannot see: hidden from every row, read as zero, not written
     import torch
 
@@ -501,7 +514,7 @@ def test_lengths_and_pages_that_lead_nowhere(ctx):
 
 @pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
 @pytest.mark.parametrize("offset", [0, 1])
-def test_strided_rows(ctx, precision, offset):
+def test_strided_rows(ctx, form, precision, offset):
     # q, k and v as one row of a joint projection, at and off 16-byte alignment
     import torch
 
