@@ -750,7 +750,7 @@ constexpr int FEW = 8;  // rows (x group) of a sequence that few_rows takes besi
 // Waves a SIMD by the registers that the loop holds: many_rows' 32 columns, or
 // few_rows' query, sums, K, V and the rest.
 constexpr int waves_for(int es, int d, int rows) {
-    if (rows > 16) return es == 4 || d == 256 ? 1 : 2;
+    if (rows > 16) return d == 256 || es * d > 256 ? 1 : 2;
     const int regs = d / 8 * (rows / 8) + d / 4 + d * es / 4 + 60;
     return regs <= 128 ? 4 : regs <= 172 ? 3 : regs <= 250 ? 2 : 1;
 }
@@ -924,9 +924,9 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
     if (p.tile_rows < 128) {
         // few_rows, bound by memory: a workgroup for each CU.  many_rows, bound
         // by its arithmetic, of which one wave keeps half a SIMD busy: as many
-        // as are at work at once, and none that would wait for a place.  Each gets as many tiles as
-        // take as long as joining the splits does (a launch, 4 us): 16, or
-        // fewer large ones.
+        // as are at work at once, and none that would wait for a place.  Each
+        // gets as many tiles as take as long as joining the splits does (a
+        // launch, 4 us): 16, or fewer large ones.
         const size_t least = std::min(std::max(2048 / (kv->es * kv->d), 4), 16);
         const size_t want = p.tile_rows <= 16 ? up_to(cus, blocks) : resident / blocks;
         const size_t most = pos_tiles / least;
