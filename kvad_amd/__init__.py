@@ -10,6 +10,7 @@ Rust operator API so that tests and benchmarks read like the reference's own:
     matvec_many(ctx, jobs)           quant.rs:628    quant::matvec_many
     KvCache.push/keys/truncate/...   model/mod.rs:612-749
     attend(ctx, spec, q, cache, layer, n)   model/mod.rs:769
+    PagedCache.push/read/attend      a cache by pages, in fewer bits, for many sequences
 
 There is no CPU fallback: if libkvad_hip.so is missing this import fails.
 """

@@ -3,7 +3,9 @@
 // the attention over it (paged_attn.hip).
 //
 // Both kernels move each byte once and are bound by HBM, or by the launch for
-// a few rows.  A workgroup takes the 32 positions of one layout tile, one KV
+// a few rows (20001 positions of 8 heads of 128 read from i8: 43 us for 206 MB,
+// 4.8 TB/s, a large copy's rate; 4500 rows written in 13 us, 3.6 TB/s; 48 single
+// rows 2.5 us).  A workgroup takes the 32 positions of one layout tile, one KV
 // head, K and V: a cache unit of V runs over positions and a row over dims, so
 // the tile is turned in LDS, and both sides go in whole lines: rows of
 // head_dim floats, and 16-byte units 32 to 256 in a run.

@@ -24,6 +24,15 @@
 // piece a product of its own.  few_rows: 8 or 16 rows on 16x16x32 products; with
 // 8, the pieces are the two halves of the 16 columns, so that one product does
 // both, and their sums meet in the scores (by a lane move) and at the end.
+//
+// What bounds them.  few_rows: HBM (64 sequences of up to 4000 i8 positions, 8
+// heads of 128: 76 us for 362 MB, 4.8 TB/s, a large copy's rate), or for one
+// short sequence the trips to memory and the joining launch.  many_rows: the
+// matrix cores, 49% at work, behind 6 vector instructions a product (a wave
+// issues one in 8 cycles, so two waves a SIMD, all that 256 registers allow,
+// just fill it): 512 tokens behind 8000, f16, 32 heads of 128: 139 us, 498
+// TFLOP/s of the scores and values or 997 of the products run for them, where a
+// large bf16 product of the library reaches 1200.
 #include <algorithm>
 #include <utility>
 
@@ -67,6 +76,12 @@ __device__ __forceinline__ float shfl(float v, int x) { return __shfl_xor(v, x);
 template <int I>
 __device__ __forceinline__ float of_lane(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x150 + I, 0xf, 0xf, true));
+}
+// A product with another lane's value is one instruction if the two are found
+// beside each other: computed here, not where it is first wanted.
+__device__ __forceinline__ float here_and_now(float v) {
+    asm volatile("" : "+v"(v));
+    return v;
 }
 // the largest of each row of 16, in all of its lanes
 __device__ __forceinline__ unsigned row_max(unsigned v) {
@@ -430,13 +445,13 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
                           (a.window != INT32_MAX && start + TILE > a.sinks && start < w.p_hi - a.window + 1);
         here = table.find(a, w, next_t, next_page);
         load_k(here);
-        __builtin_amdgcn_sched_barrier(0);
-        only_finite(vs, ks);
-        float st[16];
-        each<16>([&](auto i) { st[i] = sc[i.value] * of_lane<i>(ks); });
-        const float sv = vs, v_inv = ES == 4 ? inv_pow2(vs) : 0.0f;
-        __builtin_amdgcn_sched_barrier(0);
+        float sk = ks, sv = vs;
         load_s(here);
+        __builtin_amdgcn_sched_barrier(0);
+        only_finite(sv, sk);
+        float st[16];
+        each<16>([&](auto i) { st[i] = here_and_now(sc[i.value] * of_lane<i>(sk)); });
+        const float v_inv = ES == 4 ? inv_pow2(sv) : 0.0f;
 
         // ---- weights ----
         unsigned vtop;
@@ -479,7 +494,7 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
             each<16>([&](auto i) {
                 const float p = exp2_(__builtin_fmaf(st[i], rowf, shift));
                 part[i & 3] = part[i & 3] + p;
-                x[i] = p * of_lane<i>(sv);
+                x[i] = here_and_now(p * of_lane<i>(sv));
             });
             sum = sum + ((part[0] + part[1]) + (part[2] + part[3]));
             split8(x, ph[0], pl[0]);
@@ -651,17 +666,17 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
                           (a.window != INT32_MAX && start + TILE > a.sinks && start < w.p_hi - a.window + 1);
         here = table.find(a, w, next_t, next_page);
         load_k(here);
+        float sk = ks, sv = vs;
+        load_s(here);
         __builtin_amdgcn_sched_barrier(0);
-        only_finite(vs, ks);
+        only_finite(sv, sk);
         float st[8];
         each<8>([&](auto i) {
             float s = sc[i >> 2][i.value & 3];
             if (PACKED) s = s + other_half(s);
-            st[i] = s * of_lane<i>(ks);
+            st[i] = s * of_lane<i>(sk);
         });
-        const float sv = vs, v_inv = ES == 4 ? inv_pow2(vs) : 0.0f;
-        __builtin_amdgcn_sched_barrier(0);
-        load_s(here);
+        const float v_inv = ES == 4 ? inv_pow2(sv) : 0.0f;
 
         // ---- weights ----
         unsigned vtop;
@@ -902,9 +917,11 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
     // few_rows where no sequence has more rows than it takes, where many_rows
     // does not fit the registers, and for small calls: up to 16 tiles a CU its
     // way in and out is shorter (100 new tokens of 32 heads of 128, f16: 5.9 us
-    // against 8.5; 100 behind 3000, i8: 31 against 28).  Else 128 rows a
-    // workgroup where that alone fills the device (a 6000-token prompt, f16:
-    // 646 us against 694 with 32), 32 where it does not.
+    // against 8.5; 300: 12.0 against 12.6; 100 behind 3000, i8: 30 against 28,
+    // f32: 60 against 42).  Else 128 rows a workgroup, whose waves read the same
+    // K and V at about the same time, where that alone fills the device (a
+    // 6000-token prompt, f16: 580 us against 618 with 32 and 747 with 16), 32
+    // where it does not.
     const size_t rows = b.row_start ? SIZE_MAX : (size_t)b.per * group, cus = (size_t)cu_count;
     const size_t resident = cus * waves_for(kv->es, kv->d, 32);  // many_rows' workgroups
     const bool small = tiles(16) * kv->n_kv_head * over(16) <= 16 * cus;
