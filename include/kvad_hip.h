@@ -324,7 +324,7 @@ int kh_paged_read_dev(const kh_paged *kv, size_t layer, const kh_batch *b, float
  *
  * Calls of few rows over many positions are split over the positions and
  * joined through `ws`, 16-byte aligned device memory of up to
- * kh_paged_attend_ws bytes (less: fewer splits).  ws NULL takes the context's
+ * kh_paged_attend_ws bytes (less: fewer splits).  ws NULL takes the cache's own
  * scratch, and none while the stream is captured: a call in a graph that should
  * be split brings its own, one for each graph that may run at the same time. */
 int kh_paged_attend(kh_paged *kv, size_t layer, const kh_batch *b, size_t n_head, const float *q, float scale,

@@ -670,7 +670,7 @@ class PagedCache:
                                        window, sinks, out_ptr, out_stride, ws_ptr, ws_bytes))
 
     def attend_ws(self, batch: Batch, n_head: int, window: int = 0, sinks: int = 0) -> int:
-        """Bytes of workspace with which attend_dev splits such a call as it would with the context's."""
+        """Bytes of workspace with which attend_dev splits such a call as it would with the cache's own."""
         n = _sz()
         _check(lib.kh_paged_attend_ws(self.h, C.byref(batch), n_head, window, sinks, C.byref(n)))
         return n.value

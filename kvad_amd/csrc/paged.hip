@@ -4,8 +4,8 @@
 //
 // Both kernels move each byte once and are bound by HBM, or by the launch for
 // a few rows (20001 positions of 8 heads of 128 read from i8: 43 us for 206 MB,
-// 4.8 TB/s, a large copy's rate; 4500 rows written in 13 us, 3.6 TB/s; 48 single
-// rows 2.5 us).  A workgroup takes the 32 positions of one layout tile, one KV
+// 4.8 TB/s, a large copy's rate; 4500 rows written in 13 us, 3.5 TB/s; 48 single
+// rows 3.7 us).  A workgroup takes the 32 positions of one layout tile, one KV
 // head, K and V: a cache unit of V runs over positions and a row over dims, so
 // the tile is turned in LDS, and both sides go in whole lines: rows of
 // head_dim floats, and 16-byte units 32 to 256 in a run.
@@ -471,6 +471,7 @@ int kh_paged_free(kh_paged *kv) {
         Guard g(kv->ctx);
         (void)hipStreamSynchronize(kv->ctx->stream);
         for (char *p : kv->layers) (void)hipFree(p);
+        if (kv->scratch.ptr) (void)hipFree(kv->scratch.ptr);
     }
     delete kv;
     return KH_OK;
@@ -579,6 +580,7 @@ int check_attend(const kh_paged *kv, size_t layer, const kh_batch *b, size_t n_h
     if (!(scale > 0.0f) || !std::isfinite(scale)) return refuse(what, "scale is positive and finite");
     if (b->n_rows == 0) return KH_OK;
     if (!q || !out) return refuse(what, "null argument");
+    if (q == out) return refuse(what, "out is not q");
     if (!aligned4(q) || !aligned4(out)) return refuse(what, "rows are of 32-bit floats");
     const size_t width = n_head * kv->head_dim;
     if ((q_stride && q_stride < width) || (out_stride && out_stride < width))
@@ -610,18 +612,18 @@ AttnCall call_of(const kh_paged *kv, size_t layer, const kh_batch *b, size_t n_h
     return c;
 }
 
-// The plan, its partials in the caller's workspace or the context's scratch.
-int attend(AttnCall &c, void *ws, size_t ws_bytes) {
-    kh_ctx *ctx = c.kv->ctx;
+// The plan, its partials in the caller's workspace or the cache's scratch.
+int attend(kh_paged *kv, AttnCall &c, void *ws, size_t ws_bytes) {
+    kh_ctx *ctx = kv->ctx;
     if (ws && (reinterpret_cast<uintptr_t>(ws) & 15)) return fail(KH_EINVAL, "kh_paged_attend: ws is not 16-byte aligned");
-    // the context's scratch may move before a captured graph runs: there the
+    // the scratch may move before a captured graph runs: there the
     // call takes none and its positions are not split
     const size_t most = ws ? ws_bytes : capturing(ctx->stream) ? 0 : SIZE_MAX;
     AttnPlan p = plan_attn(ctx->cu_count, c.kv, c.b, c.n_head, c.max_len, c.window, c.sinks, most);
     c.ws = ws;
     if (!ws && p.ws_bytes) {
-        if (ensure(ctx, ctx->ws, p.ws_bytes) == KH_OK) {
-            c.ws = ctx->ws.ptr;
+        if (ensure(ctx, kv->scratch, p.ws_bytes) == KH_OK) {
+            c.ws = kv->scratch.ptr;
         } else {  // no room: unsplit
             (void)hipGetLastError();
             p = plan_attn(ctx->cu_count, c.kv, c.b, c.n_head, c.max_len, c.window, c.sinks, 0);
@@ -644,8 +646,8 @@ int kh_paged_attend_ws(const kh_paged *kv, const kh_batch *b, size_t n_head, siz
     return guarded([&]() -> int {
         if (!bytes) return fail(KH_EINVAL, "kh_paged_attend_ws: null argument");
         *bytes = 0;
-        const float some = 0.0f;
-        if (int rc = check_attend(kv, 0, b, n_head, &some, 0, 1.0f, &some, 0, "kh_paged_attend_ws")) return rc;
+        const float some[2] = {};
+        if (int rc = check_attend(kv, 0, b, n_head, some, 0, 1.0f, some + 1, 0, "kh_paged_attend_ws")) return rc;
         if (b->n_rows == 0) return KH_OK;
         const AttnCall c = call_of(kv, 0, b, n_head, nullptr, 0, 1.0f, window, sinks, nullptr, 0);
         *bytes = plan_attn(kv->ctx->cu_count, kv, c.b, c.n_head, c.max_len, c.window, c.sinks, SIZE_MAX).ws_bytes;
@@ -662,7 +664,7 @@ int kh_paged_attend_dev(kh_paged *kv, size_t layer, const kh_batch *b, size_t n_
         if (b->n_rows == 0) return KH_OK;
         Guard g(kv->ctx);
         AttnCall c = call_of(kv, layer, b, n_head, q, q_stride, scale, window, sinks, out, out_stride);
-        return attend(c, ws, ws_bytes);
+        return attend(kv, c, ws, ws_bytes);
     });
 }
 
@@ -685,7 +687,7 @@ int kh_paged_attend(kh_paged *kv, size_t layer, const kh_batch *b, size_t n_head
         KH_HIP(hipMemcpyAsync(p + up256(n), out, n, hipMemcpyHostToDevice, ctx->stream));
         AttnCall c = call_of(kv, layer, &dev, n_head, reinterpret_cast<float *>(p), 0, scale, window, sinks,
                              reinterpret_cast<float *>(p + up256(n)), 0);
-        if ((rc = attend(c, nullptr, 0))) return rc;
+        if ((rc = attend(kv, c, nullptr, 0))) return rc;
         KH_HIP(hipMemcpyAsync(out, p + up256(n), n, hipMemcpyDeviceToHost, ctx->stream));
         KH_HIP(hipStreamSynchronize(ctx->stream));
         return KH_OK;

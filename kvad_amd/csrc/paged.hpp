@@ -15,6 +15,9 @@ struct kh_paged {
     size_t block = 0;               // bytes of one page of one head
     size_t bytes = 0;               // of all layers
     std::vector<char *> layers;
+    // Partials of split attention calls.  Its own, not the context's: no captured
+    // graph names it, so it may grow whatever was captured.
+    kh::Workspace scratch;
 };
 
 namespace kh {
@@ -97,8 +100,7 @@ struct AttnCall {
     float scale;
     int window, sinks;   // window INT32_MAX: none
     size_t max_len;      // positions of the longest sequence, for the split alone
-    void *ws;
-    size_t ws_bytes;
+    void *ws;            // partials
 };
 // How a call is cut up, from its sizes alone.
 struct AttnPlan {

@@ -803,3 +803,58 @@ def test_freed_with_its_context(ctx):
     other.close()
     assert cache.h is None
     cache.free()
+
+
+def test_a_split_call_leaves_a_captured_graph_of_another_operator_its_scratch(ctx):
+    # contiguous attention over a long cache, captured with the context's
+    # scratch as its first call made it; paged attention, which needs more for
+    # its splits, between the replays
+    import torch
+
+    H, kv, hd, L = 8, 2, 64, 6000
+    q, k, v = torch.randn(H, hd, device="cuda"), torch.randn(L, kv, hd, device="cuda"), torch.randn(L, kv, hd, device="cuda")
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    torch.cuda.synchronize()
+    fresh, stream = K.Context(0), torch.cuda.Stream()
+    try:
+        fresh.set_stream(stream.cuda_stream)
+        K.attend_dev(fresh, K.Spec(H, kv, hd), q.data_ptr(), k.data_ptr(), v.data_ptr(), L, want.data_ptr())
+        fresh.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            K.attend_dev(fresh, K.Spec(H, kv, hd), q.data_ptr(), k.data_ptr(), v.data_ptr(), L, out.data_ptr())
+        p = Pool(fresh, np.random.default_rng(71), "f32", 2, 256, 64, [9000])
+        p.push([9000])
+        for rows in (1, 9, 40):
+            assert rows == 1 or p.cache.attend_ws(p.batch([rows]), 32) > 1 << 20
+            p.check([rows], 32)
+            out.fill_(float("nan"))
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+        del g
+    finally:
+        fresh.set_stream(None)
+        fresh.close()
+
+
+def test_calls_of_several_threads(ctx):
+    # one context, one cache, two threads: calls in some order, each its own
+    from concurrent.futures import ThreadPoolExecutor
+
+    p = Pool(ctx, np.random.default_rng(73), "i8", 2, 64, 32, [3000, 200])
+    p.push([3000, 200])
+    qs = [p.rng.standard_normal((n + 1, 4, 64)).astype(np.float32) for n in range(8)]
+    batches = [p.batch([n, 1]) for n in range(8)]
+    alone = [p.cache.attend(0, b, 4, q) for b, q in zip(batches, qs)]
+    with ThreadPoolExecutor(2) as pool:
+        both = list(pool.map(lambda i: p.cache.attend(0, batches[i], 4, qs[i]), range(8)))
+    for a, b in zip(alone, both):
+        np.testing.assert_array_equal(a, b)
+
+
+def test_out_is_not_q(ctx):
+    p = Pool(ctx, np.random.default_rng(79), "f16", 2, 64, 32, [40])
+    with pytest.raises(K.KvadError, match="out is not q"):
+        p.cache.attend_dev(0, p.batch([1]), 4, 64, 64)
