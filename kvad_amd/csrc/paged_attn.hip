@@ -943,17 +943,23 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
         // by its arithmetic, of which one wave keeps half a SIMD busy: as many
         // as are at work at once, and none that would wait for a place.  Each
         // gets as many tiles as take as long as joining the splits does (a
-        // launch, 4 us): 16, or fewer large ones.
+        // launch, 4 us): 16, or fewer large ones; and where all splits together
+        // save a wave less turns than that, there are none.
         const size_t least = std::min(std::max(2048 / (kv->es * kv->d), 4), 16);
         const size_t want = p.tile_rows <= 16 ? up_to(cus, blocks) : resident / blocks;
-        const size_t most = pos_tiles / least;
         const int forced = env_int("KVAD_PAGED_SPLITS", 0);
-        size_t splits = forced > 0 ? std::min((size_t)forced, pos_tiles) : std::min(want, most);
+        size_t splits = forced > 0 ? std::min((size_t)forced, pos_tiles) : std::min(want, up_to(pos_tiles, least));
+        if (!forced && splits > 1 && up_to(pos_tiles, 4) < up_to(up_to(pos_tiles, splits), 4) + least / 4) splits = 1;
         splits = std::min(splits, (size_t)1024);
         const size_t each = 4 * (size_t)b.n_rows * n_head * (kv->d + 2);
         if (ws_max / each < splits) splits = ws_max / each;
         if (splits > 1) {
+            // few_rows waits for memory, and as long for one wave's tile as for
+            // four: whole turns of the four waves (1500 positions, f32, 16 heads
+            // of 128: 10.7 us against 12.0).  many_rows does not: the splits as
+            // even as they can be (100 behind 2000, i8: 23.4 us against 24.1)
             p.split_tiles = (int)up_to(pos_tiles, splits);
+            if (p.tile_rows <= 16) p.split_tiles = 4 * (int)up_to(p.split_tiles, 4);
             p.splits = (int)up_to(pos_tiles, p.split_tiles);
             p.ws_bytes = p.splits > 1 ? each * p.splits : 0;
         }
