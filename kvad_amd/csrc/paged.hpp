@@ -109,6 +109,7 @@ struct AttnPlan {
     int per;           // tiles of each sequence where rows are not
     int splits;        // of the positions, over workgroups
     int split_tiles;   // 32-position tiles a split
+    int join_waves;    // that join a row's splits
     size_t ws_bytes;   // of partials
 };
 AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head, size_t max_len, int window, int sinks,

@@ -334,6 +334,9 @@ __device__ __forceinline__ void put_row(const Args &a, const Job &w, const Row &
                 float4u{o[4 * c] * inv, o[4 * c + 1] * inv, o[4 * c + 2] * inv, o[4 * c + 3] * inv};
 }
 
+// Rows of K and V whose raw loads many_rows has one set of registers for.
+constexpr bool shares_registers(int es, int d) { return es == 4 && d >= 128; }
+
 // 32 rows; WS waves share them (1: each has its own).
 template <int ES, int D, int WS>
 __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float *lds) {
@@ -356,33 +359,37 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
     // its half from the lanes beside it
     const unsigned s_lane = (unsigned)(2 * P * D * ES) + 4 * (16 * h + (lane & 15));
     const Table table(a, w.seq);
-    int4 kraw[NK], vraw[DT * ES];
+    // Wide rows (SHARED): K and V take turns in the same registers, half of
+    // the dims at a time, each half loaded as soon as the other's is used.
+    constexpr bool SHARED = shares_registers(ES, D);
+    int4 kraw[NK], vown[SHARED ? 1 : DT * ES];
+    int4 *const vraw = SHARED ? kraw : vown;
     float ks, vs, k_own = 0.0f;
     auto load_s = [&](const Where &x) {
         ks = load4(x.r, s_lane, 4 * x.in_page);
         vs = load4(x.r, s_lane, 4 * P + 4 * x.in_page);
+        if (ES == 4) k_own = dev::bldf(x.r, (unsigned)(2 * P * D * ES) + 4 * (x.in_page + tile_pos(n)));
     };
-    auto load_k = [&](const Where &x) {
+    auto load_k = [&](const Where &x, int from, int to) {
 #pragma unroll
-        for (int i = 0; i < NK; i++) {
+        for (int i = from; i < to; i++) {
             const int unit = k_load_unit(ES, i, 0);
             kraw[i] = load16(x.r, k_lane, (unsigned)(unit * P + x.in_page) * 16);
         }
-        if (ES == 4) k_own = dev::bldf(x.r, (unsigned)(2 * P * D * ES) + 4 * (x.in_page + tile_pos(n)));
     };
-    auto load_v = [&](const Where &x) {
+    auto load_v = [&](const Where &x, int from, int to) {
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-            for (int c = 0; c < ES; c++)
-                vraw[dt * ES + c] = load16(x.r, v_lane + (c * D + dt * 32) * 16, (unsigned)(x.in_page * D * ES));
+        for (int i = from; i < to; i++) {
+            const int dt = i / ES, c = i % ES;
+            vraw[i] = load16(x.r, v_lane + (c * D + dt * 32) * 16, (unsigned)(x.in_page * D * ES));
+        }
     };
 
     const int t_at = w.t_at + (WS == 1 ? 0 : wave), t_end = w.t_end;
     Where here;  // its K ahead of the query: one trip to memory, not two
     if (t_at < t_end) {
         here = table.find(a, w, t_at, table.page_of(a, w, t_at));
-        load_k(here);
+        load_k(here, 0, NK);
         load_s(here);
     }
 
@@ -405,7 +412,7 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
         // the next tile (this one again behind the last: the loads in flight
         // are the same at every wait, and none waits for more than its own)
         const int next_t = min(t + WS, t_end - 1), next_page = table.page_of(a, w, next_t);
-        load_v(here);
+        if (!SHARED) load_v(here, 0, DT * ES);
         __builtin_amdgcn_sched_barrier(0);
 
         // ---- scores: register i is position start + 16 h + i ----
@@ -437,6 +444,12 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
                 sc = mfma(kh, qh[i], sc);
                 sc = mfma(kh, ql[i], sc);
                 sc = mfma(kl, qh[i], sc);
+                if (SHARED && (i + 1) % (NS / 2) == 0) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int half = i / (NS / 2);
+                    load_v(here, half * (NK / 2), (half + 1) * (NK / 2));
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         }
         const int start = here.start;
@@ -444,7 +457,7 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
         const bool edge = !there || start + TILE - 1 > w.p_lo ||
                           (a.window != INT32_MAX && start + TILE > a.sinks && start < w.p_hi - a.window + 1);
         here = table.find(a, w, next_t, next_page);
-        load_k(here);
+        if (!SHARED) load_k(here, 0, NK);
         float sk = ks, sv = vs;
         load_s(here);
         __builtin_amdgcn_sched_barrier(0);
@@ -525,6 +538,11 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
                 acc[dt] = mfma(vh, ph[c], acc[dt]);
                 acc[dt] = mfma(vh, pl[c], acc[dt]);
                 acc[dt] = mfma(vl, ph[c], acc[dt]);
+                if constexpr (SHARED && (k + 1) % DT == 0) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    load_k(here, k / DT * (NK / 2), (k / DT + 1) * (NK / 2));
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         });
     }
@@ -757,15 +775,12 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
     put_row(a, w, row, o, ref, sum, z == 0, D, [&](int c) { return 16 * c + 4 * z; });
 }
 
-// Bytes of a row of K up to which many_rows fits the registers; wider rows (f32,
-// 256 dims) are taken 16 at a time, however many there are.
-constexpr int MANY_MAX = 512;
 constexpr int FEW = 8;  // rows (x group) of a sequence that few_rows takes beside longer ones
 
 // Waves a SIMD by the registers that the loop holds: many_rows' 32 columns, or
 // few_rows' query, sums, K, V and the rest.
 constexpr int waves_for(int es, int d, int rows) {
-    if (rows > 16) return d == 256 || es * d > 256 ? 1 : 2;
+    if (rows > 16) return d == 256 ? 1 : 2;
     const int regs = d / 8 * (rows / 8) + d / 4 + d * es / 4 + 60;
     return regs <= 128 ? 4 : regs <= 172 ? 3 : regs <= 250 ? 2 : 1;
 }
@@ -815,7 +830,10 @@ void attn_kernel(Args a) {
 }
 
 // The splits of a row and head, joined at the largest reference, by WM waves:
-// one, or four that take every fourth split where there are many.
+// one, or four that take every fourth split where there are many and the rows
+// few enough for a workgroup each at once (one decoded token of 14 heads, 128
+// splits: 10.4 us in all against 20.2; 20 tokens of 32 heads, 10 splits: 18.5
+// against 16.9).
 template <int D, int WM>
 __global__ __launch_bounds__(256) void merge_kernel(Args a) {
     const int n_head = a.n_kv * a.group;
@@ -877,13 +895,11 @@ template <int ES, int D>
 int launch(const Args &a, const AttnPlan &p, unsigned blocks, size_t items, hipStream_t stream) {
     if (p.tile_rows == 8) attn_kernel<ES, D, 8><<<blocks, 256, 0, stream>>>(a);
     else if (p.tile_rows == 16) attn_kernel<ES, D, 16><<<blocks, 256, 0, stream>>>(a);
-    else if constexpr (ES * D <= MANY_MAX) {
-        if (p.tile_rows == 32) attn_kernel<ES, D, 32><<<blocks, 256, 0, stream>>>(a);
-        else attn_kernel<ES, D, 128><<<blocks, 256, 0, stream>>>(a);
-    }
+    else if (p.tile_rows == 32) attn_kernel<ES, D, 32><<<blocks, 256, 0, stream>>>(a);
+    else attn_kernel<ES, D, 128><<<blocks, 256, 0, stream>>>(a);
     KH_HIP(hipGetLastError());
     if (p.splits > 1) {
-        if (p.splits > 8) merge_kernel<D, 4><<<(unsigned)items, 256, 0, stream>>>(a);
+        if (p.join_waves > 1) merge_kernel<D, 4><<<(unsigned)items, 256, 0, stream>>>(a);
         else merge_kernel<D, 1><<<(unsigned)((items + 3) / 4), 256, 0, stream>>>(a);
         KH_HIP(hipGetLastError());
     }
@@ -898,6 +914,38 @@ int launch_d(int d, const Args &a, const AttnPlan &p, unsigned blocks, size_t it
 }
 
 size_t up_to(size_t n, size_t m) { return (n + m - 1) / m; }
+
+// Splits of few_rows, bound by memory: a workgroup for each CU.  Each gets as
+// many tiles as take as long as joining the splits does (a launch, 4 us): 16, or
+// fewer large ones; and where all splits together save a wave less turns than
+// that, there are none.
+size_t few_splits(const kh_paged *kv, size_t blocks, size_t pos_tiles, size_t cus) {
+    const size_t least = std::min(std::max(2048 / (kv->es * kv->d), 4), 16);
+    const size_t splits = std::min(up_to(cus, blocks), up_to(pos_tiles, least));
+    return up_to(pos_tiles, 4) < up_to(up_to(pos_tiles, splits), 4) + least / 4 ? 1 : splits;
+}
+// Splits of many_rows, bound by arithmetic: those whose slowest CU ends first.
+// A wave's turn takes 1 us (128 dims, f16 or i8; f32 2), those of two workgroups
+// on a CU together half as much again (f32, whose vector instructions are what
+// counts, three quarters); a join its launch and the partials' way out and in.
+// Never more workgroups than find a place at once.  5000 f16 positions, 32 heads
+// on 8 of 128: 20 rows, one split 30 us, 8 or 10 of them 17, 20 of them 20; 200
+// rows behind 3000, whose one split has 200 workgroups, 33 us against 37 with
+// two; 512 of 14 heads of 64 behind 8000 52 us, with two 49.
+size_t many_splits(const kh_paged *kv, size_t blocks, size_t pos_tiles, size_t cus, size_t resident, size_t items) {
+    const double turn = (kv->d + 32) / 160.0 * (kv->es == 4 ? 2.0 : 1.0), both = kv->es == 4 ? 1.75 : 1.5;
+    const double join = 8e-6 / 2.4 * (double)items * (kv->d + 2);
+    size_t splits = 1;
+    double least = 0.0;
+    for (size_t s = 1; s <= std::min(resident / blocks, pos_tiles); s++) {
+        const double us = (double)up_to(up_to(pos_tiles, s), 4) * turn * (blocks * s > cus ? both : 1.0) +
+                          (s > 1 ? 2.5 + join * (double)s : 0.0);
+        if (s > 1 && us >= least) continue;
+        splits = s;
+        least = us;
+    }
+    return splits;
+}
 
 }  // namespace
 
@@ -914,24 +962,23 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
         if (window != INT32_MAX) span = std::min(span, (size_t)window + rows / group + sinks + 2 * TILE);
         return up_to(span, TILE);
     };
-    // few_rows where no sequence has more rows than it takes, where many_rows
-    // does not fit the registers, and for small calls: up to 16 tiles a CU its
-    // way in and out is shorter (100 new tokens of 32 heads of 128, f16: 5.9 us
-    // against 8.5; 300: 12.0 against 12.6; 100 behind 3000, i8: 30 against 28,
-    // f32: 60 against 42).  Else 128 rows a workgroup, whose waves read the same
-    // K and V at about the same time, where that alone fills the device (a
-    // 6000-token prompt, f16: 580 us against 618 with 32 and 747 with 16), 32
-    // where it does not.
+    // few_rows where no sequence has more rows than it takes, and for small
+    // calls: up to 16 tiles a CU its way in and out is shorter (100 new tokens
+    // of 32 heads of 128, f16: 5.9 us against 8.5; 300: 12.0 against 12.6; 100
+    // behind 3000, i8: 30 against 26, f32: 60 against 39).  Else 128 rows a
+    // workgroup, whose waves read the same K and V at about the same time, where
+    // that alone fills the device (a 6000-token prompt, f16: 580 us against 618
+    // with 32 and 747 with 16), 32 where it does not.
     const size_t rows = b.row_start ? SIZE_MAX : (size_t)b.per * group, cus = (size_t)cu_count;
     const size_t resident = cus * waves_for(kv->es, kv->d, 32);  // many_rows' workgroups
     const bool small = tiles(16) * kv->n_kv_head * over(16) <= 16 * cus;
     p.tile_rows = rows <= 8                                            ? 8
-                  : rows <= 16 || small || kv->es * kv->d > MANY_MAX ? 16
+                  : rows <= 16 || small                              ? 16
                   : tiles(128) * kv->n_kv_head >= resident           ? 128
                                                                      : 32;
     // for experiments, and for tests of each form: any form does any call
     const int form = env_int("KVAD_PAGED_TILE", 0);
-    if (form == 8 || form == 16 || ((form == 32 || form == 128) && kv->es * kv->d <= MANY_MAX)) p.tile_rows = form;
+    if (form == 8 || form == 16 || form == 32 || form == 128) p.tile_rows = form;
     p.tiles = (int)tiles(p.tile_rows);
     p.per = b.row_start ? 0 : (int)up_to((size_t)b.per * group, p.tile_rows);
     const size_t pos_tiles = over(p.tile_rows);
@@ -939,17 +986,11 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
     p.splits = 1;
     p.split_tiles = (int)pos_tiles;
     if (p.tile_rows < 128) {
-        // few_rows, bound by memory: a workgroup for each CU.  many_rows, bound
-        // by its arithmetic, of which one wave keeps half a SIMD busy: as many
-        // as are at work at once, and none that would wait for a place.  Each
-        // gets as many tiles as take as long as joining the splits does (a
-        // launch, 4 us): 16, or fewer large ones; and where all splits together
-        // save a wave less turns than that, there are none.
-        const size_t least = std::min(std::max(2048 / (kv->es * kv->d), 4), 16);
-        const size_t want = p.tile_rows <= 16 ? up_to(cus, blocks) : resident / blocks;
         const int forced = env_int("KVAD_PAGED_SPLITS", 0);
-        size_t splits = forced > 0 ? std::min((size_t)forced, pos_tiles) : std::min(want, up_to(pos_tiles, least));
-        if (!forced && splits > 1 && up_to(pos_tiles, 4) < up_to(up_to(pos_tiles, splits), 4) + least / 4) splits = 1;
+        size_t splits = 1;
+        if (forced > 0) splits = std::min((size_t)forced, pos_tiles);
+        else if (p.tile_rows <= 16) splits = few_splits(kv, blocks, pos_tiles, cus);
+        else splits = many_splits(kv, blocks, pos_tiles, cus, resident, (size_t)b.n_rows * n_head);
         splits = std::min(splits, (size_t)1024);
         const size_t each = 4 * (size_t)b.n_rows * n_head * (kv->d + 2);
         if (ws_max / each < splits) splits = ws_max / each;
@@ -962,6 +1003,7 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
             if (p.tile_rows <= 16) p.split_tiles = 4 * (int)up_to(p.split_tiles, 4);
             p.splits = (int)up_to(pos_tiles, p.split_tiles);
             p.ws_bytes = p.splits > 1 ? each * p.splits : 0;
+            p.join_waves = p.splits > 8 && (size_t)b.n_rows * n_head <= cus ? 4 : 1;
         }
     }
     return p;
