@@ -18,7 +18,8 @@
 // one row's weights for the positions that V's operand wants of it, so the
 // weights go from one product to the next in registers, and K and V come from
 // memory in operand order (paged_layout.hpp): there is no LDS in the loop.  K of
-// the next tile and V of this one are loaded while the weights are computed.
+// the next tile and V of this one are loaded while the weights are computed
+// (wide f32 rows: by halves, each as soon as its registers are free).
 //
 // Two forms of the wave's work.  many_rows: 32 rows on 32x32x16 products, each
 // piece a product of its own.  few_rows: 8 or 16 rows on 16x16x32 products; with
@@ -334,7 +335,9 @@ __device__ __forceinline__ void put_row(const Args &a, const Job &w, const Row &
                 float4u{o[4 * c] * inv, o[4 * c + 1] * inv, o[4 * c + 2] * inv, o[4 * c + 3] * inv};
 }
 
-// Rows of K and V whose raw loads many_rows has one set of registers for.
+// Rows of K and V whose raw loads many_rows has one set of registers for: two
+// sets leave 128 dims one wave a SIMD and 256 none (512 f32 tokens behind 8000,
+// 32 heads on 8 of 128: 286 us against 342; 16 of 256: 329 against 638 by 16 rows).
 constexpr bool shares_registers(int es, int d) { return es == 4 && d >= 128; }
 
 // 32 rows; WS waves share them (1: each has its own).
