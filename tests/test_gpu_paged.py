@@ -858,3 +858,47 @@ def test_out_is_not_q(ctx):
     p = Pool(ctx, np.random.default_rng(79), "f16", 2, 64, 32, [40])
     with pytest.raises(K.KvadError, match="out is not q"):
         p.cache.attend_dev(0, p.batch([1]), 4, 64, 64)
+
+
+@pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
+@pytest.mark.parametrize("hd", [128, 256])
+def test_wide_rows_behind_masks_and_splits(ctx, form, monkeypatch, precision, hd):
+    # what test_what_is_hidden_changes_nothing does with 64 dims: stale values
+    # behind the end and between sinks and window, chunks and splits of them
+    rng = np.random.default_rng(83)
+    held, rows = 300, 37
+    k, v = (rng.standard_normal((held + rows, 2, hd)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((rows, 4, hd)).astype(np.float32)
+    for splits in ("", "3"):
+        monkeypatch.setenv("KVAD_PAGED_SPLITS", splits)
+        outs = []
+        for dirty in (False, True):
+            p = Pool(ctx, np.random.default_rng(83), precision, 2, hd, 32, [384])
+            if dirty:
+                full = np.full((384, 2, hd), np.nan, np.float32)
+                p.cache.push(0, K.Batch.host([384], p.pages, [384]), full, full)
+            p.push([held], k=k[:held], v=v[:held])
+            p.push([rows], k=k[held:], v=v[held:])
+            outs.append(p.check([rows], 4, q=q))
+            if dirty:
+                mid = np.full((100, 2, hd), np.inf, np.float32)
+                p.cache.push(0, K.Batch.host([140], p.pages, [100]), mid, mid)
+            outs.append(p.cache.attend(0, p.batch([rows]), 4, q, window=70, sinks=40))
+            if dirty:  # and seen, they are what the rows become
+                out = p.cache.attend(0, p.batch([rows]), 4, q, window=70, sinks=41)
+                assert np.all(np.isnan(out))
+        for a, b in zip(outs[:2], outs[2:]):
+            assert np.all(np.isfinite(a))
+            np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+def test_long_chunks_of_wide_f32_rows(ctx, monkeypatch, hd):
+    # waves with rows of their own, and waves that share them
+    for tile in ("128", "32"):
+        monkeypatch.setenv("KVAD_PAGED_TILE", tile)
+        p = Pool(ctx, np.random.default_rng(89), "f32", 2, hd, 64, [700, 130])
+        p.push([450, 0])
+        p.push([250, 130])
+        p.check([250, 130], 6)
+        p.check([250, 130], 6, window=100, sinks=3)
