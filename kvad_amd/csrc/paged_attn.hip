@@ -110,6 +110,15 @@ __device__ __forceinline__ void only_finite(float &v_scale, float &k_scale) {
 // the value 8 lanes on, in each row of 16
 __device__ __forceinline__ float other_half(float v) { return dev::dppf<0x128>(v); }
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
+// A sum of weights at a reference `by` powers of two on (negative, or zero).  A
+// reference holds the exponent of V's scales, so it can move by more than a
+// float's exponents: rows of zeros ahead of large ones, whose sums are large and
+// count in full.  So in two steps, none of which is flushed; sums of values are
+// not large where the reference was low, and take one.
+__device__ __forceinline__ float moved(float sum, float by) {
+    const float half = exp2_(0.5f * by);
+    return sum * half * half;
+}
 
 // hi + lo of two floats.  hi is cut off, not rounded: one instruction that the
 // compiler cannot split into two conversions, whose ties need not agree, one
@@ -284,7 +293,7 @@ __device__ __forceinline__ void join_waves(float (&o)[N], float &ref, float &sum
     const float f = exp2_(ref - all);
     sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; w++) sum = sum + s_sum[w][col] * exp2_(s_ref[w][col] - all);
+    for (int w = 0; w < 4; w++) sum = sum + moved(s_sum[w][col], s_ref[w][col] - all);
     ref = all;
 #pragma unroll
     for (int k = 0; k < N; k++) o[k] = o[k] * f;
@@ -496,8 +505,8 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
             const float all = fmaxf(want, shfl(want, 32));
             const float next = all > ref + SLACK ? all : ref;
             const float f = exp2_(ref - next);
+            sum = moved(sum, ref - next);
             ref = next;
-            sum = sum * f;
 #pragma unroll
             for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -723,8 +732,8 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
             all = fmaxf(all, shfl(all, 32));
             const float next = all > ref + SLACK ? all : ref;
             const float f = exp2_(ref - next);
+            sum = moved(sum, ref - next);
             ref = next;
-            sum = sum * f;
 #pragma unroll
             for (int db = 0; db < DB; db++) acc[db] = acc[db] * f;
         }
@@ -876,7 +885,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args a) {
                     acc = acc + v[u] * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), j));
             }
         }
-        sum = sum + (m.y == 0.0f ? 0.0f : m.y * exp2_(m.x - all));
+        sum = sum + (m.y == 0.0f ? 0.0f : moved(m.y, m.x - all));
     }
     for (int o = 1; o < 64; o <<= 1) sum = sum + __shfl_xor(sum, o);
     if (WM > 1) {

@@ -902,3 +902,21 @@ def test_long_chunks_of_wide_f32_rows(ctx, monkeypatch, hd):
         p.push([250, 130])
         p.check([250, 130], 6)
         p.check([250, 130], 6, window=100, sinks=3)
+
+
+# ---- values, scales and queries at the ends of the range ------------------------------
+
+@pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
+@pytest.mark.parametrize("small, large", [(None, 44), (None, 90), (-100, 30), (-60, 80), (-118, 88)])
+@pytest.mark.parametrize("splits", ["", "3"])
+def test_small_values_before_large_ones_keep_their_weights(ctx, form, monkeypatch, precision, small, large, splits):
+    # zeros (None) or rows of 2^small, then rows of 2^large, and the other way
+    # round: what the small ones give is lost beside the large, but their weights
+    # are half of the sum that divides
+    monkeypatch.setenv("KVAD_PAGED_SPLITS", splits)
+    p = Pool(ctx, np.random.default_rng(97), precision, 2, 64, 32, [200, 200])
+    size = np.full((200, 1, 1), 2.0 ** large, np.float32)
+    size[:100] = 0 if small is None else 2.0 ** small
+    p.push([200, 200], v=p.rows(400) * np.concatenate([size, size[::-1]]))
+    p.check([7, 7], 4)
+    p.check([1, 30], 4, window=150, sinks=20)
