@@ -320,7 +320,7 @@ int kh_paged_read_dev(const kh_paged *kv, size_t layer, const kh_batch *b, float
  * that sees nothing is zero.  scale > 0 (model::attend's is
  * 1 / sqrt(head_dim)).  No weight is dropped for its size, unlike kh_attend's;
  * a position's part in the result is held to 2^-32 of the largest weight times
- * the largest |v| that the row sees.
+ * the largest |v| that the row sees, or times 2^-107 where all are smaller.
  *
  * Calls of few rows over many positions are split over the positions and
  * joined through `ws`, 16-byte aligned device memory of up to

@@ -52,10 +52,19 @@ typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));  // rows 
 typedef const __attribute__((address_space(4))) int32_t const_i32;
 
 constexpr float LOW = -3.0e38f;  // a running maximum that nothing has raised
-// Weights are kept at 2^BASE times their size over the row's reference, which
-// follows the maximum only when it is SLACK powers of two behind: under 2^15,
-// f16's range, and the sums are rescaled for few tiles.
+// Weights times V's scales are kept at 2^BASE times their size over the row's
+// reference, which follows their bound only when it is SLACK powers of two
+// behind: under 2^15, f16's range, and the sums are rescaled for few tiles.
 constexpr float BASE = 8.0f, SLACK = 6.0f;
+// A weight alone is as much smaller or larger as V's scales are large or small,
+// 2^89 (|v| of 2^96 as i8) to 2^-126.  So V_UP powers of two of the product are in
+// the scale, and the reference takes the scales' exponent as V_LOW or more: weights
+// of up to 2^122, 16 of which a lane adds, and of 2^-94 for the largest of a row,
+// with 32 powers of two below it.  Sums are kept at 2^-24 of that, for millions of
+// tiles of the first and normal floats of the second.  What rows of V with scales
+// under 2^V_LOW give is held to up to 5 bits less.
+constexpr int V_UP = 13, V_LOW = -121;
+constexpr float V_SCALE = 0x1p13f, SUM_SCALE = 0x1p-24f, OUT_SCALE = SUM_SCALE / V_SCALE;  // out: values over sum
 
 struct Args {
     const char *pool;
@@ -100,12 +109,13 @@ template <int N, typename F>
 __device__ __forceinline__ void each(F f) {
     each_(f, std::make_integer_sequence<int, N>{});
 }
-// A row of V that is not finite, by its scale: no part of any sum, and NaN as
-// a score, so that only rows that see it are NaN.
+// V's scale at 2^V_UP.  A row of V that is not finite, by its scale, or whose
+// scale is too large for that (i8, from 2^122 on): no part of any sum, and NaN as a
+// score, so that only rows that see it are NaN.
 __device__ __forceinline__ void only_finite(float &v_scale, float &k_scale) {
-    const bool finite = (__builtin_bit_cast(int, v_scale) & 0x7fffffff) < 0x7f800000;
+    const bool finite = (__builtin_bit_cast(int, v_scale) & 0x7fffffff) < 0x7f800000 - (V_UP << 23);
     k_scale = finite ? k_scale : __builtin_bit_cast(float, NAN_BITS);
-    v_scale = finite ? v_scale : 0.0f;
+    v_scale = finite ? v_scale * V_SCALE : 0.0f;
 }
 // the value 8 lanes on, in each row of 16
 __device__ __forceinline__ float other_half(float v) { return dev::dppf<0x128>(v); }
@@ -209,6 +219,11 @@ struct Where {
     dev::rsrc_t r;
     int start, in_page;
     bool there;
+    // V's bytes ahead of it.  Named a scalar: where the compiler computes it with
+    // the vector unit, each load would be a loop over the values it may have.
+    __device__ __forceinline__ unsigned v_at(int row_bytes) const {
+        return (unsigned)__builtin_amdgcn_readfirstlane(in_page * row_bytes);
+    }
 };
 struct Table {
     const_i32 *pages;
@@ -247,15 +262,18 @@ struct Row {
 template <int NS, typename F>
 __device__ __forceinline__ int load_q(const float *x, int hd, F dim0, float (&v)[NS][8]) {
     int amax = 0;
+    float4u f[NS][2];
+#pragma unroll
+    for (int i = 0; i < NS; i++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) f[i][c] = *reinterpret_cast<const float4u *>(x + min(dim0(i) + 4 * c, hd - 4));
+    __builtin_amdgcn_sched_barrier(0);  // all loads ahead of the first use
 #pragma unroll
     for (int i = 0; i < NS; i++) {
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            const int d = dim0(i) + 4 * c;
-            const float4u f = *reinterpret_cast<const float4u *>(x + min(d, hd - 4));
+        for (int c = 0; c < 2; c++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[i][4 * c + e] = d < hd ? f[e] : 0.0f;
-        }
+            for (int e = 0; e < 4; e++) v[i][4 * c + e] = dim0(i) + 4 * c < hd ? f[i][c][e] : 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; e++) amax = max(amax, __builtin_bit_cast(int, v[i][e]) & 0x7fffffff);
     }
@@ -271,8 +289,12 @@ __device__ __forceinline__ float q_scale(int amax, float scale, float &rowf) {
 // 1 / 2^k from 2^k
 __device__ __forceinline__ float inv_pow2(float s) { return __builtin_bit_cast(float, 0x7f000000 - __builtin_bit_cast(int, s)); }
 
-// The exponent of the largest of V's scales, within what the weights can take.
-__device__ __forceinline__ float scale_exp(unsigned bits) { return (float)min(max((int)(bits >> 23) - 127, -90), 90); }
+// The exponent of the largest of V's scales, from the bits of it at 2^V_UP.
+__device__ __forceinline__ float scale_exp(unsigned bits) { return (float)max((int)(bits >> 23) - 127 - V_UP, V_LOW); }
+// 1 / 2^k from 2^(k + V_UP)
+__device__ __forceinline__ float inv_v(float s) {
+    return __builtin_bit_cast(float, 0x7f000000 + (V_UP << 23) - __builtin_bit_cast(int, s));
+}
 
 // The sums of four waves over the same rows, column `col` of `cols` a lane, at
 // the largest reference: two and two and then one, through lds.  Wave 0 has them.
@@ -341,7 +363,8 @@ __device__ __forceinline__ void put_row(const Args &a, const Job &w, const Row &
     for (int c = 0; c < N / 4; c++)
         if (dim(c) < a.hd)
             *reinterpret_cast<float4u *>(to + dim(c)) =
-                float4u{o[4 * c] * inv, o[4 * c + 1] * inv, o[4 * c + 2] * inv, o[4 * c + 3] * inv};
+                float4u{o[4 * c] * OUT_SCALE * inv, o[4 * c + 1] * OUT_SCALE * inv, o[4 * c + 2] * OUT_SCALE * inv,
+                        o[4 * c + 3] * OUT_SCALE * inv};
 }
 
 // Rows of K and V whose raw loads many_rows has one set of registers for: two
@@ -390,10 +413,11 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
         }
     };
     auto load_v = [&](const Where &x, int from, int to) {
+        const unsigned at = x.v_at(D * ES);
 #pragma unroll
         for (int i = from; i < to; i++) {
             const int dt = i / ES, c = i % ES;
-            vraw[i] = load16(x.r, v_lane + (c * D + dt * 32) * 16, (unsigned)(x.in_page * D * ES));
+            vraw[i] = load16(x.r, v_lane + (c * D + dt * 32) * 16, at);
         }
     };
 
@@ -476,7 +500,7 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
         only_finite(sv, sk);
         float st[16];
         each<16>([&](auto i) { st[i] = here_and_now(sc[i.value] * of_lane<i>(sk)); });
-        const float v_inv = ES == 4 ? inv_pow2(sv) : 0.0f;
+        const float v_inv = ES == 4 ? inv_v(sv) : 0.0f;
 
         // ---- weights ----
         unsigned vtop;
@@ -512,7 +536,7 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
 #pragma unroll
                 for (int i = 0; i < 16; i++) acc[dt][i] = acc[dt][i] * f;
         }
-        const float shift = BASE - ref;
+        const float shift = BASE - V_UP - ref;
         h8 ph[2], pl[2];
         {
             float x[16], part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -521,7 +545,7 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
                 part[i & 3] = part[i & 3] + p;
                 x[i] = here_and_now(p * of_lane<i>(sv));
             });
-            sum = sum + ((part[0] + part[1]) + (part[2] + part[3]));
+            sum = __builtin_fmaf((part[0] + part[1]) + (part[2] + part[3]), SUM_SCALE, sum);
             split8(x, ph[0], pl[0]);
             split8(x + 8, ph[1], pl[1]);
         }
@@ -613,14 +637,15 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
         }
     };
     auto load_v = [&](const Where &x) {
+        const unsigned at = x.v_at(D * ES);
 #pragma unroll
         for (int db = 0; db < DB; db++) {
             if (ES == 1) {
-                vraw8[db % (ES == 1 ? DB : 1)] = load8(x.r, v_lane + 256 * db, (unsigned)(x.in_page * D * ES));
+                vraw8[db % (ES == 1 ? DB : 1)] = load8(x.r, v_lane + 256 * db, at);
             } else {
 #pragma unroll
                 for (int c = 0; c < NV; c++)
-                    vraw[(db * NV + c) % (ES == 1 ? 1 : DB * NV)] = load16(x.r, v_lane + 256 * db + c * D * 16, (unsigned)(x.in_page * D * ES));
+                    vraw[(db * NV + c) % (ES == 1 ? 1 : DB * NV)] = load16(x.r, v_lane + 256 * db + c * D * 16, at);
             }
         }
     };
@@ -706,7 +731,7 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
             if (PACKED) s = s + other_half(s);
             st[i] = s * of_lane<i>(sk);
         });
-        const float v_inv = ES == 4 ? inv_pow2(sv) : 0.0f;
+        const float v_inv = ES == 4 ? inv_v(sv) : 0.0f;
 
         // ---- weights ----
         unsigned vtop;
@@ -737,7 +762,7 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
 #pragma unroll
             for (int db = 0; db < DB; db++) acc[db] = acc[db] * f;
         }
-        const float shift = BASE - ref;
+        const float shift = BASE - V_UP - ref;
         h8 ph, pl;
         {
             float x[8], part[2] = {0.0f, 0.0f};
@@ -746,7 +771,7 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
                 part[i & 1] = part[i & 1] + p;
                 x[i] = p * of_lane<i>(sv);
             });
-            sum = sum + (part[0] + part[1]);
+            sum = __builtin_fmaf(part[0] + part[1], SUM_SCALE, sum);
             split8(x, ph, pl);
             if (low) ph = pl;
         }
@@ -900,7 +925,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args a) {
     float *o = a.out + (size_t)row * a.out_stride + (item - (size_t)row * n_head) * a.hd;
 #pragma unroll
     for (int e = 0; e < E; e++)
-        if (E * lane + e < a.hd) o[E * lane + e] = acc[e] * inv;
+        if (E * lane + e < a.hd) o[E * lane + e] = acc[e] * OUT_SCALE * inv;
 }
 
 template <int ES, int D>

@@ -920,3 +920,21 @@ def test_small_values_before_large_ones_keep_their_weights(ctx, form, monkeypatc
     p.push([200, 200], v=p.rows(400) * np.concatenate([size, size[::-1]]))
     p.check([7, 7], 4)
     p.check([1, 30], 4, window=150, sinks=20)
+
+
+# Tolerance: reference()'s, and for what f16's least step is worth where V is
+# smaller than the reference follows it (rows under 2^-107): 2^-32 of that, a
+# position; and f32's own least step.
+@pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
+@pytest.mark.parametrize("size", [-80, -95, -105, -112, -120, 93])
+def test_values_of_one_size(ctx, form, precision, size):
+    p = Pool(ctx, np.random.default_rng(101), precision, 2, 64, 32, [150, 40])
+    p.push([150, 40], v=p.rows(190) * np.float32(2.0 ** size))
+    q = (p.rng.standard_normal((50, 4, 64)) * 1.5).astype(np.float32)
+    got = p.cache.attend(0, p.batch([30, 20]), 4, q)
+    for s, (a, e) in enumerate(((0, 30), (30, 50))):
+        k, v = p.held(s)
+        want, tol = reference(q[a:e], k, v, len(k) - (e - a), 0.125)
+        err = np.abs(got[a:e] - want)
+        assert np.all(err <= tol + len(k) * 2.0 ** -139 + 2.0 ** -149), np.max(err) / np.max(np.abs(want))
+        assert np.linalg.norm(err) <= 2.0 ** -10 * np.linalg.norm(want)
