@@ -280,10 +280,13 @@ __device__ __forceinline__ int load_q(const float *x, int hd, F dim0, float (&v)
     return amax;
 }
 // The power of two that brings a query under 2^15, inverted, and the score, in
-// powers of two, of an accumulated product of 1.
+// powers of two, of an accumulated product of 1: not zero, by which a hidden
+// position's -infinity would be NaN (scores that small are all alike: a product is
+// under 2^120), and not infinite, by which a product of zero would be.
 __device__ __forceinline__ float q_scale(int amax, float scale, float &rowf) {
     const int e = min(max((amax >> 23) - 126 - 15, -126), 113);
-    rowf = (scale * 1.44269504088896341f) * __builtin_bit_cast(float, (127 + e) << 23);
+    const float f = scale * (1.44269504088896341f * __builtin_bit_cast(float, (127 + e) << 23));
+    rowf = fminf(fmaxf(f, 0x1p-149f), 3.40282347e38f);
     return __builtin_bit_cast(float, (127 - e) << 23);
 }
 // 1 / 2^k from 2^k

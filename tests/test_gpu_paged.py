@@ -938,3 +938,25 @@ def test_values_of_one_size(ctx, form, precision, size):
         err = np.abs(got[a:e] - want)
         assert np.all(err <= tol + len(k) * 2.0 ** -139 + 2.0 ** -149), np.max(err) / np.max(np.abs(want))
         assert np.linalg.norm(err) <= 2.0 ** -10 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
+@pytest.mark.parametrize("scale, size", [(0.125, 1.0), (3.0, 1.0), (1e-3, 1e3), (1e-8, 1.0), (1e-20, 1e19), (1e-38, 1.0),
+                                         (1e-45, 1.0), (2.0 ** 120, 2.0 ** -120), (3e38, 2.0 ** -127)])
+def test_scales(ctx, form, precision, scale, size):
+    # small and large ones beside queries that are zero, and of about their inverse
+    p = Pool(ctx, np.random.default_rng(103), precision, 2, 64, 32, [90, 40])
+    p.push([90, 40])
+    q = (p.rng.standard_normal((50, 4, 64)) * size).astype(np.float32)
+    q[::3] = 0
+    q[1::3, 1] = 0
+    p.check([20, 30], 4, q=q, scale=scale)
+    p.check([20, 30], 4, q=q, scale=scale, window=37, sinks=3)
+
+
+@pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
+def test_keys_of_zeros_weigh_alike_at_any_scale(ctx, form, precision):
+    p = Pool(ctx, np.random.default_rng(107), precision, 2, 64, 32, [90])
+    p.push([90], k=np.zeros((90, 2, 64), np.float32))
+    for scale in (1e-45, 1.0, 3e38):
+        p.check([20], 4, scale=scale)
