@@ -202,8 +202,9 @@ struct Job {
 };
 
 __device__ __forceinline__ void find_range(const Args &a, Job &w) {
-    w.p_lo = w.first + w.row0 / a.group;
-    w.p_hi = w.first + (w.row0 + w.nr - 1) / a.group;
+    // named scalars (the vector unit divides): so is what is made of them
+    w.p_lo = __builtin_amdgcn_readfirstlane(w.first + w.row0 / a.group);
+    w.p_hi = __builtin_amdgcn_readfirstlane(w.first + (w.row0 + w.nr - 1) / a.group);
     w.range = range_of(w.p_lo, w.p_hi, a.b.max_pages << a.page_shift, a.window, a.sinks);
     w.t_at = 0;
     w.t_end = w.range.n;
