@@ -827,11 +827,15 @@ constexpr int waves_for(int es, int d, int rows) {
 }
 
 // A workgroup takes ROWS rows: its waves share 8, 16 or 32, or take 32 of 128
-// each; with 32 and 128 a sequence of FEW rows or less goes to few_rows.
+// each; with 32 and 128 a sequence of FEW rows or less goes to few_rows.  Where
+// 128 leave 32 or less to a workgroup, its waves share those: one wave alone would
+// go over the whole of the positions (a prompt of 3000 beside 63 single tokens
+// behind 3000 to 4000, 32 heads on 2 of 128: i8 282 us against 183, f32 517 against
+// 390).
 template <int ES, int D, int ROWS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(waves_for(ES, D, ROWS))))
 void attn_kernel(Args a) {
-    constexpr int REGS = ROWS == 32 ? D / 2 : D / 4;  // of a lane, that join_waves takes
+    constexpr int REGS = ROWS > 16 ? D / 2 : D / 4;  // of a lane, that join_waves takes
     __shared__ __attribute__((aligned(16))) float lds[join_floats<REGS>()];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Job w;
@@ -861,9 +865,9 @@ void attn_kernel(Args a) {
         few_rows<ES, D, ROWS>(a, w, wave, lds);
     } else if (seq_rows * a.group <= FEW) {
         few_rows<ES, D, FEW>(a, w, wave, lds);
-    } else if constexpr (ROWS == 32) {
+    } else if (ROWS == 32 || w.nr <= 32) {
         many_rows<ES, D, 4>(a, w, wave, lds);
-    } else {
+    } else if constexpr (ROWS == 128) {
         w.row0 += 32 * wave;
         w.nr = min(w.nr - 32 * wave, 32);
         if (w.nr > 0) many_rows<ES, D, 1>(a, w, wave, nullptr);
@@ -1008,14 +1012,17 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
     // of 32 heads of 128, f16: 5.9 us against 8.5; 300: 12.0 against 12.6; 100
     // behind 3000, i8: 30 against 26, f32: 60 against 39).  Else 128 rows a
     // workgroup, whose waves read the same K and V at about the same time, where
-    // that alone fills the device (a 6000-token prompt, f16: 580 us against 618
-    // with 32 and 747 with 16), 32 where it does not.
+    // rows enough to fill as many waves as the device holds come together (a
+    // 6000-token prompt, f16: 580 us against 618 with 32 and 747 with 16), 32 where
+    // they do not (64 sequences of 10 to 20 new tokens, 32 heads on 8 of 128, i8: 174
+    // us with 32 and 217 with 128; 300 of them, f16: 284 and 261).  Rows count, not
+    // workgroups: one that a sequence's few rows leave nearly empty is no reason.
     const size_t rows = b.row_start ? SIZE_MAX : (size_t)b.per * group, cus = (size_t)cu_count;
     const size_t resident = cus * waves_for(kv->es, kv->d, 32);  // many_rows' workgroups
     const bool small = tiles(16) * kv->n_kv_head * over(16) <= 16 * cus;
     p.tile_rows = rows <= 8                                            ? 8
                   : rows <= 16 || small                              ? 16
-                  : tiles(128) * kv->n_kv_head >= resident           ? 128
+                  : (size_t)b.n_rows * n_head / 128 >= resident      ? 128
                                                                      : 32;
     // for experiments, and for tests of each form: any form does any call
     const int form = env_int("KVAD_PAGED_TILE", 0);

@@ -960,3 +960,22 @@ def test_keys_of_zeros_weigh_alike_at_any_scale(ctx, form, precision):
     p.push([90], k=np.zeros((90, 2, 64), np.float32))
     for scale in (1e-45, 1.0, 3e38):
         p.check([20], 4, scale=scale)
+
+
+@pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
+@pytest.mark.parametrize("H, kv, hd", [(12, 2, 64), (32, 8, 128), (10, 1, 256)])
+def test_short_sequences_share_a_workgroups_waves_in_the_widest_form(ctx, monkeypatch, precision, H, kv, hd):
+    # sequences of 9 to 32 rows (x group), each over the whole of its cache:
+    # 128 rows a workgroup give them its four waves, as 32 do, to the bit
+    rng = np.random.default_rng(109)
+    p = Pool(ctx, rng, precision, kv, hd, 64, [400, 90, 700, 300])
+    p.push([400, 90, 700, 300])
+    group = H // kv
+    counts = [-(-9 // group), 32 // group, 0, 32 // group - 1]
+    q = rng.standard_normal((sum(counts), H, hd)).astype(np.float32)
+    monkeypatch.setenv("KVAD_PAGED_SPLITS", "1")
+    outs = []
+    for tile in ("32", "128"):
+        monkeypatch.setenv("KVAD_PAGED_TILE", tile)
+        outs.append(p.check(counts, H, q=q, got=p.cache.attend(0, p.batch(counts), H, q)))
+    np.testing.assert_array_equal(*outs)
