@@ -979,3 +979,61 @@ def test_short_sequences_share_a_workgroups_waves_in_the_widest_form(ctx, monkey
         monkeypatch.setenv("KVAD_PAGED_TILE", tile)
         outs.append(p.check(counts, H, q=q, got=p.cache.attend(0, p.batch(counts), H, q)))
     np.testing.assert_array_equal(*outs)
+
+
+# The error of random rows as a whole, which the bound of an element (a worst
+# case) does not hold: dropping the low piece of q, a weight or a f32 row of K or
+# V is an error of 2^-12 a term, and shows.  With both, each of the three pairs of
+# pieces is off by 2^-22 at most, so by 2^-23 on the average; scores (standard
+# deviation 1.5) by about 1.5 x 2^-23 x log2 e and some 2^-24 of their sum; a
+# weight by that, exp2's 2^-23 and its own pieces; independent from one position
+# to the next, as the values are: 2^-21 of the norm, sums in 32 bits included, and
+# 2^-18 is eight times that.
+@pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
+@pytest.mark.parametrize("H, kv, hd, held, rows, splits", [
+    (4, 2, 128, 5000, 3, ""), (4, 2, 128, 5000, 3, "9"), (2, 1, 256, 700, 20, ""), (2, 1, 256, 2000, 2, "5"),
+    (6, 2, 64, 300, 40, ""), (3, 3, 64, 3000, 1, "1")])
+def test_error_of_the_whole(ctx, form, monkeypatch, precision, H, kv, hd, held, rows, splits):
+    monkeypatch.setenv("KVAD_PAGED_SPLITS", splits)
+    p = Pool(ctx, np.random.default_rng(113), precision, kv, hd, 64, [held + rows])
+    p.push([held + rows])
+    q = (p.rng.standard_normal((rows, H, hd)) * 1.5).astype(np.float32)
+    got = p.cache.attend(0, p.batch([rows]), H, q)
+    want, _ = reference(q, *p.held(0), held, float(np.float32(hd ** -0.5)))
+    assert np.linalg.norm(got - want) <= 2.0 ** -18 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
+@pytest.mark.parametrize("size", [-100, -60, 60, 93])
+def test_keys_of_many_sizes(ctx, form, precision, size):
+    # keys and queries of inverse sizes, beside keys of zeros: common scores
+    p = Pool(ctx, np.random.default_rng(127), precision, 2, 64, 32, [90, 40])
+    k = p.rows(130) * np.float32(2.0 ** size)
+    k[5::7] = 0
+    p.push([90, 40], k=k)
+    q = (p.rng.standard_normal((50, 4, 64)) * 1.5 * 2.0 ** -size).astype(np.float32)
+    p.check([20, 30], 4, q=q)
+
+
+@pytest.mark.parametrize("precision", ["f32", "f16", "i8"])
+def test_scores_as_large_as_their_step_allows(ctx, form, precision):
+    # of up to 2^24, f32's step 1 there: one key for all is a mean to the last
+    # bits still, and one position ahead of all others takes the whole weight
+    rng = np.random.default_rng(131)
+    p = Pool(ctx, rng, precision, 1, 64, 32, [200, 200])
+    one = np.zeros((200, 1, 64), np.float32)
+    one[:, 0, 0] = 2.0 ** 12
+    ahead = one.copy()
+    ahead[77, 0, 0] = 2.0 ** 13
+    v = p.rows(400)
+    p.push([200, 200], k=np.concatenate([one, ahead]), v=v)
+    q = np.zeros((20, 2, 64), np.float32)
+    q[:, 0, 0], q[:, 1, 0] = 2.0 ** 11, -(2.0 ** 11)
+    got = p.cache.attend(0, p.batch([10, 10]), 2, q, scale=1.0)
+    held = [p.held(s)[1].astype(np.float64) for s in range(2)]
+    for i in range(10):
+        mean = held[0][:191 + i, 0].mean(0)
+        assert np.max(np.abs(got[i] - mean)) <= 2.0 ** -20
+        np.testing.assert_allclose(got[10 + i, 0], held[1][77, 0], rtol=2.0 ** -20, atol=2.0 ** -30)
+        others = np.delete(held[1][:191 + i, 0], 77, 0).mean(0)
+        assert np.max(np.abs(got[10 + i, 1] - others)) <= 2.0 ** -20
