@@ -13,6 +13,7 @@
 #include <cstring>
 #include <memory>
 #include <new>
+#include <set>
 
 #include "paged.hpp"
 
@@ -357,7 +358,8 @@ int stage_batch(kh_ctx *ctx, const kh_batch *b, char *p, kh_batch *dev) {
     return KH_OK;
 }
 
-// kh_batch_check, with the number of distinct-page marks as a scratch vector.
+// What kh_batch_check and the host calls check of a batch's arrays; with `writes`
+// the pages that hold new rows are collected, and one that comes twice refused.
 int check_tables(const kh_batch *b, size_t page_size, size_t n_pages, bool writes) {
     const size_t cap = b->max_pages * page_size;
     const size_t per = b->row_start ? 0 : b->n_rows / b->n_seq;
@@ -424,7 +426,6 @@ int kh_paged_new(kh_ctx *ctx, size_t n_layer, size_t n_kv_head, size_t head_dim,
         kv->n_layer = n_layer;
         kv->n_kv_head = n_kv_head;
         kv->head_dim = head_dim;
-        kv->precision = precision;
         kv->es = precision == KH_F32 ? 4 : precision == KH_F16 ? 2 : 1;
         kv->d = stored_dims((int)head_dim);
         kv->page = (int)page_size;

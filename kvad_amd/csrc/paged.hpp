@@ -9,7 +9,7 @@
 struct kh_paged {
     kh_ctx *ctx = nullptr;
     size_t n_layer = 0, n_kv_head = 0, head_dim = 0;
-    int precision = 0, es = 0, d = 0;
+    int es = 0, d = 0;              // bytes an element, dims a row as it is kept
     int page = 0, page_shift = 0;
     size_t n_pages = 0;
     size_t block = 0;               // bytes of one page of one head
