@@ -255,13 +255,15 @@ int kh_mla_attend_dev(kh_ctx *ctx, size_t n_head, const float *q_lat, const floa
  *   KH_F32  as they are
  *   KH_F16  half precision, rounded to nearest, times a power of two: for a
  *           row of a head with largest magnitude amax = f 2^e, 0.5 <= f < 1,
- *           x / 2^(e - 15) is rounded (no row overflows; exponents from -126)
+ *           x / 2^(e - 15) is rounded (exponents from -126)
  *   KH_I8   codes -127 .. 127 times amax / 127, rounded half away from zero
  *           as QActivation::new rounds (quant.rs:1051-1059), but over the
  *           head's row; a scale below 2^-126 is 0
- * and a row with a NaN or an infinity in it reads back as NaN (KH_F32: as it
- * is), and makes the attention of the rows that see it NaN, of no others.
- * Largest magnitude of a value the attention takes: 2^96. */
+ * A value that rounds past f32's range reads back as infinity: KH_F16 from
+ * 2^128 - 2^116 on, KH_I8 the largest floats alone.  A row with a NaN or an
+ * infinity in it reads back as NaN (KH_F32: as it is), and makes the attention
+ * of the rows that see it NaN, of no others.  Largest magnitude of a key or a
+ * value that the attention takes: 2^96. */
 typedef struct kh_paged kh_paged;
 
 /* New rows of some sequences, one call's worth.  Rows row_start[s] ..
@@ -313,14 +315,16 @@ int kh_paged_read_dev(const kh_paged *kv, size_t layer, const kh_batch *b, float
                       size_t v_stride);
 /* Attention of the batch's rows over the cache, their own positions (pushed
  * before) among it: with q and out [n_rows][n_head][head_dim] (rows q_stride
- * and out_stride floats apart, 0: packed; out is not q) and head h reading KV
- * head h / (n_head / n_kv_head), a row at position p weights the positions t
- * in softmax(scale * q . k_t) over 0 <= t <= p; with window > 0 over those with
- * t > p - window or t < sinks alone, and pages in between are not read.  A row
- * that sees nothing is zero.  scale > 0 (model::attend's is
- * 1 / sqrt(head_dim)).  No weight is dropped for its size, unlike kh_attend's;
- * a position's part in the result is held to 2^-32 of the largest weight times
- * the largest |v| that the row sees, or times 2^-107 where all are smaller.
+ * and out_stride floats apart, 0: packed; no row of out lies over one of q) and
+ * head h reading KV head h / (n_head / n_kv_head), a row at position p weights
+ * the positions t in softmax(scale * q . k_t) over 0 <= t <= p; with window > 0
+ * over those with t > p - window or t < sinks alone, and pages in between are
+ * not read.  A row that sees nothing is zero.  scale > 0 (model::attend's is
+ * 1 / sqrt(head_dim)); scores are of up to 2^24 in magnitude: past that f32's
+ * step is more than 1, and results may be infinite or NaN.  No weight is
+ * dropped for its size, unlike kh_attend's; a position's part in the result is
+ * held to 2^-32 of the largest weight times the largest |v| that the row sees,
+ * or times 2^-107 where all are smaller.
  *
  * Calls of few rows over many positions are split over the positions and
  * joined through `ws`, 16-byte aligned device memory of up to

@@ -27,12 +27,12 @@
 // both, and their sums meet in the scores (by a lane move) and at the end.
 //
 // What bounds them.  few_rows: HBM (64 sequences of up to 4000 i8 positions, 8
-// heads of 128: 76 us for 362 MB, 4.8 TB/s, a large copy's rate), or for one
+// heads of 128: 74 us for 362 MB, 4.9 TB/s, a large copy's rate), or for one
 // short sequence the trips to memory and the joining launch.  many_rows: the
-// matrix cores, 49% at work, behind 6 vector instructions a product (a wave
+// matrix cores, 47% at work, behind 6 vector instructions a product (a wave
 // issues one in 8 cycles, so two waves a SIMD, all that 256 registers allow,
-// just fill it): 512 tokens behind 8000, f16, 32 heads of 128: 139 us, 498
-// TFLOP/s of the scores and values or 997 of the products run for them, where a
+// just fill it): 512 tokens behind 8000, f16, 32 heads of 128: 141 us, 490
+// TFLOP/s of the scores and values or 980 of the products run for them, where a
 // large bf16 product of the library reaches 1200.
 #include <algorithm>
 #include <utility>
@@ -974,7 +974,7 @@ size_t few_splits(const kh_paged *kv, size_t blocks, size_t pos_tiles, size_t cu
 // on a CU together half as much again (f32, whose vector instructions are what
 // counts, three quarters); a join its launch and the partials' way out and in.
 // Never more workgroups than find a place at once.  5000 f16 positions, 32 heads
-// on 8 of 128: 20 rows, one split 30 us, 8 or 10 of them 17, 20 of them 20; 200
+// on 8 of 128: 20 rows, one split 45 us, 8 or 10 of them 17, 20 of them 20; 200
 // rows behind 3000, whose one split has 200 workgroups, 33 us against 37 with
 // two; 512 of 14 heads of 64 behind 8000 52 us, with two 49.
 size_t many_splits(const kh_paged *kv, size_t blocks, size_t pos_tiles, size_t cus, size_t resident, size_t items) {
@@ -1013,7 +1013,7 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
     // behind 3000, i8: 30 against 26, f32: 60 against 39).  Else 128 rows a
     // workgroup, whose waves read the same K and V at about the same time, where
     // rows enough to fill as many waves as the device holds come together (a
-    // 6000-token prompt, f16: 580 us against 618 with 32 and 747 with 16), 32 where
+    // 6000-token prompt, f16: 558 us against 621 with 32 and 753 with 16), 32 where
     // they do not (64 sequences of 10 to 20 new tokens, 32 heads on 8 of 128, i8: 174
     // us with 32 and 217 with 128; 300 of them, f16: 284 and 261).  Rows count, not
     // workgroups: one that a sequence's few rows leave nearly empty is no reason.
