@@ -324,7 +324,8 @@ int kh_paged_read_dev(const kh_paged *kv, size_t layer, const kh_batch *b, float
  * step is more than 1, and results may be infinite or NaN.  No weight is
  * dropped for its size, unlike kh_attend's; a position's part in the result is
  * held to 2^-32 of the largest weight times the largest |v| that the row sees,
- * or times 2^-107 where all are smaller.
+ * or to 2^-147 where that is less, and a weight to some 2^-24 of itself for each
+ * power of two that its score and the sizes of V are away from 1.
  *
  * Calls of few rows over many positions are split over the positions and
  * joined through `ws`, 16-byte aligned device memory of up to

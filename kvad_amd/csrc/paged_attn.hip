@@ -57,14 +57,21 @@ constexpr float LOW = -3.0e38f;  // a running maximum that nothing has raised
 // behind: under 2^15, f16's range, and the sums are rescaled for few tiles.
 constexpr float BASE = 8.0f, SLACK = 6.0f;
 // A weight alone is as much smaller or larger as V's scales are large or small,
-// 2^89 (|v| of 2^96 as i8) to 2^-126.  So V_UP powers of two of the product are in
-// the scale, and the reference takes the scales' exponent as V_LOW or more: weights
-// of up to 2^122, 16 of which a lane adds, and of 2^-94 for the largest of a row,
-// with 32 powers of two below it.  Sums are kept at 2^-24 of that, for millions of
-// tiles of the first and normal floats of the second.  What rows of V with scales
-// under 2^V_LOW give is held to up to 5 bits less.
-constexpr int V_UP = 13, V_LOW = -121;
-constexpr float V_SCALE = 0x1p13f, SUM_SCALE = 0x1p-24f, OUT_SCALE = SUM_SCALE / V_SCALE;  // out: values over sum
+// and its exponent, a float, is the less exact the further it is from 0.  So UP
+// powers of two of the product are in the scale, about as many as keep the weights
+// near 1 where V is, and the reference takes the scales' exponent as LEAST or more:
+// f32 and f16, scales of 2^82 (|v| of 2^96) to 2^-126, weights of up to 2^120, of
+// which a lane adds 16, and of 2^-94 for the largest of a row, with 32 powers of
+// two below it; i8, scales of 2^89 on and codes of up to 127, 2^122 and 2^-94, and
+// rows with scales under 2^-121 held to up to 5 bits less.  Sums are kept at 2^-24
+// of that, for millions of tiles of the first and normal floats of the second.
+constexpr float SUM_SCALE = 0x1p-24f;
+template <int ES>
+struct VScale {
+    static constexpr int UP = ES == 1 ? 13 : 20, LEAST = ES == 1 ? -121 : -126;
+    static constexpr float TIMES = ES == 1 ? 0x1p13f : 0x1p20f;
+};
+constexpr float out_scale(int es) { return SUM_SCALE / (es == 1 ? VScale<1>::TIMES : VScale<4>::TIMES); }  // values over sum
 
 struct Args {
     const char *pool;
@@ -77,7 +84,7 @@ struct Args {
     size_t block;
     int n_kv, group, hd, n_pages, page, page_shift;
     int tiles_per, splits, split_tiles, window, sinks;
-    float scale;
+    float scale, out_scale;
 };
 
 __device__ __forceinline__ float shfl(float v, int x) { return __shfl_xor(v, x); }
@@ -109,13 +116,14 @@ template <int N, typename F>
 __device__ __forceinline__ void each(F f) {
     each_(f, std::make_integer_sequence<int, N>{});
 }
-// V's scale at 2^V_UP.  A row of V that is not finite, by its scale, or whose
-// scale is too large for that (i8, from 2^122 on): no part of any sum, and NaN as a
-// score, so that only rows that see it are NaN.
+// V's scale at 2^UP.  A row of V that is not finite, by its scale, or whose scale
+// is too large for that (|v| from 2^122 on): no part of any sum, and NaN as a score,
+// so that only rows that see it are NaN.
+template <int ES>
 __device__ __forceinline__ void only_finite(float &v_scale, float &k_scale) {
-    const bool finite = (__builtin_bit_cast(int, v_scale) & 0x7fffffff) < 0x7f800000 - (V_UP << 23);
+    const bool finite = (__builtin_bit_cast(int, v_scale) & 0x7fffffff) < 0x7f800000 - (VScale<ES>::UP << 23);
     k_scale = finite ? k_scale : __builtin_bit_cast(float, NAN_BITS);
-    v_scale = finite ? v_scale * V_SCALE : 0.0f;
+    v_scale = finite ? v_scale * VScale<ES>::TIMES : 0.0f;
 }
 // the value 8 lanes on, in each row of 16
 __device__ __forceinline__ float other_half(float v) { return dev::dppf<0x128>(v); }
@@ -293,11 +301,15 @@ __device__ __forceinline__ float q_scale(int amax, float scale, float &rowf) {
 // 1 / 2^k from 2^k
 __device__ __forceinline__ float inv_pow2(float s) { return __builtin_bit_cast(float, 0x7f000000 - __builtin_bit_cast(int, s)); }
 
-// The exponent of the largest of V's scales, from the bits of it at 2^V_UP.
-__device__ __forceinline__ float scale_exp(unsigned bits) { return (float)max((int)(bits >> 23) - 127 - V_UP, V_LOW); }
-// 1 / 2^k from 2^(k + V_UP)
+// The exponent of the largest of V's scales, from the bits of it at 2^UP.
+template <int ES>
+__device__ __forceinline__ float scale_exp(unsigned bits) {
+    return (float)max((int)(bits >> 23) - 127 - VScale<ES>::UP, VScale<ES>::LEAST);
+}
+// 1 / 2^k from 2^(k + UP)
+template <int ES>
 __device__ __forceinline__ float inv_v(float s) {
-    return __builtin_bit_cast(float, 0x7f000000 + (V_UP << 23) - __builtin_bit_cast(int, s));
+    return __builtin_bit_cast(float, 0x7f000000u + ((unsigned)VScale<ES>::UP << 23) - __builtin_bit_cast(unsigned, s));
 }
 
 // The sums of four waves over the same rows, column `col` of `cols` a lane, at
@@ -346,7 +358,7 @@ constexpr int join_floats() { return 256 + 2 * (N < 64 ? N : 64) * 64; }
 
 // A lane's part of a row's result, four dims from dim(c) on in o[4 c ..]: into
 // the output, or beside the other splits'.
-template <int N, typename F>
+template <int ES, int N, typename F>
 __device__ __forceinline__ void put_row(const Args &a, const Job &w, const Row &row, const float (&o)[N], float ref,
                                         float sum, bool tells, int stored, F dim) {
     const size_t r = (size_t)(w.seq_row + row.j);
@@ -362,13 +374,13 @@ __device__ __forceinline__ void put_row(const Args &a, const Job &w, const Row &
         return;
     }
     float *to = a.out + r * a.out_stride + (size_t)q_head * a.hd;
+    constexpr float down = out_scale(ES);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int c = 0; c < N / 4; c++)
         if (dim(c) < a.hd)
             *reinterpret_cast<float4u *>(to + dim(c)) =
-                float4u{o[4 * c] * OUT_SCALE * inv, o[4 * c + 1] * OUT_SCALE * inv, o[4 * c + 2] * OUT_SCALE * inv,
-                        o[4 * c + 3] * OUT_SCALE * inv};
+                float4u{o[4 * c] * down * inv, o[4 * c + 1] * down * inv, o[4 * c + 2] * down * inv, o[4 * c + 3] * down * inv};
 }
 
 // Rows of K and V whose raw loads many_rows has one set of registers for: two
@@ -501,10 +513,10 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
         float sk = ks, sv = vs;
         load_s(here);
         __builtin_amdgcn_sched_barrier(0);
-        only_finite(sv, sk);
+        only_finite<ES>(sv, sk);
         float st[16];
         each<16>([&](auto i) { st[i] = here_and_now(sc[i.value] * of_lane<i>(sk)); });
-        const float v_inv = ES == 4 ? inv_v(sv) : 0.0f;
+        const float v_inv = ES == 4 ? inv_v<ES>(sv) : 0.0f;
 
         // ---- weights ----
         unsigned vtop;
@@ -527,7 +539,7 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
 #pragma unroll
         for (int i = 1; i < 16; i++) top = fmaxf(top, st[i]);
         // the reference bounds weight times V's scale
-        const float want = __builtin_fmaf(top, rowf, scale_exp(vtop));
+        const float want = __builtin_fmaf(top, rowf, scale_exp<ES>(vtop));
         if (__any(want > ref + SLACK)) {
             // each row for itself: what it gives does not hang on the rows beside it
             const float all = fmaxf(want, shfl(want, 32));
@@ -540,7 +552,7 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
 #pragma unroll
                 for (int i = 0; i < 16; i++) acc[dt][i] = acc[dt][i] * f;
         }
-        const float shift = BASE - V_UP - ref;
+        const float shift = BASE - VScale<ES>::UP - ref;
         h8 ph[2], pl[2];
         {
             float x[16], part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -595,7 +607,7 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
         if (wave > 0) return;
     }
     if (n >= w.nr) return;
-    put_row(a, w, row, o, ref, sum, h == 0, D, [&](int c) { return 32 * (c >> 2) + 8 * (c & 3) + 4 * h; });
+    put_row<ES>(a, w, row, o, ref, sum, h == 0, D, [&](int c) { return 32 * (c >> 2) + 8 * (c & 3) + 4 * h; });
 }
 
 // ROWS rows, 8 or 16, shared by the workgroup's four waves.
@@ -728,14 +740,14 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
         float sk = ks, sv = vs;
         load_s(here);
         __builtin_amdgcn_sched_barrier(0);
-        only_finite(sv, sk);
+        only_finite<ES>(sv, sk);
         float st[8];
         each<8>([&](auto i) {
             float s = sc[i >> 2][i.value & 3];
             if (PACKED) s = s + other_half(s);
             st[i] = s * of_lane<i>(sk);
         });
-        const float v_inv = ES == 4 ? inv_v(sv) : 0.0f;
+        const float v_inv = ES == 4 ? inv_v<ES>(sv) : 0.0f;
 
         // ---- weights ----
         unsigned vtop;
@@ -755,7 +767,7 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
         float top = st[0];
 #pragma unroll
         for (int i = 1; i < 8; i++) top = fmaxf(top, st[i]);
-        const float want = __builtin_fmaf(top, rowf, scale_exp(vtop));
+        const float want = __builtin_fmaf(top, rowf, scale_exp<ES>(vtop));
         if (__any(want > ref + SLACK)) {
             float all = fmaxf(want, shfl(want, 16));
             all = fmaxf(all, shfl(all, 32));
@@ -766,7 +778,7 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
 #pragma unroll
             for (int db = 0; db < DB; db++) acc[db] = acc[db] * f;
         }
-        const float shift = BASE - V_UP - ref;
+        const float shift = BASE - VScale<ES>::UP - ref;
         h8 ph, pl;
         {
             float x[8], part[2] = {0.0f, 0.0f};
@@ -813,7 +825,7 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
     }
     join_waves(o, ref, sum, wave, lane, n, z == 0, lds);
     if (wave > 0 || n >= w.nr) return;
-    put_row(a, w, row, o, ref, sum, z == 0, D, [&](int c) { return 16 * c + 4 * z; });
+    put_row<ES>(a, w, row, o, ref, sum, z == 0, D, [&](int c) { return 16 * c + 4 * z; });
 }
 
 constexpr int FEW = 8;  // rows (x group) of a sequence that few_rows takes beside longer ones
@@ -933,7 +945,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args a) {
     float *o = a.out + (size_t)row * a.out_stride + (item - (size_t)row * n_head) * a.hd;
 #pragma unroll
     for (int e = 0; e < E; e++)
-        if (E * lane + e < a.hd) o[E * lane + e] = acc[e] * OUT_SCALE * inv;
+        if (E * lane + e < a.hd) o[E * lane + e] = acc[e] * a.out_scale * inv;
 }
 
 template <int ES, int D>
@@ -1082,6 +1094,7 @@ int launch_attn(kh_ctx *ctx, const AttnCall &c, const AttnPlan &p) {
     a.window = c.window;
     a.sinks = c.sinks;
     a.scale = c.scale;
+    a.out_scale = out_scale(kv->es);
     const unsigned blocks = (unsigned)((size_t)p.tiles * kv->n_kv_head * p.splits);
     if (kv->es == 4) return launch_d<4>(kv->d, a, p, blocks, items, ctx->stream);
     if (kv->es == 2) return launch_d<2>(kv->d, a, p, blocks, items, ctx->stream);
