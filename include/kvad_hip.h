@@ -340,6 +340,48 @@ int kh_paged_attend_dev(kh_paged *kv, size_t layer, const kh_batch *b, size_t n_
 int kh_paged_attend_ws(const kh_paged *kv, const kh_batch *b, size_t n_head, size_t window, size_t sinks,
                        size_t *bytes);
 
+/* ---- page tables on the device ------------------------------------------ */
+
+/* Tables of a kh_batch advanced by the device itself, so that a captured step
+ * needs no host between its replays: which pages a sequence has, which are free,
+ * and where each new row goes.  All arrays are the caller's device memory, read
+ * and written when the work runs, and a kh_batch over len, pages and row_start
+ * is what the cache's calls take.  n_seq is up to 4096, page_size as the
+ * cache's.  Calls on one table are made on one stream, one behind the other. */
+typedef struct kh_page_table {
+    size_t n_seq, max_pages, page_size, n_pages;
+    int32_t *len;        /* [n_seq]: positions each sequence holds */
+    int32_t *pages;      /* [n_seq][max_pages]: -1 where it has no page */
+    int32_t *row_start;  /* [n_seq + 1]: the last step's rows, as kh_batch's */
+    int32_t *free_pages; /* [n_pages]: a stack, its top at n_free[0] - 1 */
+    int32_t *n_free;     /* [1] */
+    int32_t *status;     /* [4]: why the last call was refused (0: it was not),
+                            how many have been, and two of the library's own */
+} kh_page_table;
+/* What a refused call leaves in status[0]. */
+#define KH_PAGES_SHORT 1     /* fewer free pages than the step needs */
+#define KH_PAGES_TOO_LONG 2  /* a sequence past max_pages */
+#define KH_PAGES_ROWS 3      /* rows below zero, or more in all than n_rows */
+#define KH_PAGES_TABLE 4     /* lengths or n_free out of range, or more pages
+                                given back than the stack holds */
+/* No sequence holds a position, every page is free, page 0 on top. */
+int kh_pages_init_dev(kh_ctx *ctx, const kh_page_table *t);
+/* rows[s] new rows for each sequence: len[s] += rows[s], row_start their sums,
+ * and the pages that the new positions need taken from the stack's top, the
+ * first sequence's first.  position[r] and slot[r] (each n_rows, or NULL) are a
+ * row's position in its sequence and its page * page_size + position %
+ * page_size; -1 in both for rows behind the last sequence's.  A step that
+ * cannot be done whole is refused whole, on the device: len, pages and the stack
+ * stay, row_start is all zeros (no sequence has a row: what follows in the step
+ * writes none), positions and slots are -1, and status says why. */
+int kh_pages_step_dev(kh_ctx *ctx, const kh_page_table *t, const int32_t *rows, size_t n_rows, int32_t *position,
+                      int64_t *slot);
+/* Sequences cut to their first keep[s] positions (0: ended; below zero or from
+ * len[s] on: left as they are): pages behind those go back on the stack, the
+ * last sequence's last page first, which undoes a step.  Pages that two tables
+ * name are the caller's to keep count of.  row_start stays the last step's. */
+int kh_pages_release_dev(kh_ctx *ctx, const kh_page_table *t, const int32_t *keep);
+
 /* ---- decode glue (device pointers, asynchronous on the context's stream) */
 
 /* tensor::rms_norm (tensor.rs:329-333) over m rows of n:
@@ -351,6 +393,29 @@ int kh_rms_norm_dev(kh_ctx *ctx, const float *x, const float *w, size_t m, size_
  * caller's tables [max_pos][half] (Rope::tables, tensor.rs:377-387). */
 int kh_rope_dev(kh_ctx *ctx, const float *cos_t, const float *sin_t, size_t half, float *x, size_t m,
                 size_t n_vec, size_t pos0, int interleaved);
+/* kh_rope_dev's rotation of rows at positions of their own, as a batch of many
+ * sequences has them: row r of x and of out ([m] rows x_stride and out_stride
+ * floats apart, 0: packed) begins with n_vec vectors of 2*half, rotated by row
+ * position[r] of cos_t/sin_t [max_pos][half].  position is a device array, read
+ * when the work runs (kh_pages_step_dev writes one).  A row whose position is
+ * not in 0 .. max_pos - 1 is not written.  out is x (in place, the strides
+ * alike) or apart from it; what a row holds behind its vectors stays out. */
+int kh_rope_rows_dev(kh_ctx *ctx, const float *cos_t, const float *sin_t, size_t half, size_t max_pos, const float *x,
+                     size_t x_stride, const int32_t *position, size_t m, size_t n_vec, int interleaved, float *out,
+                     size_t out_stride);
+/* The end of a block and the norm before the next one, over m rows of n: y, the
+ * block's output, normed with post_w (NULL: as it is), times gate (NULL: 1; rows
+ * gate_stride floats apart, 0: one row for all) and scale is added to the
+ * residual x, and that is normed with pre_w (NULL, and then out NULL too: not):
+ *   t = y * (1 / sqrt(mean(y^2) + eps)) * post_w
+ *   x_out = x + (t * gate) * scale
+ *   out = x_out * (1 / sqrt(mean(x_out^2) + eps)) * pre_w
+ * x_out may be x or y, out may be x or y; what is written is otherwise apart
+ * from what is read, and x_out from out.  Sums of squares are f32, each in a
+ * fixed order: |x| and |y| of up to 2^63 / sqrt(n). */
+int kh_norm_residual_dev(kh_ctx *ctx, const float *x, const float *y, const float *post_w, const float *gate,
+                         size_t gate_stride, float scale, const float *pre_w, size_t m, size_t n, float eps,
+                         float *x_out, float *out);
 /* swiglu_inplace (tensor.rs:344-350): gate[i] = silu(gate[i]) * up[i]. */
 int kh_swiglu_dev(kh_ctx *ctx, float *gate, const float *up, size_t n);
 /* softmax_inplace (tensor.rs:297-308) over each of m rows of n, in place. */

@@ -26,7 +26,7 @@ import numpy as np
 
 __all__ = [
     "F32", "Q8", "Q4", "Q4K", "KvadError", "Declined", "lib", "Context", "Weight", "matvec_many",
-    "KvCache", "Spec", "attend", "F16", "I8", "Batch", "PagedCache", "LIB_PATH", "Moe", "QCache", "mla_attend", "mla_attend_dev", "Llm", "LlmSpec", "Parked", "SOFTMAX", "SIGMOID", "GREEDY", "GROUP_LIMITED", "NOAUX_TC",
+    "KvCache", "Spec", "attend", "F16", "I8", "Batch", "PagedCache", "PageTable", "LIB_PATH", "Moe", "QCache", "mla_attend", "mla_attend_dev", "Llm", "LlmSpec", "Parked", "SOFTMAX", "SIGMOID", "GREEDY", "GROUP_LIMITED", "NOAUX_TC",
 ]
 
 F32, Q8, Q4, Q4K = 0, 1, 2, 3
@@ -124,8 +124,13 @@ _SIGS = {
     "kh_paged_attend": (C.c_int, [_p, _sz, _p, _sz, _p, C.c_float, _sz, _sz, _p]),
     "kh_paged_attend_dev": (C.c_int, [_p, _sz, _p, _sz, _p, _sz, C.c_float, _sz, _sz, _p, _sz, _p, _sz]),
     "kh_paged_attend_ws": (C.c_int, [_p, _p, _sz, _sz, _sz, C.POINTER(_sz)]),
+    "kh_pages_init_dev": (C.c_int, [_p, _p]),
+    "kh_pages_step_dev": (C.c_int, [_p, _p, _p, _sz, _p, _p]),
+    "kh_pages_release_dev": (C.c_int, [_p, _p, _p]),
     "kh_rms_norm_dev": (C.c_int, [_p, _p, _p, _sz, _sz, C.c_float, _p]),
     "kh_rope_dev": (C.c_int, [_p, _p, _p, _sz, _p, _sz, _sz, _sz, C.c_int]),
+    "kh_rope_rows_dev": (C.c_int, [_p, _p, _p, _sz, _sz, _p, _sz, _p, _sz, _sz, C.c_int, _p, _sz]),
+    "kh_norm_residual_dev": (C.c_int, [_p, _p, _p, _p, _p, _sz, C.c_float, _p, _sz, _sz, C.c_float, _p, _p]),
     "kh_swiglu_dev": (C.c_int, [_p, _p, _p, _sz]),
     "kh_softmax_dev": (C.c_int, [_p, _p, _sz, _sz]),
     "kh_llm_new": (C.c_int, [_p, _p, C.POINTER(_p)]),
@@ -679,6 +684,33 @@ class PagedCache:
         return self.head_dim ** -0.5 if scale is None else scale
 
 
+class PageTable(C.Structure):
+    """kh_page_table: the tables of a Batch advanced on the device, over the
+    caller's device arrays (int32): len [n_seq], pages [n_seq, max_pages],
+    row_start [n_seq + 1], free [n_pages], n_free [1], status [4]."""
+    _fields_ = [("n_seq", _sz), ("max_pages", _sz), ("page_size", _sz), ("n_pages", _sz), ("len", _p), ("pages", _p),
+                ("row_start", _p), ("free_pages", _p), ("n_free", _p), ("status", _p)]
+    # status[0] of a refused call
+    SHORT, TOO_LONG, ROWS, TABLE = 1, 2, 3, 4
+
+    def init_dev(self, ctx: Context) -> None:
+        """No sequence holds a position and every page is free."""
+        _check(lib.kh_pages_init_dev(ctx.h, C.byref(self)))
+
+    def step_dev(self, ctx: Context, rows_ptr: int, n_rows: int, position_ptr: int | None = None,
+                 slot_ptr: int | None = None) -> None:
+        """rows[s] new rows for each sequence, with pages, positions (int32) and slots (int64)."""
+        _check(lib.kh_pages_step_dev(ctx.h, C.byref(self), rows_ptr, n_rows, position_ptr, slot_ptr))
+
+    def release_dev(self, ctx: Context, keep_ptr: int) -> None:
+        """Sequences cut to their first keep[s] positions, pages behind those free again."""
+        _check(lib.kh_pages_release_dev(ctx.h, C.byref(self), keep_ptr))
+
+    def batch(self, n_rows: int, max_len: int = 0) -> Batch:
+        """The last step's rows, as the cache's calls take them."""
+        return Batch(self.n_seq, n_rows, self.len, self.pages, self.max_pages, row_start=self.row_start, max_len=max_len)
+
+
 def mla_attend(ctx: Context, cache: "KvCache", layer: int, n_head: int, q_lat, q_pe, n_positions: int,
                scale: float) -> np.ndarray:
     """The latent-attention core of DeepSeek's Model::attend (model/deepseek.rs:553-591)
@@ -794,6 +826,21 @@ def rms_norm_dev(ctx: Context, x_ptr: int, w_ptr: int, m: int, n: int, eps: floa
 def rope_dev(ctx: Context, cos_ptr: int, sin_ptr: int, half: int, x_ptr: int, m: int, n_vec: int, pos0: int,
              interleaved: bool = False) -> None:
     _check(lib.kh_rope_dev(ctx.h, cos_ptr, sin_ptr, half, x_ptr, m, n_vec, pos0, int(interleaved)))
+
+
+def rope_rows_dev(ctx: Context, cos_ptr: int, sin_ptr: int, half: int, max_pos: int, x_ptr: int, position_ptr: int, m: int,
+                  n_vec: int, out_ptr: int, interleaved: bool = False, x_stride: int = 0, out_stride: int = 0) -> None:
+    """rope_dev of rows at positions of their own, read from the device."""
+    _check(lib.kh_rope_rows_dev(ctx.h, cos_ptr, sin_ptr, half, max_pos, x_ptr, x_stride, position_ptr, m, n_vec,
+                                int(interleaved), out_ptr, out_stride))
+
+
+def norm_residual_dev(ctx: Context, x_ptr: int, y_ptr: int, m: int, n: int, eps: float, x_out_ptr: int,
+                      post_ptr: int | None = None, gate_ptr: int | None = None, gate_stride: int = 0, scale: float = 1.0,
+                      pre_ptr: int | None = None, out_ptr: int | None = None) -> None:
+    """x_out = x + scale * gate * norm(y; post), out = norm(x_out; pre): the end of a block and the norm before the next."""
+    _check(lib.kh_norm_residual_dev(ctx.h, x_ptr, y_ptr, post_ptr, gate_ptr, gate_stride, scale, pre_ptr, m, n, eps,
+                                    x_out_ptr, out_ptr))
 
 
 def swiglu_dev(ctx: Context, gate_ptr: int, up_ptr: int, n: int) -> None:

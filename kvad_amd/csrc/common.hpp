@@ -9,6 +9,7 @@
 #include <cstdlib>
 #include <map>
 #include <mutex>
+#include <new>
 #include <set>
 #include <string>
 #include <vector>
@@ -44,6 +45,18 @@ inline bool capturing(hipStream_t stream) {
 inline int env_int(const char *name, int dflt) {
     const char *v = getenv(name);
     return v && *v ? atoi(v) : dflt;
+}
+
+// No exception leaves a C entry whose body runs in this.
+template <typename F>
+int guarded(F f) {
+    try {
+        return f();
+    } catch (const std::bad_alloc &) {
+        return KH_ENOMEM;
+    } catch (...) {
+        return KH_EHIP;
+    }
 }
 
 // ---- device workspace ---------------------------------------------------

@@ -386,18 +386,6 @@ int check_tables(const kh_batch *b, size_t page_size, size_t n_pages, bool write
     return KH_OK;
 }
 
-// No exception leaves a C entry.
-template <typename F>
-int guarded(F f) {
-    try {
-        return f();
-    } catch (const std::bad_alloc &) {
-        return KH_ENOMEM;
-    } catch (...) {
-        return KH_EHIP;
-    }
-}
-
 }  // namespace
 }  // namespace paged
 }  // namespace kh

@@ -1,0 +1,332 @@
+// Page tables advanced on the device (kh_pages_*): which sequence's rows come
+// where, the pages they need from a stack of free ones, each row's position and
+// slot, and pages given back.  No counterpart in the reference, whose caches are
+// one array a conversation.
+//
+// Each call is one launch.  Every workgroup takes the sums over the sequences
+// for itself (two numbers each, in LDS: reading them again costs less than a
+// second launch), then its share of the rows and pages, each found by bisection.
+// The arrays that all of them read, the lengths and the stack's height, are
+// written by the last to finish.  Whether the call can be done is known from
+// the sums: all workgroups find the same, and either all do it or none.
+//
+// What bounds it: trips to memory one behind the other, and the launch.
+#include <algorithm>
+
+#include "common.hpp"
+
+namespace kh {
+namespace pages {
+namespace {
+
+constexpr int THREADS = 256, MAX_SEQ = 4096, ROWS = 4;  // rows a thread takes at a time
+constexpr int LIMIT = 1 << 30;                          // positions and rows are below it
+
+// kh_page_table's status
+enum { REASON, REFUSED, ARRIVED = 3 };
+enum { DONE, SHORT, TOO_LONG, BAD_ROWS, BAD_TABLE };
+
+struct Args {
+    int32_t *len, *pages, *row_start, *free_pages, *n_free, *status;
+    const int32_t *rows;  // of a step; a release's positions to keep
+    int32_t *position;
+    int64_t *slot;
+    int n_seq, max_pages, page_shift, n_pages, n_rows;
+};
+
+__device__ __forceinline__ int pages_for(int positions, int shift) { return (int)(((unsigned)positions + (1u << shift) - 1) >> shift); }
+// a sum that stops at LIMIT: of operands up to LIMIT, whatever their order
+__device__ __forceinline__ int add(int a, int b) { return (int)min((unsigned)a + (unsigned)b, (unsigned)LIMIT); }
+
+// What a call makes of a sequence: rows (none for a release) and pages given or
+// taken back, from where on in its table.
+struct Change {
+    int rows, pages, first, bad;
+};
+template <bool STEP>
+__device__ __forceinline__ Change change_of(const Args &a, int s) {
+    const int cap = a.max_pages << a.page_shift;
+    int len = a.len[s], arg = a.rows[s];
+    Change c{0, 0, 0, DONE};
+    if (len < 0 || len > cap) {
+        c.bad = BAD_TABLE;
+    } else if (STEP) {
+        if (arg < 0 || arg > a.n_rows) {
+            c.bad = BAD_ROWS;
+        } else if (arg > cap - len) {
+            c.bad = TOO_LONG;
+            c.rows = arg;
+        } else {
+            c.rows = arg;
+            c.first = pages_for(len, a.page_shift);
+            c.pages = pages_for(len + arg, a.page_shift) - c.first;
+        }
+    } else if (arg >= 0 && arg < len) {
+        c.first = pages_for(arg, a.page_shift);
+        c.pages = pages_for(len, a.page_shift) - c.first;
+    }
+    return c;
+}
+
+// The sums before each sequence, in LDS, and over all of them.
+struct Sums {
+    int rows[MAX_SEQ], pages[MAX_SEQ];
+    int wave_rows[THREADS / 64], wave_pages[THREADS / 64];
+};
+__device__ __forceinline__ int scan(int v, int lane) {
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(v, o);
+        if (lane >= o) v = add(v, up);
+    }
+    return v;
+}
+// Returns the worst of the sequences' faults, in every thread.
+template <bool STEP>
+__device__ __forceinline__ int sum_up(const Args &a, Sums &s, int &rows, int &pages) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int each = (a.n_seq + THREADS - 1) / THREADS, from = threadIdx.x * each, to = min(from + each, a.n_seq);
+    int r = 0, p = 0, bad = DONE;
+    for (int i = from; i < to; i++) {
+        const Change c = change_of<STEP>(a, i);
+        s.rows[i] = r;
+        s.pages[i] = p;
+        r = add(r, c.rows);
+        p = add(p, c.pages);
+        bad = max(bad, c.bad);
+    }
+    const int r_to = scan(r, lane), p_to = scan(p, lane);
+    if (lane == 63) {
+        s.wave_rows[wave] = r_to;
+        s.wave_pages[wave] = p_to;
+    }
+    const int worst = __syncthreads_or(bad == BAD_TABLE) ? BAD_TABLE : __syncthreads_or(bad == BAD_ROWS) ? BAD_ROWS : __syncthreads_or(bad == TOO_LONG) ? TOO_LONG : DONE;
+    int r0 = __shfl_up(r_to, 1), p0 = __shfl_up(p_to, 1);
+    if (lane == 0) r0 = p0 = 0;
+    rows = pages = 0;
+    for (int w = 0; w < THREADS / 64; w++) {
+        if (w < wave) {
+            r0 = add(r0, s.wave_rows[w]);
+            p0 = add(p0, s.wave_pages[w]);
+        }
+        rows = add(rows, s.wave_rows[w]);
+        pages = add(pages, s.wave_pages[w]);
+    }
+    for (int i = from; i < to; i++) {
+        s.rows[i] = add(s.rows[i], r0);
+        s.pages[i] = add(s.pages[i], p0);
+    }
+    __syncthreads();
+    return worst;
+}
+// The last sequence that starts at i or before it: the one that has item i.
+__device__ __forceinline__ int find(const int *starts, int n, int i) {
+    int lo = 0, hi = n;  // starts[lo] <= i < starts[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (starts[mid] <= i) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Whether this workgroup is the last of the launch to come here.
+__device__ __forceinline__ bool last_one(const Args &a) {
+    __syncthreads();
+    if (gridDim.x == 1) return true;
+    __shared__ int s_last;
+    if (threadIdx.x == 0) {
+        __threadfence();
+        s_last = atomicAdd(&a.status[ARRIVED], 1) == (int)gridDim.x - 1;
+        if (s_last) a.status[ARRIVED] = 0;
+    }
+    __syncthreads();
+    return s_last;
+}
+__device__ __forceinline__ void report(const Args &a, int reason) {
+    a.status[REASON] = reason;
+    if (reason != DONE) a.status[REFUSED] = a.status[REFUSED] + 1;
+}
+
+__global__ __launch_bounds__(THREADS) void step_kernel(Args a) {
+    __shared__ Sums s;
+    int rows, need;
+    int reason = sum_up<true>(a, s, rows, need);
+    const int n_free = *a.n_free;
+    if (n_free < 0 || n_free > a.n_pages) reason = BAD_TABLE;
+    else if (reason == DONE && rows > a.n_rows) reason = BAD_ROWS;
+    else if (reason == DONE && need > n_free) reason = SHORT;
+    if (reason != DONE) rows = need = 0;
+    const int at = blockIdx.x * THREADS + threadIdx.x, step = gridDim.x * THREADS;
+    // pages into the tables, from the stack's top
+    for (int i = at; i < need; i += step) {
+        const int q = find(s.pages, a.n_seq, i);
+        a.pages[(size_t)q * a.max_pages + pages_for(a.len[q], a.page_shift) + (i - s.pages[q])] = a.free_pages[n_free - 1 - i];
+    }
+    // positions and slots
+    const int mask = (1 << a.page_shift) - 1;
+    for (int i = at * ROWS; i < a.n_rows; i += step * ROWS) {
+        int q = i < rows ? find(s.rows, a.n_seq, i) : 0;
+        int len = a.len[q], next = q + 1 < a.n_seq ? s.rows[q + 1] : rows, column = -1, page = -1;
+#pragma unroll
+        for (int e = 0; e < ROWS; e++) {
+            const int r = i + e;
+            if (r >= a.n_rows) break;
+            int position = -1;
+            int64_t slot = -1;
+            if (r < rows) {
+                if (r >= next) {
+                    do next = ++q + 1 < a.n_seq ? s.rows[q + 1] : rows;
+                    while (r >= next);
+                    len = a.len[q];
+                    column = -1;
+                }
+                position = len + (r - s.rows[q]);
+                const int c = position >> a.page_shift;
+                if (c != column) {
+                    column = c;
+                    const int fresh = c - pages_for(len, a.page_shift);
+                    page = fresh < 0 ? a.pages[(size_t)q * a.max_pages + c] : a.free_pages[n_free - 1 - s.pages[q] - fresh];
+                }
+                slot = (int64_t)page << a.page_shift | (position & mask);
+                if (page < 0 || page >= a.n_pages) slot = -1;
+            }
+            if (a.position) a.position[r] = position;
+            if (a.slot) a.slot[r] = slot;
+        }
+    }
+    if (blockIdx.x == 0) {
+        for (int q = threadIdx.x; q < a.n_seq; q += THREADS) a.row_start[q] = reason == DONE ? s.rows[q] : 0;
+        if (threadIdx.x == 0) a.row_start[a.n_seq] = rows;
+    }
+    if (!last_one(a)) return;
+    if (reason == DONE)
+        for (int q = threadIdx.x; q < a.n_seq; q += THREADS) a.len[q] = a.len[q] + a.rows[q];
+    if (threadIdx.x == 0) {
+        if (reason == DONE) *a.n_free = n_free - need;
+        report(a, reason);
+    }
+}
+
+__global__ __launch_bounds__(THREADS) void release_kernel(Args a) {
+    __shared__ Sums s;
+    int rows, back;
+    int reason = sum_up<false>(a, s, rows, back);
+    const int n_free = *a.n_free;
+    if (n_free < 0 || n_free > a.n_pages || back > a.n_pages - n_free) reason = BAD_TABLE;
+    if (reason != DONE) back = 0;
+    // the reverse of the order in which a step gives pages
+    for (int i = blockIdx.x * THREADS + threadIdx.x; i < back; i += gridDim.x * THREADS) {
+        const int q = find(s.pages, a.n_seq, i);
+        int32_t *entry = &a.pages[(size_t)q * a.max_pages + pages_for(a.rows[q], a.page_shift) + (i - s.pages[q])];
+        a.free_pages[n_free + back - 1 - i] = *entry;
+        *entry = -1;
+    }
+    if (!last_one(a)) return;
+    if (reason == DONE)
+        for (int q = threadIdx.x; q < a.n_seq; q += THREADS) {
+            const int keep = a.rows[q];
+            if (keep >= 0 && keep < a.len[q]) a.len[q] = keep;
+        }
+    if (threadIdx.x == 0) {
+        if (reason == DONE) *a.n_free = n_free + back;
+        report(a, reason);
+    }
+}
+
+__global__ __launch_bounds__(THREADS) void init_kernel(Args a) {
+    const size_t at = (size_t)blockIdx.x * THREADS + threadIdx.x, step = (size_t)gridDim.x * THREADS;
+    for (size_t i = at; i < (size_t)a.n_pages; i += step) a.free_pages[i] = a.n_pages - 1 - (int)i;
+    for (size_t i = at; i < (size_t)a.n_seq * a.max_pages; i += step) a.pages[i] = -1;
+    for (size_t i = at; i <= (size_t)a.n_seq; i += step) {
+        a.row_start[i] = 0;
+        if (i < (size_t)a.n_seq) a.len[i] = 0;
+    }
+    if (at < 4) a.status[at] = 0;
+    if (at == 0) *a.n_free = a.n_pages;
+}
+
+bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+int refuse(const char *what, const char *why) { return fail(KH_EINVAL, std::string(what) + ": " + why); }
+
+int check(kh_ctx *ctx, const kh_page_table *t, Args &a, const char *what) {
+    if (!ctx || !t) return refuse(what, "null argument");
+    if (t->n_seq == 0 || t->n_seq > MAX_SEQ) return refuse(what, "needs 1 to 4096 sequences");
+    if (t->page_size < 32 || t->page_size > 1024 || (t->page_size & (t->page_size - 1)))
+        return refuse(what, "pages hold 32, 64, ... or 1024 positions");
+    if (t->max_pages == 0 || t->max_pages > (size_t)LIMIT / t->page_size)
+        return refuse(what, "a sequence holds 1 to 2^30 positions");
+    if (t->n_pages == 0 || t->n_pages > (size_t)LIMIT) return refuse(what, "needs 1 to 2^30 pages");
+    if (!t->len || !t->pages || !t->row_start || !t->free_pages || !t->n_free || !t->status)
+        return refuse(what, "null argument");
+    for (const void *p : {t->len, t->pages, t->row_start, t->free_pages, t->n_free, t->status})
+        if (!aligned(p, 4)) return refuse(what, "the table's arrays are of 32-bit integers");
+    int shift = 0;
+    while (((size_t)1 << shift) < t->page_size) shift++;
+    a = Args{t->len, t->pages, t->row_start, t->free_pages, t->n_free, t->status, nullptr, nullptr, nullptr,
+             (int)t->n_seq, (int)t->max_pages, shift, (int)t->n_pages, 0};
+    return KH_OK;
+}
+unsigned blocks_for(size_t items, unsigned most) {
+    return (unsigned)std::min<size_t>(std::max<size_t>((items + THREADS - 1) / THREADS, 1), most);
+}
+
+}  // namespace
+}  // namespace pages
+}  // namespace kh
+
+using namespace kh;
+using namespace kh::pages;
+
+extern "C" {
+
+int kh_pages_init_dev(kh_ctx *ctx, const kh_page_table *t) {
+    return guarded([&]() -> int {
+        Args a;
+        if (int rc = check(ctx, t, a, "kh_pages_init_dev")) return rc;
+        std::lock_guard<std::recursive_mutex> lock(ctx->mu);
+        (void)hipSetDevice(ctx->device);
+        init_kernel<<<blocks_for(std::max(t->n_pages, t->n_seq * t->max_pages), 1024), THREADS, 0, ctx->stream>>>(a);
+        KH_HIP(hipGetLastError());
+        return KH_OK;
+    });
+}
+
+int kh_pages_step_dev(kh_ctx *ctx, const kh_page_table *t, const int32_t *rows, size_t n_rows, int32_t *position,
+                      int64_t *slot) {
+    return guarded([&]() -> int {
+        Args a;
+        if (int rc = check(ctx, t, a, "kh_pages_step_dev")) return rc;
+        if (!rows) return refuse("kh_pages_step_dev", "null argument");
+        if (!aligned(rows, 4) || !aligned(position, 4) || !aligned(slot, 8))
+            return refuse("kh_pages_step_dev", "rows and positions are 32-bit integers, slots 64-bit ones");
+        if (n_rows >= (size_t)LIMIT) return refuse("kh_pages_step_dev", "2^30 rows or more");
+        a.rows = rows;
+        a.n_rows = (int)n_rows;
+        a.position = position;
+        a.slot = slot;
+        std::lock_guard<std::recursive_mutex> lock(ctx->mu);
+        (void)hipSetDevice(ctx->device);
+        const unsigned blocks = blocks_for(n_rows / ROWS, 2 * (unsigned)ctx->cu_count);
+        step_kernel<<<blocks, THREADS, 0, ctx->stream>>>(a);
+        KH_HIP(hipGetLastError());
+        return KH_OK;
+    });
+}
+
+int kh_pages_release_dev(kh_ctx *ctx, const kh_page_table *t, const int32_t *keep) {
+    return guarded([&]() -> int {
+        Args a;
+        if (int rc = check(ctx, t, a, "kh_pages_release_dev")) return rc;
+        if (!keep) return refuse("kh_pages_release_dev", "null argument");
+        if (!aligned(keep, 4)) return refuse("kh_pages_release_dev", "positions to keep are 32-bit integers");
+        a.rows = keep;
+        std::lock_guard<std::recursive_mutex> lock(ctx->mu);
+        (void)hipSetDevice(ctx->device);
+        const size_t most = std::min(t->n_pages, t->n_seq * t->max_pages);
+        release_kernel<<<blocks_for(most / 16, (unsigned)ctx->cu_count), THREADS, 0, ctx->stream>>>(a);
+        KH_HIP(hipGetLastError());
+        return KH_OK;
+    });
+}
+
+}  // extern "C"
