@@ -43,10 +43,11 @@ extern "C" {
 #define KH_Q4 2
 #define KH_Q4K 3
 /* How a paged KV cache keeps its rows (kh_paged_new), beside KH_F32: half
- * precision, or 8-bit codes, each row of a KV head with a scale of its own.
- * Not precisions of a weight. */
+ * precision, or 8-bit codes, each row of a KV head with a scale of its own, or
+ * 4-bit floats with a scale for every 32 dims.  Not precisions of a weight. */
 #define KH_F16 4
 #define KH_I8 5
+#define KH_MXFP4 6
 
 typedef struct kh_ctx kh_ctx;
 typedef struct kh_weight kh_weight;
@@ -259,8 +260,13 @@ int kh_mla_attend_dev(kh_ctx *ctx, size_t n_head, const float *q_lat, const floa
  *   KH_I8   codes -127 .. 127 times amax / 127, rounded half away from zero
  *           as QActivation::new rounds (quant.rs:1051-1059), but over the
  *           head's row; a scale below 2^-126 is 0
+ *   KH_MXFP4  0, 0.5, 1, 1.5, 2, 3, 4 or 6 (E2M1) and a sign times a power of
+ *           two 2^e for each 32 dims of the head's row from its first on: 3.5 2^e
+ *           <= amax < 7 2^e, the nearest of them, of two as near the one of even
+ *           code; e not under -128, nor more than 26 under the row's largest.
+ *           4.25 bits a value, and 32 a row
  * A value that rounds past f32's range reads back as infinity: KH_F16 from
- * 2^128 - 2^116 on, KH_I8 the largest floats alone.  A row with a NaN or an
+ * 2^128 - 2^116 on, KH_MXFP4 from 1.75 2^127 on, KH_I8 the largest floats alone.  A row with a NaN or an
  * infinity in it reads back as NaN (KH_F32: as it is), and makes the attention
  * of the rows that see it NaN, of no others.  Largest magnitude of a key or a
  * value that the attention takes: 2^96. */
@@ -290,7 +296,7 @@ typedef struct kh_batch {
 
 /* n_pages pages of page_size positions (32, 64, ... 1024) per layer; head_dim a
  * multiple of 4 up to 256 (kept as 64, 128 or 256 dims); precision KH_F32,
- * KH_F16 or KH_I8.  Slots that no row was written to hold zeros. */
+ * KH_F16, KH_I8 or KH_MXFP4.  Slots that no row was written to hold zeros. */
 int kh_paged_new(kh_ctx *ctx, size_t n_layer, size_t n_kv_head, size_t head_dim, int precision, size_t page_size,
                  size_t n_pages, kh_paged **out);
 int kh_paged_free(kh_paged *kv);

@@ -26,11 +26,11 @@ import numpy as np
 
 __all__ = [
     "F32", "Q8", "Q4", "Q4K", "KvadError", "Declined", "lib", "Context", "Weight", "matvec_many",
-    "KvCache", "Spec", "attend", "F16", "I8", "Batch", "PagedCache", "PageTable", "LIB_PATH", "Moe", "QCache", "mla_attend", "mla_attend_dev", "Llm", "LlmSpec", "Parked", "SOFTMAX", "SIGMOID", "GREEDY", "GROUP_LIMITED", "NOAUX_TC",
+    "KvCache", "Spec", "attend", "F16", "I8", "MXFP4", "Batch", "PagedCache", "PageTable", "LIB_PATH", "Moe", "QCache", "mla_attend", "mla_attend_dev", "Llm", "LlmSpec", "Parked", "SOFTMAX", "SIGMOID", "GREEDY", "GROUP_LIMITED", "NOAUX_TC",
 ]
 
 F32, Q8, Q4, Q4K = 0, 1, 2, 3
-F16, I8 = 4, 5                            # rows of a PagedCache, beside F32
+F16, I8, MXFP4 = 4, 5, 6                  # rows of a PagedCache, beside F32
 SOFTMAX, SIGMOID = 0, 1                   # Scoring, model/ffn.rs:173-177
 GREEDY, GROUP_LIMITED, NOAUX_TC = 0, 1, 2  # Select, model/ffn.rs:179-195
 OK, DECLINED = 0, 1
@@ -612,7 +612,7 @@ class Batch(C.Structure):
 
 class PagedCache:
     """kh_paged: a pool of KV pages per layer that sequences hold by page
-    number, rows kept as F32, F16 or I8, and the attention over them.  The
+    number, rows kept as F32, F16, I8 or MXFP4, and the attention over them.  The
     _dev forms take device addresses and run on the context's stream; the
     others take a Batch.host and numpy arrays."""
 

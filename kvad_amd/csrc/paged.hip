@@ -249,10 +249,202 @@ __global__ __launch_bounds__(256) void read_kernel(MoveArgs a) {
     }
 }
 
+// ---- 4-bit rows ----------------------------------------------------------------
+// The exponent of a group's step from the bits of its largest magnitude: amax is
+// 3.5 to 7 steps, so that the largest is cut by 1 of 7 at the most.  Not under
+// -128, amax's under 7 2^-128 being subnormal or nearly so.
+__device__ __forceinline__ int mx_exp(int amax_bits) { return max(((amax_bits + 0x200000) >> 23) - 129, -128); }
+// The exponent of a row's scale from the largest of its groups' exponents: the
+// factors, 2^12 down to f16's least normal 2^-14, keep the codes times them under 2^15.
+__device__ __forceinline__ int mx_row_exp(int top) { return max(top - 12, -126); }
+constexpr int MX_LEAST = -14;  // of a factor's exponent
+__device__ __forceinline__ unsigned mx_factor(int e) { return (unsigned)(e + 15) << 2; }
+// Four values as codes, 4 bits each: nearest, ties to even, past 6 is 6.
+__device__ __forceinline__ unsigned mx_codes(float4u x, int e) {
+    const unsigned lo = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, ldexpf(x[0], -e), ldexpf(x[1], -e), 1.0f, 0);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(lo, ldexpf(x[2], -e), ldexpf(x[3], -e), 1.0f, 1) & 0xffff;
+}
+__device__ __forceinline__ int max8(int v) {
+    for (int o = 1; o < 8; o <<= 1) v = max(v, __shfl_xor(v, o));
+    return v;
+}
+
+// As push_kernel.  A group's 32 dims are one step of the 8 lanes that have a row.
+// V's words of 8 positions that the run fills in part keep the rest of theirs: they
+// are loaded with the rows.
+template <int D>
+__global__ __launch_bounds__(256) void push_mx_kernel(MoveArgs a) {
+    constexpr int G = D / 32, ROW = D / 2 + 16, VROW = D + 4;
+    __shared__ __attribute__((aligned(16))) char s_k[TILE * ROW];
+    __shared__ __attribute__((aligned(16))) uint8_t s_v[TILE * VROW];  // a code a byte
+    const int head = blockIdx.x % a.n_kv;
+    Tile t;
+    if (!find_tile(a, blockIdx.x / a.n_kv, head, t) || !t.block) return;
+    const int r = threadIdx.x >> 3, c = threadIdx.x & 7;
+    const int row = t.p0 + r - t.first;  // of the sequence's new rows
+    const bool mine = row >= 0 && row < t.n;
+    const size_t at = (size_t)(t.row0 + (mine ? row : 0));
+    const float *x[2] = {a.k + at * a.k_stride + (size_t)head * a.hd, a.v + at * a.v_stride + (size_t)head * a.hd};
+    float4u f[2][G];
+#pragma unroll
+    for (int what = 0; what < 2; what++)
+#pragma unroll
+        for (int j = 0; j < G; j++) {
+            const int d = 4 * c + 32 * j;
+            f[what][j] = float4u{0.0f, 0.0f, 0.0f, 0.0f};
+            if (mine && d < a.hd) f[what][j] = *reinterpret_cast<const float4u *>(x[what] + d);
+        }
+    const int in_page = t.p0 & (a.page - 1);
+    const int lo = max(t.first - t.p0, 0), hi = min(t.first + t.n - t.p0, TILE);  // the tile's new positions
+    // word i of V's tile: [dim / 64][position / 8][dim % 16][dim / 16 % 4]
+    unsigned *v_words = reinterpret_cast<unsigned *>(t.block + mx_v_off(D, a.page, in_page, 0));
+    unsigned old[D / 64], keep[D / 64];
+#pragma unroll
+    for (int j = 0; j < D / 64; j++) {
+        const int p = 8 * (threadIdx.x >> 6), from = max(lo - p, 0), to = min(hi - p, 8);
+        keep[j] = from < to ? ~(0xffffffffu >> (32 - 4 * (to - from)) << (4 * from)) : 0xffffffffu;
+        if (keep[j] && ~keep[j]) old[j] = v_words[threadIdx.x + 256 * j];
+    }
+#pragma unroll
+    for (int what = 0; what < 2; what++) {
+        int e[G], top = -128;
+        bool finite = true;
+#pragma unroll
+        for (int j = 0; j < G; j++) {
+            int amax = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) amax = max(amax, __builtin_bit_cast(int, (float)f[what][j][i]) & 0x7fffffff);
+            amax = max8(amax);
+            finite = finite && amax < 0x7f800000;
+            e[j] = mx_exp(amax);
+            top = max(top, e[j]);
+        }
+        const int re = mx_row_exp(top);
+        unsigned long long factors = 0;
+#pragma unroll
+        for (int j = 0; j < G; j++) {
+            e[j] = max(e[j], re + MX_LEAST);
+            factors |= (unsigned long long)mx_factor(finite ? e[j] - re : 0) << (8 * j);
+            const unsigned codes = finite ? mx_codes(f[what][j], e[j]) : 0u;
+            if (what == 0) {
+                *reinterpret_cast<unsigned short *>(s_k + r * ROW + 2 * c + 16 * j) = (unsigned short)codes;
+            } else {
+                const unsigned spread = (codes & 0xf) | (codes & 0xf0) << 4 | (codes & 0xf00) << 8 | (codes & 0xf000) << 12;
+                *reinterpret_cast<unsigned *>(s_v + r * VROW + 4 * c + 32 * j) = spread;
+            }
+        }
+        if (!mine) continue;
+        if (c == 0) {
+            const int off = what ? mx_v_scale_off(D, a.page, in_page + r) : mx_k_scale_off(D, a.page, in_page + r);
+            *reinterpret_cast<float *>(t.block + off) = finite ? pow2(re) : __builtin_bit_cast(float, NAN_BITS);
+        }
+        if (c < G) {
+            const int off = what ? mx_v_factor_off(D, a.page, in_page + r, c) : mx_k_factor_off(D, a.page, in_page + r, c);
+            t.block[off] = (char)(factors >> (8 * c));
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < TILE * G; i += 256) {
+        const int pos = i & 31, unit = i >> 5;
+        if (pos >= lo && pos < hi)
+            *reinterpret_cast<int4 *>(t.block + mx_k_off(a.page, in_page + pos, unit * 32)) =
+                *reinterpret_cast<const int4 *>(s_k + pos * ROW + unit * 16);
+    }
+#pragma unroll
+    for (int j = 0; j < D / 64; j++) {
+        if (!~keep[j]) continue;
+        const int i = threadIdx.x, dim = 64 * j + (i >> 2 & 15) + 16 * (i & 3), p = 8 * (i >> 6);
+        unsigned w = 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) w |= (unsigned)s_v[(p + k) * VROW + dim] << (4 * k);
+        v_words[i + 256 * j] = keep[j] ? (w & ~keep[j]) | (old[j] & keep[j]) : w;
+    }
+}
+
+// Two codes times their row's factor (f16, exact) and scale.
+__device__ __forceinline__ void mx_values(unsigned codes, unsigned factor, float scale, float &x, float &y) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const float f = __builtin_bit_cast(float, (factor << 21) + (112u << 23));
+    const h2 v = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, f, 0);
+    x = (float)v.x * scale;
+    y = (float)v.y * scale;
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void read_mx_kernel(MoveArgs a) {
+    constexpr int G = D / 32, ROW = D / 2 + 16, VROW = D + 4;
+    __shared__ __attribute__((aligned(16))) char s_k[TILE * ROW];
+    __shared__ __attribute__((aligned(16))) uint8_t s_v[TILE * VROW];  // a code a byte
+    const int head = blockIdx.x % a.n_kv;
+    Tile t;
+    if (!find_tile(a, blockIdx.x / a.n_kv, head, t)) return;
+    const int in_page = t.p0 & (a.page - 1), r = threadIdx.x >> 3, c = threadIdx.x & 7;
+    float scale[2] = {0.0f, 0.0f};
+    uint8_t factor[2][G];
+    if (t.block) {
+        const unsigned *v_words = reinterpret_cast<const unsigned *>(t.block + mx_v_off(D, a.page, in_page, 0));
+        int4 k;
+        unsigned v[D / 64];
+        const int pos = threadIdx.x & 31, unit = threadIdx.x >> 5;
+        if (unit < G) k = *reinterpret_cast<const int4 *>(t.block + mx_k_off(a.page, in_page + pos, unit * 32));
+#pragma unroll
+        for (int j = 0; j < D / 64; j++) v[j] = v_words[threadIdx.x + 256 * j];
+        scale[0] = *reinterpret_cast<const float *>(t.block + mx_k_scale_off(D, a.page, in_page + r));
+        scale[1] = *reinterpret_cast<const float *>(t.block + mx_v_scale_off(D, a.page, in_page + r));
+#pragma unroll
+        for (int j = 0; j < G; j++) {
+            factor[0][j] = (uint8_t)t.block[mx_k_factor_off(D, a.page, in_page + r, j)];
+            factor[1][j] = (uint8_t)t.block[mx_v_factor_off(D, a.page, in_page + r, j)];
+        }
+        if (unit < G) *reinterpret_cast<int4 *>(s_k + pos * ROW + unit * 16) = k;
+#pragma unroll
+        for (int j = 0; j < D / 64; j++) {
+            const int i = threadIdx.x, dim = 64 * j + (i >> 2 & 15) + 16 * (i & 3), p = 8 * (i >> 6);
+#pragma unroll
+            for (int e = 0; e < 8; e++) s_v[(p + e) * VROW + dim] = (uint8_t)(v[j] >> (4 * e) & 15);
+        }
+    }
+    __syncthreads();
+    const int row = t.p0 + r - t.first;
+    if (row < 0 || row >= t.n) return;
+#pragma unroll
+    for (int what = 0; what < 2; what++) {
+        float *y = (what ? a.v + (size_t)(t.row0 + row) * a.v_stride : a.k + (size_t)(t.row0 + row) * a.k_stride) +
+                   (size_t)head * a.hd;
+#pragma unroll
+        for (int j = 0; j < G; j++) {
+            const int d = 4 * c + 32 * j;
+            if (d >= a.hd) break;
+            float4u f = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (t.block) {
+                unsigned lo, hi;
+                if (what == 0) {
+                    lo = *reinterpret_cast<const unsigned short *>(s_k + r * ROW + d / 2);
+                    hi = lo >> 8;
+                } else {
+                    const unsigned s = *reinterpret_cast<const unsigned *>(s_v + r * VROW + d);
+                    lo = s | s >> 4;
+                    hi = lo >> 16;
+                }
+                float v[4];
+                mx_values(lo, factor[what][j], scale[what], v[0], v[1]);
+                mx_values(hi, factor[what][j], scale[what], v[2], v[3]);
+                f = float4u{v[0], v[1], v[2], v[3]};
+            }
+            *reinterpret_cast<float4u *>(y + d) = f;
+        }
+    }
+}
+
 template <int ES, int D>
 void launch_move(bool push, const MoveArgs &a, unsigned blocks, hipStream_t stream) {
-    if (push) push_kernel<ES, D><<<blocks, 256, 0, stream>>>(a);
-    else read_kernel<ES, D><<<blocks, 256, 0, stream>>>(a);
+    if constexpr (ES == MX) {
+        if (push) push_mx_kernel<D><<<blocks, 256, 0, stream>>>(a);
+        else read_mx_kernel<D><<<blocks, 256, 0, stream>>>(a);
+    } else {
+        if (push) push_kernel<ES, D><<<blocks, 256, 0, stream>>>(a);
+        else read_kernel<ES, D><<<blocks, 256, 0, stream>>>(a);
+    }
 }
 
 template <int ES>
@@ -315,7 +507,8 @@ int move(const kh_paged *kv, size_t layer, const kh_batch *b, float *k, size_t k
     hipStream_t s = kv->ctx->stream;
     if (kv->es == 4) launch_move_d<4>(push, kv->d, a, (unsigned)blocks, s);
     else if (kv->es == 2) launch_move_d<2>(push, kv->d, a, (unsigned)blocks, s);
-    else launch_move_d<1>(push, kv->d, a, (unsigned)blocks, s);
+    else if (kv->es == 1) launch_move_d<1>(push, kv->d, a, (unsigned)blocks, s);
+    else launch_move_d<MX>(push, kv->d, a, (unsigned)blocks, s);
     KH_HIP(hipGetLastError());
     return KH_OK;
 }
@@ -400,8 +593,8 @@ int kh_paged_new(kh_ctx *ctx, size_t n_layer, size_t n_kv_head, size_t head_dim,
     return guarded([&]() -> int {
         if (out) *out = nullptr;
         if (!ctx || !out) return fail(KH_EINVAL, "kh_paged_new: null argument");
-        if (precision != KH_F32 && precision != KH_F16 && precision != KH_I8)
-            return fail(KH_EINVAL, "kh_paged_new: rows are kept as KH_F32, KH_F16 or KH_I8");
+        if (precision != KH_F32 && precision != KH_F16 && precision != KH_I8 && precision != KH_MXFP4)
+            return fail(KH_EINVAL, "kh_paged_new: rows are kept as KH_F32, KH_F16, KH_I8 or KH_MXFP4");
         if (n_layer == 0 || n_layer > 65536 || n_kv_head == 0 || n_kv_head > 65536)
             return fail(KH_EINVAL, "kh_paged_new: needs 1 to 65536 layers and KV heads");
         if (head_dim == 0 || head_dim % 4 || head_dim > 256)
@@ -414,12 +607,12 @@ int kh_paged_new(kh_ctx *ctx, size_t n_layer, size_t n_kv_head, size_t head_dim,
         kv->n_layer = n_layer;
         kv->n_kv_head = n_kv_head;
         kv->head_dim = head_dim;
-        kv->es = precision == KH_F32 ? 4 : precision == KH_F16 ? 2 : 1;
+        kv->es = precision == KH_F32 ? 4 : precision == KH_F16 ? 2 : precision == KH_I8 ? 1 : MX;
         kv->d = stored_dims((int)head_dim);
         kv->page = (int)page_size;
         while ((1 << kv->page_shift) < kv->page) kv->page_shift++;
         kv->n_pages = n_pages;
-        kv->block = block_bytes(kv->es, kv->d, kv->page);
+        kv->block = kv->es == MX ? mx_block_bytes(kv->d, kv->page) : block_bytes(kv->es, kv->d, kv->page);
         size_t layer_bytes;
         if (__builtin_mul_overflow(kv->block * n_kv_head, n_pages, &layer_bytes) ||
             __builtin_mul_overflow(layer_bytes, n_layer, &kv->bytes))

@@ -166,6 +166,25 @@ __device__ __forceinline__ h8 codes8(unsigned a, unsigned b) {
     return h8{r0.x, r0.y, r1.x, r1.y, r2.x, r2.y, r3.x, r3.y};
 }
 
+// Eight 4-bit codes times their factor, a power of two as a float.
+__device__ __forceinline__ h8 mx8(unsigned w, float factor) {
+    const h2 r0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, factor, 0), r1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, factor, 1);
+    const h2 r2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, factor, 2), r3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, factor, 3);
+    return h8{r0.x, r0.y, r1.x, r1.y, r2.x, r2.y, r3.x, r3.y};
+}
+// Byte `i` of w, the high one of an f16 power of two, as a float.
+__device__ __forceinline__ float mx_factor(unsigned w, int i) {
+    return __builtin_bit_cast(float, ((w >> (8 * i) & 0xff) << 21) + (112u << 23));
+}
+// Eight of them as f16.
+__device__ __forceinline__ h8 mx_factors(unsigned a, unsigned b) {
+    const h2 r0 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0u, a, 0x010c000cu));
+    const h2 r1 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0u, a, 0x030c020cu));
+    const h2 r2 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0u, b, 0x010c000cu));
+    const h2 r3 = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0u, b, 0x030c020cu));
+    return h8{r0.x, r0.y, r1.x, r1.y, r2.x, r2.y, r3.x, r3.y};
+}
+
 __device__ __forceinline__ f16v mfma(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f4v mfma(h8 a, h8 b, f4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
@@ -178,6 +197,19 @@ __device__ __forceinline__ float load4(dev::rsrc_t r, unsigned voff, unsigned so
 }
 __device__ __forceinline__ int4 load16(dev::rsrc_t r, unsigned voff, unsigned soff) {
     return __builtin_bit_cast(int4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
+}
+
+// Where a block's scales start, K's and then V's.
+template <int ES, int D>
+__device__ __forceinline__ unsigned scales_at(int page) {
+    return (unsigned)(ES == MX ? page * D + page * D / 16 : 2 * page * D * ES);
+}
+// A position's factors of K, D / 32 bytes.
+template <int D>
+__device__ __forceinline__ u2v load_kf(dev::rsrc_t r, unsigned voff, unsigned soff) {
+    if (D == 64) return u2v{(unsigned)__builtin_amdgcn_raw_buffer_load_b16(r, voff, soff, 0), 0u};
+    if (D == 128) return u2v{(unsigned)__builtin_amdgcn_raw_buffer_load_b32(r, voff, soff, 0), 0u};
+    return load8(r, voff, soff);
 }
 
 // The positions a wave's rows see, as a list of 32-position tiles: those of
@@ -391,7 +423,7 @@ constexpr bool shares_registers(int es, int d) { return es == 4 && d >= 128; }
 // 32 rows; WS waves share them (1: each has its own).
 template <int ES, int D, int WS>
 __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float *lds) {
-    constexpr int NK = D * ES / 32;  // loads of a lane for K
+    constexpr int NK = ES == MX ? D / 64 : D * ES / 32;  // loads of a lane for K
     constexpr int DT = D / 32;       // dim tiles of V
     constexpr int NS = D / 16;       // products over the dims
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
@@ -408,12 +440,19 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
     const unsigned v_lane = (unsigned)(P * D * ES) + (unsigned)(v_load_unit(ES, 0, h) * D + n) * 16;
     // scales: a lane holds position 16 h + lane % 16's, and takes the others of
     // its half from the lanes beside it
-    const unsigned s_lane = (unsigned)(2 * P * D * ES) + 4 * (16 * h + (lane & 15));
+    const unsigned s_lane = scales_at<ES, D>(P) + 4 * (16 * h + (lane & 15));
     const Table table(a, w.seq);
+    // 4-bit rows: K's factors of the lane's position, V's codes and factors of 8
+    // positions, two loads for each 64 dims
+    const unsigned kf_lane = (unsigned)(P * D) + (unsigned)tile_pos(n) * (D / 32);
+    const unsigned vc_lane = (unsigned)(P * D / 2) + 512 * h + 16 * (n & 15) + 8 * (n >> 4);
+    const unsigned vf_lane = (unsigned)(P * D + P * D / 32) + (D / 2) * h + 8 * (n >> 4);
+    u2v vc[ES == MX ? D / 32 : 1], vf[ES == MX ? D / 32 : 1];
+    u2v kf = {0u, 0u};
     // Wide rows (SHARED): K and V take turns in the same registers, half of
     // the dims at a time, each half loaded as soon as the other's is used.
     constexpr bool SHARED = shares_registers(ES, D);
-    int4 kraw[NK], vown[SHARED ? 1 : DT * ES];
+    int4 kraw[NK], vown[SHARED || ES == MX ? 1 : DT * ES];
     int4 *const vraw = SHARED ? kraw : vown;
     float ks, vs, k_own = 0.0f;
     auto load_s = [&](const Where &x) {
@@ -427,12 +466,23 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
             const int unit = k_load_unit(ES, i, 0);
             kraw[i] = load16(x.r, k_lane, (unsigned)(unit * P + x.in_page) * 16);
         }
+        if constexpr (ES == MX) kf = load_kf<D>(x.r, kf_lane, (unsigned)x.in_page * (D / 32));
     };
     auto load_v = [&](const Where &x, int from, int to) {
+        if constexpr (ES == MX) {
+            const unsigned at = x.v_at(D / 2), f_at = x.v_at(D / 32);
+#pragma unroll
+            for (int i = 0; i < D / 32; i++) {  // quarter 2 h + i % 2 of 64 dims i / 2
+                vc[i] = load8(x.r, vc_lane + 1024 * (i >> 1) + 256 * (i & 1), at);
+                vf[i] = load8(x.r, vf_lane + 16 * (i >> 1) + (D / 4) * (i & 1), f_at);
+            }
+            return;
+        }
         const unsigned at = x.v_at(D * ES);
 #pragma unroll
         for (int i = from; i < to; i++) {
-            const int dt = i / ES, c = i % ES;
+            constexpr int E = ES == MX ? 1 : ES;
+            const int dt = i / E, c = i % E;
             vraw[i] = load16(x.r, v_lane + (c * D + dt * 32) * 16, at);
         }
     };
@@ -449,7 +499,7 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
     float rowf;
     {
         float v[NS][8];
-        int amax = load_q<NS>(row.query(a, w), a.hd, [&](int i) { return k_dim(ES, i, h, 0); }, v);
+        int amax = load_q<NS>(row.query(a, w), a.hd, [&](int i) { return ES == MX ? mx_k_dim(i, h, 0) : k_dim(ES, i, h, 0); }, v);
         amax = max(amax, __shfl_xor(amax, 32));
         const float inv = q_scale(amax, a.scale, rowf);
 #pragma unroll
@@ -469,7 +519,20 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
 
         // ---- scores: register i is position start + 16 h + i ----
         f16v sc = f16v{0.0f};
-        if (ES == 1) {
+        if constexpr (ES == MX) {
+            const unsigned f[2] = {kf.x >> (8 * h), kf.y >> (8 * h)};
+#pragma unroll
+            for (int i = 0; i < NK; i++) {
+                const float factor = mx_factor(f[i >> 1], 2 * (i & 1));
+                const unsigned word[4] = {(unsigned)kraw[i].x, (unsigned)kraw[i].y, (unsigned)kraw[i].z, (unsigned)kraw[i].w};
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const h8 k = mx8(word[c], factor);
+                    sc = mfma(k, qh[4 * i + c], sc);
+                    sc = mfma(k, ql[4 * i + c], sc);
+                }
+            }
+        } else if (ES == 1) {
 #pragma unroll
             for (int i = 0; i < NK; i++) {
                 const h8 k0 = codes8(kraw[i].x, kraw[i].y), k1 = codes8(kraw[i].z, kraw[i].w);
@@ -569,7 +632,12 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
         // ---- O^T += V^T P^T ----
         each<DT * 2>([&](auto k) {
             constexpr int dt = k / 2, c = k % 2;
-            if constexpr (ES == 1) {
+            if constexpr (ES == MX) {
+                constexpr int at = dt / 2 * 2 + c;
+                const h8 v = mx8(dt % 2 ? vc[at].y : vc[at].x, 1.0f) * mx_factors(vf[at].x, vf[at].y);
+                acc[dt] = mfma(v, ph[c], acc[dt]);
+                acc[dt] = mfma(v, pl[c], acc[dt]);
+            } else if constexpr (ES == 1) {
                 const int4 r = vraw[dt];
                 const h8 v = c ? codes8(r.z, r.w) : codes8(r.x, r.y);
                 acc[dt] = mfma(v, ph[c], acc[dt]);
@@ -607,14 +675,17 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
         if (wave > 0) return;
     }
     if (n >= w.nr) return;
-    put_row<ES>(a, w, row, o, ref, sum, h == 0, D, [&](int c) { return 32 * (c >> 2) + 8 * (c & 3) + 4 * h; });
+    put_row<ES>(a, w, row, o, ref, sum, h == 0, D, [&](int c) {
+        const int row_of = 8 * (c & 3) + 4 * h;  // of the dim tile, the first of four
+        return ES == MX ? mx_v_dim(c >> 2, row_of) : 32 * (c >> 2) + row_of;
+    });
 }
 
 // ROWS rows, 8 or 16, shared by the workgroup's four waves.
 template <int ES, int D, int ROWS>
 __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float *lds) {
     constexpr bool PACKED = ROWS == 8;  // columns 0 .. 7 the high pieces, 8 .. 15 the low ones
-    constexpr int NK = D * ES / 64;     // loads of a lane for K, a block of 16 positions
+    constexpr int NK = ES == MX ? (D + 127) / 128 : D * ES / 64;  // loads of a lane for K, a block of 16 positions
     constexpr int DB = D / 16;          // dim blocks of V
     constexpr int NS = D / 32;          // products over the dims
     constexpr int NV = ES == 4 ? 2 : 1; // loads of a lane for V, a dim block
@@ -629,12 +700,19 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
     float ref = LOW, sum = 0.0f;
 
     const int P = a.page;
-    const unsigned k_lane = (unsigned)(few_k_unit(ES, 0, z) * P + few_pos(n, 0)) * 16;
-    const unsigned v_lane = (unsigned)(P * D * ES) + 16 * n + few_v_off(ES, D, 0, z);
-    const unsigned s_lane = (unsigned)(2 * P * D * ES) + 4 * (8 * z + (lane & 7));  // scales: position 8 z + lane % 8's
+    const unsigned k_lane = ES == MX ? (unsigned)(mx_few_k_lane(D, P, z) + few_pos(n, 0) * 16)
+                                     : (unsigned)(few_k_unit(ES, 0, z) * P + few_pos(n, 0)) * 16;
+    const unsigned v_lane = ES == MX ? (unsigned)(P * D / 2) + 256 * z + 16 * n
+                                     : (unsigned)(P * D * ES) + 16 * n + few_v_off(ES, D, 0, z);
+    const unsigned s_lane = scales_at<ES, D>(P) + 4 * (8 * z + (lane & 7));  // scales: position 8 z + lane % 8's
     const Table table(a, w.seq);
+    // 4-bit rows: K's factors of the lane's two positions, V's of 8 positions of 64 dims
+    const unsigned kf_lane = (unsigned)(P * D) + (unsigned)few_pos(n, 0) * (D / 32);
+    const unsigned vf_lane = (unsigned)(P * D + P * D / 32) + (D / 4) * z;
+    int4 vf[ES == MX ? D / 64 : 1];
+    u2v kf[2];
     int4 kraw[2 * NK];
-    int4 vraw[ES == 1 ? 1 : DB * NV];
+    int4 vraw[ES == 1 ? 1 : ES == MX ? D / 64 : DB * NV];
     u2v vraw8[ES == 1 ? DB : 1];
     float ks, vs, k_own[2] = {0.0f, 0.0f};
     auto load_s = [&](const Where &x) {
@@ -644,6 +722,18 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
     auto load_k = [&](const Where &x) {
 #pragma unroll
         for (int b = 0; b < 2; b++) {
+            if constexpr (ES == MX) {
+                if (D == 64) {
+                    const u2v half = load8(x.r, k_lane + 64 * b, (unsigned)x.in_page * 16);
+                    kraw[b] = make_int4((int)half.x, (int)half.y, 0, 0);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NK; i++)
+                        kraw[b * NK + i] = load16(x.r, k_lane + 64 * b, (unsigned)(4 * i * P + x.in_page) * 16);
+                }
+                kf[b] = load_kf<D>(x.r, kf_lane + 4 * b * (D / 32), (unsigned)x.in_page * (D / 32));
+                continue;
+            }
 #pragma unroll
             for (int i = 0; i < NK; i++) {
                 const int unit = few_k_unit(ES, i, 0);
@@ -653,6 +743,15 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
         }
     };
     auto load_v = [&](const Where &x) {
+        if constexpr (ES == MX) {
+            const unsigned at = x.v_at(D / 2), f_at = x.v_at(D / 32);
+#pragma unroll
+            for (int i = 0; i < D / 64; i++) {
+                vraw[i] = load16(x.r, v_lane + 1024 * i, at);
+                vf[i] = load16(x.r, vf_lane + 16 * i, f_at);
+            }
+            return;
+        }
         const unsigned at = x.v_at(D * ES);
 #pragma unroll
         for (int db = 0; db < DB; db++) {
@@ -678,7 +777,7 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
     float rowf;
     {
         float v[NS][8];
-        int amax = load_q<NS>(row.query(a, w), a.hd, [&](int i) { return few_k_dim(ES, i, z, 0); }, v);
+        int amax = load_q<NS>(row.query(a, w), a.hd, [&](int i) { return ES == MX ? mx_few_k_dim(D, i, z, 0) : few_k_dim(ES, i, z, 0); }, v);
         amax = max(amax, __shfl_xor(amax, 16));
         amax = max(amax, __shfl_xor(amax, 32));
         const float inv = q_scale(amax, a.scale, rowf);
@@ -702,7 +801,22 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
         f4v sc[2] = {f4v{0.0f}, f4v{0.0f}};
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            if (ES == 1) {
+            if constexpr (ES == MX) {
+                // the factor of the lane's unit, all of 32 dims
+                const unsigned f[2] = {kf[b].x >> (D == 64 ? 8 * (z >> 1) : 8 * z), kf[b].y >> (8 * z)};
+#pragma unroll
+                for (int i = 0; i < NK; i++) {
+                    const int4 r = kraw[b * NK + i];
+                    const float factor = mx_factor(f[i & 1], 0);
+                    const unsigned word[4] = {(unsigned)r.x, (unsigned)r.y, (unsigned)r.z, (unsigned)r.w};
+#pragma unroll
+                    for (int c = 0; c < (D == 64 ? 2 : 4); c++) {
+                        const h8 k = mx8(word[c], factor);
+                        sc[b] = mfma(k, qh[4 * i + c], sc[b]);
+                        if (!PACKED) sc[b] = mfma(k, ql[(4 * i + c) % (PACKED ? 1 : NS)], sc[b]);
+                    }
+                }
+            } else if (ES == 1) {
 #pragma unroll
                 for (int i = 0; i < NK; i++) {
                     const int4 r = kraw[b * NK + i];
@@ -796,7 +910,11 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
 #pragma unroll
         for (int db = 0; db < DB; db++) {
             h8 vh, vl;
-            if (ES == 1) {
+            if constexpr (ES == MX) {
+                const int4 r = vraw[db / 4], f = vf[db / 4];
+                const unsigned word = (unsigned)(db % 4 == 0 ? r.x : db % 4 == 1 ? r.y : db % 4 == 2 ? r.z : r.w);
+                vh = mx8(word, 1.0f) * (db % 4 < 2 ? mx_factors((unsigned)f.x, (unsigned)f.y) : mx_factors((unsigned)f.z, (unsigned)f.w));
+            } else if (ES == 1) {
                 const u2v r = vraw8[db % (ES == 1 ? DB : 1)];
                 vh = codes8(r.x, r.y);
             } else if (ES == 2) {
@@ -834,7 +952,7 @@ constexpr int FEW = 8;  // rows (x group) of a sequence that few_rows takes besi
 // few_rows' query, sums, K, V and the rest.
 constexpr int waves_for(int es, int d, int rows) {
     if (rows > 16) return d == 256 ? 1 : 2;
-    const int regs = d / 8 * (rows / 8) + d / 4 + d * es / 4 + 60;
+    const int regs = d / 8 * (rows / 8) + d / 4 + (es == MX ? d / 8 : d * es / 4) + 60;
     return regs <= 128 ? 4 : regs <= 172 ? 3 : regs <= 250 ? 2 : 1;
 }
 
@@ -977,7 +1095,7 @@ size_t up_to(size_t n, size_t m) { return (n + m - 1) / m; }
 // fewer large ones; and where all splits together save a wave less turns than
 // that, there are none.
 size_t few_splits(const kh_paged *kv, size_t blocks, size_t pos_tiles, size_t cus) {
-    const size_t least = std::min(std::max(2048 / (kv->es * kv->d), 4), 16);
+    const size_t least = std::min(std::max(4096 / ((kv->es == MX ? 1 : 2 * kv->es) * kv->d), 4), 16);
     const size_t splits = std::min(up_to(cus, blocks), up_to(pos_tiles, least));
     return up_to(pos_tiles, 4) < up_to(up_to(pos_tiles, splits), 4) + least / 4 ? 1 : splits;
 }
@@ -1098,7 +1216,8 @@ int launch_attn(kh_ctx *ctx, const AttnCall &c, const AttnPlan &p) {
     const unsigned blocks = (unsigned)((size_t)p.tiles * kv->n_kv_head * p.splits);
     if (kv->es == 4) return launch_d<4>(kv->d, a, p, blocks, items, ctx->stream);
     if (kv->es == 2) return launch_d<2>(kv->d, a, p, blocks, items, ctx->stream);
-    return launch_d<1>(kv->d, a, p, blocks, items, ctx->stream);
+    if (kv->es == 1) return launch_d<1>(kv->d, a, p, blocks, items, ctx->stream);
+    return launch_d<MX>(kv->d, a, p, blocks, items, ctx->stream);
 }
 
 }  // namespace paged

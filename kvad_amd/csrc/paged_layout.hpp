@@ -29,6 +29,29 @@ namespace paged {
 constexpr int TILE = 32;  // positions the attention takes at a time; divides every page
 
 KH_HD int stored_dims(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+// Rows in 4 bits (MXFP4, "es" 0): E2M1 codes, two a byte, 32 dims of a row
+// sharing a factor, a power of two kept as the high byte of its f16, all of a
+// row's times the row's f32 scale.  Of a block, K's codes and V's, then K's
+// factors and V's, then the scales:
+//   K        [dim / 32][position][32 dims]              a lane's unit: a factor's dims
+//   V        [position / 32][dim / 64][position / 8 % 4][dim % 16][dim / 16 % 4][8 positions]
+//   factors  K [position][dim / 32], V [position / 8][dim / 32][8 positions]
+// V's unit of 16 bytes is 8 positions of the four dims 16 apart that a lane of
+// the 16x16x32 product has of 64: one load, where single dims would be four.
+constexpr int MX = 0, MX_GROUP = 32;
+KH_HD size_t mx_block_bytes(int d, int page) { return (size_t)page * (d + d / 16 + 8); }
+// the byte of a code; an even dim's (K) or position's (V) is its low half
+KH_HD int mx_k_off(int page, int pos, int dim) { return (dim / 32 * page + pos) * 16 + dim % 32 / 2; }
+KH_HD int mx_v_off(int d, int page, int pos, int dim) {
+    return page * d / 2 + pos / 32 * 16 * d + dim / 64 * 1024 + pos / 8 % 4 * 256 + dim % 16 * 16 + dim / 16 % 4 * 4 + pos % 8 / 2;
+}
+KH_HD int mx_k_factor_off(int d, int page, int pos, int group) { return page * d + pos * (d / 32) + group; }
+KH_HD int mx_v_factor_off(int d, int page, int pos, int group) {
+    return page * d + page * d / 32 + pos / 8 * (d / 4) + group * 8 + pos % 8;
+}
+KH_HD int mx_k_scale_off(int d, int page, int pos) { return page * d + page * d / 16 + 4 * pos; }
+KH_HD int mx_v_scale_off(int d, int page, int pos) { return page * d + page * d / 16 + 4 * page + 4 * pos; }
+
 KH_HD size_t block_bytes(int es, int d, int page) { return (size_t)2 * page * d * es + (size_t)8 * page; }
 
 KH_HD int k_off(int es, int page, int pos, int dim) {
@@ -78,6 +101,19 @@ KH_HD int few_k_dim(int es, int s, int z, int e) {
 KH_HD int few_v_off(int es, int d, int c, int z) {
     return es == 4 ? (2 * z + c) * d * 16 : es == 2 ? z * d * 16 : (z >> 1) * d * 16 + 8 * (z & 1);
 }
+
+// The same of 4-bit rows.  32x32x16: K's load j (of d / 64) is unit 2 j + h, four
+// products of a word each; V's are words of 8 positions, quarters 2 h and 2 h + 1
+// of the tile, the lane's dims of 64 being two that lie beside each other in a
+// unit, for the two dim tiles t of the 64.
+KH_HD int mx_k_dim(int s, int h, int e) { return 64 * (s >> 2) + 32 * h + 8 * (s & 3) + e; }
+KH_HD int mx_v_dim(int dt, int n) { return 64 * (dt >> 1) + (n & 15) + 32 * (n >> 4) + 16 * (dt & 1); }
+// 16x16x32: K's load j (of d / 128) is unit 4 j + z, four products; of 64 dims
+// half of unit z / 2, two products.  V's dim block db is word db % 4 of its unit.
+KH_HD int mx_few_k_dim(int d, int s, int z, int e) {
+    return d == 64 ? 16 * z + 8 * s + e : 128 * (s >> 2) + 32 * z + 8 * (s & 3) + e;
+}
+KH_HD int mx_few_k_lane(int d, int page, int z) { return d == 64 ? (z >> 1) * page * 16 + 8 * (z & 1) : z * page * 16; }
 
 }  // namespace paged
 }  // namespace kh
