@@ -84,6 +84,7 @@ struct Args {
     size_t block;
     int n_kv, group, hd, n_pages, page, page_shift;
     int tiles_per, splits, split_tiles, window, sinks;
+    int longest_first;
     float scale, out_scale;
 };
 
@@ -126,7 +127,16 @@ __device__ __forceinline__ void only_finite(float &v_scale, float &k_scale) {
     v_scale = finite ? v_scale * VScale<ES>::TIMES : 0.0f;
 }
 // the value 8 lanes on, in each row of 16
-__device__ __forceinline__ float other_half(float v) { return dev::dppf<0x128>(v); }
+__device__ __forceinline__ float other_half(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x128, 0xf, 0xf, true));
+}
+// A copy made here: the register that v was loaded into takes the next load at
+// once, where a copy at the loop's end would wait for that load.
+__device__ __forceinline__ float copy(float v) {
+    float r;
+    asm volatile("v_mov_b32 %0, %1" : "=v"(r) : "v"(v));
+    return r;
+}
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 // A sum of weights at a reference `by` powers of two on (negative, or zero).  A
 // reference holds the exponent of V's scales, so it can move by more than a
@@ -436,7 +446,7 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
     float ref = LOW, sum = 0.0f;  // the row's reference and this lane's part of its sum
 
     const int P = a.page;
-    const unsigned k_lane = (unsigned)(k_load_unit(ES, 0, h) * P + tile_pos(n)) * 16;
+    const unsigned k_lane = (unsigned)(k_load_unit(ES, 0, h) * P + (ES == MX ? mx_tile_slot(n) : tile_pos(n))) * 16;
     const unsigned v_lane = (unsigned)(P * D * ES) + (unsigned)(v_load_unit(ES, 0, h) * D + n) * 16;
     // scales: a lane holds position 16 h + lane % 16's, and takes the others of
     // its half from the lanes beside it
@@ -573,7 +583,8 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
                           (a.window != INT32_MAX && start + TILE > a.sinks && start < w.p_hi - a.window + 1);
         here = table.find(a, w, next_t, next_page);
         if (!SHARED) load_k(here, 0, NK);
-        float sk = ks, sv = vs;
+        // (4-bit rows: no faster for it)
+        float sk = ES == MX ? ks : copy(ks), sv = ES == MX ? vs : copy(vs);
         load_s(here);
         __builtin_amdgcn_sched_barrier(0);
         only_finite<ES>(sv, sk);
@@ -682,7 +693,12 @@ __device__ __forceinline__ void many_rows(const Args &a, Job &w, int wave, float
 }
 
 // ROWS rows, 8 or 16, shared by the workgroup's four waves.
-template <int ES, int D, int ROWS>
+// AHEAD, of 4-bit rows, whose tiles are small: two sets of registers for what is
+// loaded, all of the next tile on its way while this one is computed.  For calls
+// that give a CU one workgroup or none: there a wave has a SIMD to itself and what
+// it waits for is not hidden by another (32 sequences of 16000, 8 KV heads of 128:
+// 104 us against 116, 5.6 TB/s; 64 of 4000, two workgroups a CU: 57.7 against 56.4).
+template <int ES, int D, int ROWS, bool AHEAD>
 __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float *lds) {
     constexpr bool PACKED = ROWS == 8;  // columns 0 .. 7 the high pieces, 8 .. 15 the low ones
     constexpr int NK = ES == MX ? (D + 127) / 128 : D * ES / 64;  // loads of a lane for K, a block of 16 positions
@@ -700,7 +716,7 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
     float ref = LOW, sum = 0.0f;
 
     const int P = a.page;
-    const unsigned k_lane = ES == MX ? (unsigned)(mx_few_k_lane(D, P, z) + few_pos(n, 0) * 16)
+    const unsigned k_lane = ES == MX ? (unsigned)(mx_few_k_lane(D, P, z) + mx_few_slot(n, 0) * 16)
                                      : (unsigned)(few_k_unit(ES, 0, z) * P + few_pos(n, 0)) * 16;
     const unsigned v_lane = ES == MX ? (unsigned)(P * D / 2) + 256 * z + 16 * n
                                      : (unsigned)(P * D * ES) + 16 * n + few_v_off(ES, D, 0, z);
@@ -709,46 +725,52 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
     // 4-bit rows: K's factors of the lane's two positions, V's of 8 positions of 64 dims
     const unsigned kf_lane = (unsigned)(P * D) + (unsigned)few_pos(n, 0) * (D / 32);
     const unsigned vf_lane = (unsigned)(P * D + P * D / 32) + (D / 4) * z;
-    int4 vf[ES == MX ? D / 64 : 1];
-    u2v kf[2];
-    int4 kraw[2 * NK];
-    int4 vraw[ES == 1 ? 1 : ES == MX ? D / 64 : DB * NV];
-    u2v vraw8[ES == 1 ? DB : 1];
-    float ks, vs, k_own[2] = {0.0f, 0.0f};
-    auto load_s = [&](const Where &x) {
-        ks = load4(x.r, s_lane, 4 * x.in_page);
-        vs = load4(x.r, s_lane, 4 * P + 4 * x.in_page);
+    struct Raw {  // what is loaded of a tile
+        Where x;
+        int4 vf[ES == MX ? D / 64 : 1];
+        u2v kf[2];
+        int4 kraw[2 * NK];
+        int4 vraw[ES == 1 ? 1 : ES == MX ? D / 64 : DB * NV];
+        u2v vraw8[ES == 1 ? DB : 1];
+        float ks, vs, k_own[2];
     };
-    auto load_k = [&](const Where &x) {
+    auto load_s = [&](Raw &raw) {
+        const Where &x = raw.x;
+        raw.ks = load4(x.r, s_lane, 4 * x.in_page);
+        raw.vs = load4(x.r, s_lane, 4 * P + 4 * x.in_page);
+    };
+    auto load_k = [&](Raw &raw) {
+        const Where &x = raw.x;
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             if constexpr (ES == MX) {
                 if (D == 64) {
-                    const u2v half = load8(x.r, k_lane + 64 * b, (unsigned)x.in_page * 16);
-                    kraw[b] = make_int4((int)half.x, (int)half.y, 0, 0);
+                    const u2v half = load8(x.r, k_lane + 256 * b, (unsigned)x.in_page * 16);
+                    raw.kraw[b] = make_int4((int)half.x, (int)half.y, 0, 0);
                 } else {
 #pragma unroll
                     for (int i = 0; i < NK; i++)
-                        kraw[b * NK + i] = load16(x.r, k_lane + 64 * b, (unsigned)(4 * i * P + x.in_page) * 16);
+                        raw.kraw[b * NK + i] = load16(x.r, k_lane + 256 * b, (unsigned)(4 * i * P + x.in_page) * 16);
                 }
-                kf[b] = load_kf<D>(x.r, kf_lane + 4 * b * (D / 32), (unsigned)x.in_page * (D / 32));
+                raw.kf[b] = load_kf<D>(x.r, kf_lane + 4 * b * (D / 32), (unsigned)x.in_page * (D / 32));
                 continue;
             }
 #pragma unroll
             for (int i = 0; i < NK; i++) {
                 const int unit = few_k_unit(ES, i, 0);
-                kraw[b * NK + i] = load16(x.r, k_lane + 64 * b, (unsigned)(unit * P + x.in_page) * 16);
+                raw.kraw[b * NK + i] = load16(x.r, k_lane + 64 * b, (unsigned)(unit * P + x.in_page) * 16);
             }
-            if (ES == 4) k_own[b] = dev::bldf(x.r, (unsigned)(2 * P * D * ES) + 4 * (x.in_page + few_pos(n, b)));
+            if (ES == 4) raw.k_own[b] = dev::bldf(x.r, (unsigned)(2 * P * D * ES) + 4 * (x.in_page + few_pos(n, b)));
         }
     };
-    auto load_v = [&](const Where &x) {
+    auto load_v = [&](Raw &raw) {
+        const Where &x = raw.x;
         if constexpr (ES == MX) {
             const unsigned at = x.v_at(D / 2), f_at = x.v_at(D / 32);
 #pragma unroll
             for (int i = 0; i < D / 64; i++) {
-                vraw[i] = load16(x.r, v_lane + 1024 * i, at);
-                vf[i] = load16(x.r, vf_lane + 16 * i, f_at);
+                raw.vraw[i] = load16(x.r, v_lane + 1024 * i, at);
+                raw.vf[i] = load16(x.r, vf_lane + 16 * i, f_at);
             }
             return;
         }
@@ -756,21 +778,26 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
 #pragma unroll
         for (int db = 0; db < DB; db++) {
             if (ES == 1) {
-                vraw8[db % (ES == 1 ? DB : 1)] = load8(x.r, v_lane + 256 * db, at);
+                raw.vraw8[db % (ES == 1 ? DB : 1)] = load8(x.r, v_lane + 256 * db, at);
             } else {
 #pragma unroll
                 for (int c = 0; c < NV; c++)
-                    vraw[(db * NV + c) % (ES == 1 ? 1 : DB * NV)] = load16(x.r, v_lane + 256 * db + c * D * 16, at);
+                    raw.vraw[(db * NV + c) % (ES == 1 ? 1 : DB * NV)] = load16(x.r, v_lane + 256 * db + c * D * 16, at);
             }
         }
     };
 
     const int t_at = w.t_at + wave, t_end = w.t_end;
-    Where here;
+    Raw first, second;
+    first.k_own[0] = first.k_own[1] = 0.0f;
+    int ahead = 0;  // the next tile's page
     if (t_at < t_end) {
-        here = table.find(a, w, t_at, table.page_of(a, w, t_at));
-        load_k(here);
-        load_s(here);
+        const int page = table.page_of(a, w, t_at);
+        if (AHEAD) ahead = table.page_of(a, w, min(t_at + 4, t_end - 1));
+        first.x = table.find(a, w, t_at, page);
+        load_k(first);
+        load_s(first);
+        if (AHEAD) load_v(first);
     }
 
     h8 qh[NS], ql[PACKED ? 1 : NS];
@@ -792,9 +819,20 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
         }
     }
 
-    for (int t = t_at; t < t_end; t += 4) {
-        const int next_t = min(t + 4, t_end - 1), next_page = table.page_of(a, w, next_t);
-        load_v(here);
+    // one tile, out of raw, with the next one (this again behind the last) into next
+    auto step = [&](Raw &raw, Raw &next, int t) {
+        const int next_t = min(t + 4, t_end - 1);
+        int next_page = 0;
+        if constexpr (AHEAD) {
+            next.x = table.find(a, w, next_t, ahead);
+            ahead = table.page_of(a, w, min(t + 8, t_end - 1));
+            load_k(next);
+            load_s(next);
+            load_v(next);
+        } else {
+            next_page = table.page_of(a, w, next_t);
+            load_v(raw);
+        }
         __builtin_amdgcn_sched_barrier(0);
 
         // ---- scores: register 4 b + i is position start + 8 z + 4 b + i ----
@@ -803,10 +841,10 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
         for (int b = 0; b < 2; b++) {
             if constexpr (ES == MX) {
                 // the factor of the lane's unit, all of 32 dims
-                const unsigned f[2] = {kf[b].x >> (D == 64 ? 8 * (z >> 1) : 8 * z), kf[b].y >> (8 * z)};
+                const unsigned f[2] = {raw.kf[b].x >> (D == 64 ? 8 * (z >> 1) : 8 * z), raw.kf[b].y >> (8 * z)};
 #pragma unroll
                 for (int i = 0; i < NK; i++) {
-                    const int4 r = kraw[b * NK + i];
+                    const int4 r = raw.kraw[b * NK + i];
                     const float factor = mx_factor(f[i & 1], 0);
                     const unsigned word[4] = {(unsigned)r.x, (unsigned)r.y, (unsigned)r.z, (unsigned)r.w};
 #pragma unroll
@@ -819,7 +857,7 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
             } else if (ES == 1) {
 #pragma unroll
                 for (int i = 0; i < NK; i++) {
-                    const int4 r = kraw[b * NK + i];
+                    const int4 r = raw.kraw[b * NK + i];
                     const h8 k0 = codes8(r.x, r.y), k1 = codes8(r.z, r.w);
                     sc[b] = mfma(k0, qh[2 * i % NS], sc[b]);
                     if (!PACKED) sc[b] = mfma(k0, ql[2 * i % (PACKED ? 1 : NS)], sc[b]);
@@ -827,15 +865,15 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
                     if (!PACKED) sc[b] = mfma(k1, ql[(2 * i + 1) % (PACKED ? 1 : NS)], sc[b]);
                 }
             } else {
-                const float inv = ES == 4 ? inv_pow2(k_own[b]) : 0.0f;
+                const float inv = ES == 4 ? inv_pow2(raw.k_own[b]) : 0.0f;
 #pragma unroll
                 for (int i = 0; i < NS; i++) {
                     h8 kh, kl;
                     if (ES == 2) {
-                        kh = __builtin_bit_cast(h8, kraw[(b * NK + i) % (2 * NK)]);
+                        kh = __builtin_bit_cast(h8, raw.kraw[(b * NK + i) % (2 * NK)]);
                     } else {
-                        const float4 x = __builtin_bit_cast(float4, kraw[(b * NK + 2 * i) % (2 * NK)]);
-                        const float4 y = __builtin_bit_cast(float4, kraw[(b * NK + 2 * i + 1) % (2 * NK)]);
+                        const float4 x = __builtin_bit_cast(float4, raw.kraw[(b * NK + 2 * i) % (2 * NK)]);
+                        const float4 y = __builtin_bit_cast(float4, raw.kraw[(b * NK + 2 * i + 1) % (2 * NK)]);
                         const float f[8] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv, y.x * inv, y.y * inv, y.z * inv, y.w * inv};
                         split8(f, kh, kl);
                     }
@@ -845,21 +883,28 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
                 }
             }
         }
-        const int start = here.start;
-        const bool there = here.there;
+        const int start = raw.x.start;
+        const bool there = raw.x.there;
         const bool edge = !there || start + TILE - 1 > w.p_lo ||
                           (a.window != INT32_MAX && start + TILE > a.sinks && start < w.p_hi - a.window + 1);
-        here = table.find(a, w, next_t, next_page);
-        load_k(here);
-        float sk = ks, sv = vs;
-        load_s(here);
+        float sk, sv;
+        if constexpr (AHEAD) {
+            sk = raw.ks;
+            sv = raw.vs;
+        } else {
+            next.x = table.find(a, w, next_t, next_page);
+            load_k(next);
+            sk = copy(raw.ks);
+            sv = copy(raw.vs);
+            load_s(next);
+        }
         __builtin_amdgcn_sched_barrier(0);
         only_finite<ES>(sv, sk);
         float st[8];
         each<8>([&](auto i) {
             float s = sc[i >> 2][i.value & 3];
-            if (PACKED) s = s + other_half(s);
-            st[i] = s * of_lane<i>(sk);
+            if (PACKED) s = here_and_now(s + other_half(s));
+            st[i] = here_and_now(s * of_lane<i>(sk));
         });
         const float v_inv = ES == 4 ? inv_v<ES>(sv) : 0.0f;
 
@@ -899,7 +944,7 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
             each<8>([&](auto i) {
                 const float p = exp2_(__builtin_fmaf(st[i], rowf, shift));
                 part[i & 1] = part[i & 1] + p;
-                x[i] = p * of_lane<i>(sv);
+                x[i] = here_and_now(p * of_lane<i>(sv));
             });
             sum = __builtin_fmaf(part[0] + part[1], SUM_SCALE, sum);
             split8(x, ph, pl);
@@ -911,17 +956,17 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
         for (int db = 0; db < DB; db++) {
             h8 vh, vl;
             if constexpr (ES == MX) {
-                const int4 r = vraw[db / 4], f = vf[db / 4];
+                const int4 r = raw.vraw[db / 4], f = raw.vf[db / 4];
                 const unsigned word = (unsigned)(db % 4 == 0 ? r.x : db % 4 == 1 ? r.y : db % 4 == 2 ? r.z : r.w);
                 vh = mx8(word, 1.0f) * (db % 4 < 2 ? mx_factors((unsigned)f.x, (unsigned)f.y) : mx_factors((unsigned)f.z, (unsigned)f.w));
             } else if (ES == 1) {
-                const u2v r = vraw8[db % (ES == 1 ? DB : 1)];
+                const u2v r = raw.vraw8[db % (ES == 1 ? DB : 1)];
                 vh = codes8(r.x, r.y);
             } else if (ES == 2) {
-                vh = __builtin_bit_cast(h8, vraw[db % (ES == 1 ? 1 : DB * NV)]);
+                vh = __builtin_bit_cast(h8, raw.vraw[db % (ES == 1 ? 1 : DB * NV)]);
             } else {
-                const f4v x = __builtin_bit_cast(f4v, vraw[(2 * db) % (ES == 1 ? 1 : DB * NV)]);
-                const f4v y = __builtin_bit_cast(f4v, vraw[(2 * db + 1) % (ES == 1 ? 1 : DB * NV)]);
+                const f4v x = __builtin_bit_cast(f4v, raw.vraw[(2 * db) % (ES == 1 ? 1 : DB * NV)]);
+                const f4v y = __builtin_bit_cast(f4v, raw.vraw[(2 * db + 1) % (ES == 1 ? 1 : DB * NV)]);
                 float f[8];
                 each<8>([&](auto e) {
                     f[e] = __builtin_amdgcn_fmed3f((e < 4 ? x[e & 3] : y[e & 3]) * of_lane<e>(v_inv), -65504.0f, 65504.0f);
@@ -931,6 +976,14 @@ __device__ __forceinline__ void few_rows(const Args &a, Job &w, int wave, float 
             acc[db] = mfma(vh, ph, acc[db]);
             if (!PACKED) acc[db] = mfma(vh, pl, acc[db]);
             if (ES == 4) acc[db] = mfma(vl, ph, acc[db]);
+        }
+    };
+    for (int t = t_at; t < t_end; t += 4) {
+        step(first, AHEAD ? second : first, t);
+        if constexpr (AHEAD) {
+            t += 4;
+            if (t >= t_end) break;
+            step(second, first, t);
         }
     }
     sum = sum + shfl(sum, 16);
@@ -950,10 +1003,43 @@ constexpr int FEW = 8;  // rows (x group) of a sequence that few_rows takes besi
 
 // Waves a SIMD by the registers that the loop holds: many_rows' 32 columns, or
 // few_rows' query, sums, K, V and the rest.
-constexpr int waves_for(int es, int d, int rows) {
+constexpr int waves_for(int es, int d, int rows, bool ahead = false) {
     if (rows > 16) return d == 256 ? 1 : 2;
-    const int regs = d / 8 * (rows / 8) + d / 4 + (es == MX ? d / 8 : d * es / 4) + 60;
+    const int regs = d / 8 * (rows / 8) + d / 4 + (es != MX ? d * es / 4 : ahead ? d / 4 + 40 : d / 8) + 60;
     return regs <= 128 ? 4 : regs <= 172 ? 3 : regs <= 250 ? 2 : 1;
+}
+
+// find_seq of up to 64 sequences, the longest of them first: where there are more
+// workgroups than CUs, the last to start, or to have a CU's memory to themselves,
+// are then short ones (64 sequences of 1333 to 4000, 8 KV heads of 128: 4-bit rows
+// 47 us against 44, i8 73.8 against 70.3).  Each lane adds up the tiles of
+// those before its own.  False too for sequences of about one length, which stay as
+// they come: sorting takes 0.5 us.
+template <typename F>
+__device__ __forceinline__ bool find_longest_first(const Batch &b, int tile, F count, int &seq, Seq &s, int &local, int &n) {
+    const int lane = threadIdx.x & 63;
+    const bool has = lane < b.n_seq;
+    Seq mine{0, 0, 0};
+    if (has) mine.load(b, lane);
+    const int len0 = __builtin_amdgcn_readfirstlane(mine.len), tiles = has ? count(mine) : 0;
+    if (!__ballot(has && abs(mine.len - len0) > len0 / 8)) return false;
+    const int key = min(mine.len, 1 << 24) << 6 | (63 - lane);  // all different, those of lanes that have none last
+    int first = 0;
+    if (b.row_start) {
+#pragma unroll
+        for (int j = 0; j < 64; j++)
+            first += __builtin_amdgcn_readlane(key, j) > key ? __builtin_amdgcn_readlane(tiles, j) : 0;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 64; j++) first += __builtin_amdgcn_readlane(key, j) > key;
+        first *= tiles;
+    }
+    const unsigned long long here = __ballot(tile >= first && tile - first < tiles);
+    seq = here ? __builtin_ctzll(here) : 0;
+    n = __builtin_amdgcn_readlane(tiles, seq);
+    local = here ? tile - __builtin_amdgcn_readlane(first, seq) : n;  // past the last tile: no rows
+    s = mine.of_lane(seq);
+    return true;
 }
 
 // A workgroup takes ROWS rows: its waves share 8, 16 or 32, or take 32 of 128
@@ -962,8 +1048,8 @@ constexpr int waves_for(int es, int d, int rows) {
 // go over the whole of the positions (a prompt of 3000 beside 63 single tokens
 // behind 3000 to 4000, 32 heads on 2 of 128: i8 282 us against 183, f32 517 against
 // 390).
-template <int ES, int D, int ROWS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(waves_for(ES, D, ROWS))))
+template <int ES, int D, int ROWS, bool AHEAD = false>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(waves_for(ES, D, ROWS, AHEAD))))
 void attn_kernel(Args a) {
     constexpr int REGS = ROWS > 16 ? D / 2 : D / 4;  // of a lane, that join_waves takes
     __shared__ __attribute__((aligned(16))) float lds[join_floats<REGS>()];
@@ -976,8 +1062,10 @@ void attn_kernel(Args a) {
     const int tile = rest / a.splits;
     Seq seq;
     int local, tiles;
-    if (a.b.row_start) {
-        auto count = [&](const Seq &q) { return (q.n * a.group + ROWS - 1) / ROWS; };
+    auto count = [&](const Seq &q) { return (q.n * a.group + ROWS - 1) / ROWS; };
+    if (a.longest_first && find_longest_first(a.b, tile, count, w.seq, seq, local, tiles)) {
+        if (local >= tiles) return;
+    } else if (a.b.row_start) {
         if (!find_seq(a.b, tile, count, w.seq, seq, local, tiles)) return;
     } else {
         tiles = a.tiles_per;
@@ -992,9 +1080,9 @@ void attn_kernel(Args a) {
     w.row0 = (tiles - 1 - local) * ROWS;
     w.nr = min(seq_rows * a.group - w.row0, ROWS);
     if constexpr (ROWS <= 16) {
-        few_rows<ES, D, ROWS>(a, w, wave, lds);
+        few_rows<ES, D, ROWS, AHEAD>(a, w, wave, lds);
     } else if (seq_rows * a.group <= FEW) {
-        few_rows<ES, D, FEW>(a, w, wave, lds);
+        few_rows<ES, D, FEW, false>(a, w, wave, lds);
     } else if (ROWS == 32 || w.nr <= 32) {
         many_rows<ES, D, 4>(a, w, wave, lds);
     } else if constexpr (ROWS == 128) {
@@ -1068,7 +1156,10 @@ __global__ __launch_bounds__(256) void merge_kernel(Args a) {
 
 template <int ES, int D>
 int launch(const Args &a, const AttnPlan &p, unsigned blocks, size_t items, hipStream_t stream) {
-    if (p.tile_rows == 8) attn_kernel<ES, D, 8><<<blocks, 256, 0, stream>>>(a);
+    if (ES == MX && p.ahead) {
+        if (p.tile_rows == 8) attn_kernel<ES, D, 8, ES == MX><<<blocks, 256, 0, stream>>>(a);
+        else attn_kernel<ES, D, 16, ES == MX><<<blocks, 256, 0, stream>>>(a);
+    } else if (p.tile_rows == 8) attn_kernel<ES, D, 8><<<blocks, 256, 0, stream>>>(a);
     else if (p.tile_rows == 16) attn_kernel<ES, D, 16><<<blocks, 256, 0, stream>>>(a);
     else if (p.tile_rows == 32) attn_kernel<ES, D, 32><<<blocks, 256, 0, stream>>>(a);
     else attn_kernel<ES, D, 128><<<blocks, 256, 0, stream>>>(a);
@@ -1184,6 +1275,11 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
             p.join_waves = p.splits > 8 && (size_t)b.n_rows * n_head <= cus ? 4 : 1;
         }
     }
+    const size_t all = blocks * p.splits;
+    p.ahead = kv->es == MX && p.tile_rows <= 16 && all <= cus;
+    const int ahead = env_int("KVAD_PAGED_AHEAD", -1);  // for experiments, and for tests of both
+    if (ahead >= 0) p.ahead = ahead && kv->es == MX && p.tile_rows <= 16;
+    p.longest_first = p.splits == 1 && b.n_seq > 1 && b.n_seq <= 64 && all > cus;
     return p;
 }
 
@@ -1209,6 +1305,7 @@ int launch_attn(kh_ctx *ctx, const AttnCall &c, const AttnPlan &p) {
     a.tiles_per = p.per;
     a.splits = p.splits;
     a.split_tiles = p.split_tiles;
+    a.longest_first = p.longest_first;
     a.window = c.window;
     a.sinks = c.sinks;
     a.scale = c.scale;

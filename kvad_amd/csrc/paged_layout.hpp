@@ -34,14 +34,18 @@ KH_HD int stored_dims(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 1
 // row's times the row's f32 scale.  Of a block, K's codes and V's, then K's
 // factors and V's, then the scales:
 //   K        [dim / 32][position][32 dims]              a lane's unit: a factor's dims
+//            positions of a tile of 32 in the order of mx_slot
 //   V        [position / 32][dim / 64][position / 8 % 4][dim % 16][dim / 16 % 4][8 positions]
 //   factors  K [position][dim / 32], V [position / 8][dim / 32][8 positions]
 // V's unit of 16 bytes is 8 positions of the four dims 16 apart that a lane of
 // the 16x16x32 product has of 64: one load, where single dims would be four.
-constexpr int MX = 0, MX_GROUP = 32;
+// K's order of positions: a block of 16 of the 16x16x32 product (few_pos, below)
+// lies together, whole lines a load.
+constexpr int MX = 0;
+KH_HD int mx_slot(int pos) { return (pos & ~31) | (pos >> 2 & 1) << 4 | (pos >> 3 & 3) << 2 | (pos & 3); }
 KH_HD size_t mx_block_bytes(int d, int page) { return (size_t)page * (d + d / 16 + 8); }
 // the byte of a code; an even dim's (K) or position's (V) is its low half
-KH_HD int mx_k_off(int page, int pos, int dim) { return (dim / 32 * page + pos) * 16 + dim % 32 / 2; }
+KH_HD int mx_k_off(int page, int pos, int dim) { return (dim / 32 * page + mx_slot(pos)) * 16 + dim % 32 / 2; }
 KH_HD int mx_v_off(int d, int page, int pos, int dim) {
     return page * d / 2 + pos / 32 * 16 * d + dim / 64 * 1024 + pos / 8 % 4 * 256 + dim % 16 * 16 + dim / 16 % 4 * 4 + pos % 8 / 2;
 }
@@ -106,6 +110,9 @@ KH_HD int few_v_off(int es, int d, int c, int z) {
 // products of a word each; V's are words of 8 positions, quarters 2 h and 2 h + 1
 // of the tile, the lane's dims of 64 being two that lie beside each other in a
 // unit, for the two dim tiles t of the 64.
+// The lane's place among K's positions: mx_slot of the position that row m has.
+KH_HD int mx_tile_slot(int m) { return mx_slot(tile_pos(m)); }
+KH_HD int mx_few_slot(int m, int b) { return 16 * b + m; }
 KH_HD int mx_k_dim(int s, int h, int e) { return 64 * (s >> 2) + 32 * h + 8 * (s & 3) + e; }
 KH_HD int mx_v_dim(int dt, int n) { return 64 * (dt >> 1) + (n & 15) + 32 * (n >> 4) + 16 * (dt & 1); }
 // 16x16x32: K's load j (of d / 128) is unit 4 j + z, four products; of 64 dims

@@ -201,6 +201,53 @@ def test_small_values_before_large_ones_keep_their_weights(ctx, form, monkeypatc
     T.test_small_values_before_large_ones_keep_their_weights(ctx, form, monkeypatch, MX, small, large, splits)
 
 
+@pytest.mark.parametrize("ahead", ["0", "1"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_one_tile_or_two_at_a_time(ctx, monkeypatch, ahead, hd):
+    # both ways few rows are done, to the bit: no tile, one, two, an odd number
+    # of a wave's; windows that leave tiles out; splits
+    p = Pool(ctx, np.random.default_rng(hd), MX, 2, hd, 32, [700, 130, 33, 1])
+    p.push([690, 127, 32, 0])
+    p.push([10, 3, 1, 1])
+    q = (p.rng.standard_normal((15, 4, hd)) * 1.5).astype(np.float32)
+    for tile in ("8", "16"):
+        for splits in ("1", "3"):
+            outs = []
+            for each in (ahead, "0"):
+                monkeypatch.setenv("KVAD_PAGED_TILE", tile)
+                monkeypatch.setenv("KVAD_PAGED_SPLITS", splits)
+                monkeypatch.setenv("KVAD_PAGED_AHEAD", each)
+                outs.append([p.check([10, 3, 1, 1], 4, q=q), p.check([10, 3, 1, 1], 4, q=q, window=150, sinks=3)])
+            for a, b in zip(*outs):
+                np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("precision", [MX, "i8", "f32"])
+@pytest.mark.parametrize("n_seq, kv, ragged", [(64, 8, False), (64, 8, True), (37, 8, False), (37, 9, True), (65, 8, False), (2, 200, True)])
+def test_the_longest_sequences_go_first(ctx, precision, n_seq, kv, ragged):
+    # more workgroups than CUs over sequences of very different lengths, none and
+    # alike ones among them: each gets its own
+    rng = np.random.default_rng(n_seq + kv)
+    lens = [int(n) for n in rng.integers(1, 150, n_seq)]
+    lens[0], lens[-1], lens[n_seq // 2] = 149, 149, 1
+    counts = [1] * n_seq
+    if ragged:
+        counts = [int(rng.integers(0, min(n, 3) + 1)) for n in lens]
+        lens[1] = counts[1] = 0
+    p = Pool(ctx, rng, precision, kv, 64, 32, lens)
+    p.push([n - c for n, c in zip(lens, counts)])
+    p.push(counts)
+    b = K.Batch.host(lens, p.pages, counts) if ragged else K.Batch.host(lens, p.pages, None, n_rows=n_seq)
+    q = (rng.standard_normal((sum(counts), kv, 64)) * 1.5).astype(np.float32)
+    p.check(counts, kv, q=q, got=p.cache.attend(0, b, kv, q))
+    # all of one length, longest_first's other way
+    same = [min(lens[0], 100)] * n_seq
+    p2 = Pool(ctx, rng, precision, kv, 64, 32, same)
+    p2.push(same)
+    q = (rng.standard_normal((n_seq, kv, 64)) * 1.5).astype(np.float32)
+    p2.check([1] * n_seq, kv, q=q, got=p2.cache.attend(0, K.Batch.host(same, p2.pages, None, n_rows=n_seq), kv, q))
+
+
 @pytest.mark.parametrize("size", [-80, -95, -105, -112, -120, 93])
 def test_values_of_one_size(ctx, form, size):  # noqa: F811
     T.test_values_of_one_size(ctx, form, MX, size)

@@ -42,7 +42,7 @@ int main() {
             for (int lane = 0; lane < 64; lane++) {
                 // 32x32x16, as the kernel adds the offsets up: the lane's part, and the load's
                 const int n = lane & 31, h = lane >> 5;
-                const int k_lane = (k_load_unit(MX, 0, h) * page + tile_pos(n)) * 16, pos = in_page + tile_pos(n);
+                const int k_lane = (k_load_unit(MX, 0, h) * page + mx_tile_slot(n)) * 16, pos = in_page + tile_pos(n);
                 std::vector<int> dims(d, 0);
                 for (int j = 0; j < d / 64; j++) for (int w = 0; w < 4; w++) for (int e = 0; e < 8; e++) {
                     const int dim = mx_k_dim(4 * j + w, h, e);
@@ -71,7 +71,7 @@ int main() {
                 const int r16 = lane & 15, z = lane >> 4;
                 for (int b = 0; b < 2; b++) for (int j = 0; j < (d + 127) / 128; j++) {
                     const int p = in_page + few_pos(r16, b);
-                    const int off = mx_few_k_lane(d, page, z) + few_pos(r16, 0) * 16 + 64 * b + (4 * j * page + in_page) * 16;
+                    const int off = mx_few_k_lane(d, page, z) + mx_few_slot(r16, 0) * 16 + 256 * b + (4 * j * page + in_page) * 16;
                     MUST(off % 8 == 0 && (size_t)off + (d == 64 ? 8 : 16) <= block);
                     for (int w = 0; w < (d == 64 ? 2 : 4); w++) for (int e = 0; e < 8; e++) {
                         const int dim = mx_few_k_dim(d, 4 * j + w, z, e);
