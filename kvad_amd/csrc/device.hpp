@@ -81,6 +81,22 @@ __device__ __forceinline__ float wave_sum(float v) {
     return (a + b) + (c + d);
 }
 
+// The sums of the lanes up to and with each one.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // in rows of 16: the lane 1, 2, 4, 8 below
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // the last of a row to the next one,
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // then of two rows to the other two
+}
+// The largest of each run of 8 lanes, in all of them.
+__device__ __forceinline__ int max_of_8(int v) {
+    v = max(v, dpp<DPP_XOR1>(v));
+    v = max(v, dpp<DPP_XOR2>(v));
+    return max(v, dpp<DPP_HALF_MIRROR>(v));
+}
+
 // Xor over the wave (every lane gets it).
 __device__ __forceinline__ unsigned wave_xor(unsigned v) {
     for (int o = WAVE / 2; o > 0; o >>= 1) v ^= (unsigned)__shfl_xor((int)v, o);

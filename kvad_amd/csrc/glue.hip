@@ -13,6 +13,7 @@
 // that the device holds (kh_rope_rows_dev, the same products and sums), and the
 // end of a block fused with the norms around it (kh_norm_residual_dev).
 #include <cmath>
+#include <type_traits>
 
 #include "common.hpp"
 #include "device.hpp"
@@ -177,20 +178,22 @@ struct NormResidual {
     int n;
 };
 
-// Four floats from i on of a row of n; what is past its end is zero.
+// Four floats from i on of a row of n; what is past its end is zero.  FOURS: n is a
+// multiple of four, and a load is one instruction that nothing waits for.
+template <bool FOURS>
 __device__ __forceinline__ float4u load4(const float *p, int i, int n) {
-    if (i + 4 <= n) return *reinterpret_cast<const float4u *>(p + i);
     float4u v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (i + 4 <= n) v = *reinterpret_cast<const float4u *>(p + i);
+    if (FOURS || i + 4 <= n) return v;
 #pragma unroll
     for (int e = 0; e < 3; e++)
         if (i + e < n) v[e] = p[i + e];
     return v;
 }
+template <bool FOURS>
 __device__ __forceinline__ void store4(float *p, int i, int n, float4u v) {
-    if (i + 4 <= n) {
-        *reinterpret_cast<float4u *>(p + i) = v;
-        return;
-    }
+    if (i + 4 <= n) *reinterpret_cast<float4u *>(p + i) = v;
+    if (FOURS || i + 4 <= n) return;
 #pragma unroll
     for (int e = 0; e < 3; e++)
         if (i + e < n) p[i + e] = v[e];
@@ -216,7 +219,7 @@ __device__ __forceinline__ float row_sum(float v, float *s_red) {
 // W waves hold a row, V times four floats a lane: everything is read once and
 // all loads are in flight together.  With one wave a row a workgroup takes four
 // rows and nothing waits at a barrier.
-template <int W, int V>
+template <int W, int V, bool FOURS>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_residual_kernel(NormResidual a) {
     __shared__ float s_red[2][W];
     const size_t r = W == 1 ? (size_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
@@ -226,15 +229,15 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_residual_kernel(No
 #pragma unroll
     for (int j = 0; j < V; j++) {
         const int i = 4 * (lane + 64 * W * j);
-        y[j] = load4(a.y + r * n, i, n);
-        x[j] = load4(a.x + r * n, i, n);
+        y[j] = load4<FOURS>(a.y + r * n, i, n);
+        x[j] = load4<FOURS>(a.x + r * n, i, n);
     }
 #pragma unroll
     for (int j = 0; j < V; j++) {
         const int i = 4 * (lane + 64 * W * j);
-        if (a.post) post[j] = load4(a.post, i, n);
-        if (a.gate) g[j] = load4(a.gate + r * a.gate_stride, i, n);
-        if (a.pre) pre[j] = load4(a.pre, i, n);
+        if (a.post) post[j] = load4<FOURS>(a.post, i, n);
+        if (a.gate) g[j] = load4<FOURS>(a.gate + r * a.gate_stride, i, n);
+        if (a.pre) pre[j] = load4<FOURS>(a.pre, i, n);
     }
     float sum = 0.0f;
     if (a.post) {
@@ -250,12 +253,12 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_residual_kernel(No
         const float4u t = a.gate ? y[j] * g[j] : y[j];
         x[j] = x[j] + t * a.scale;
         sum = sum + squares(x[j]);
-        store4(a.x_out + r * n, 4 * (lane + 64 * W * j), n, x[j]);
+        store4<FOURS>(a.x_out + r * n, 4 * (lane + 64 * W * j), n, x[j]);
     }
     if (!a.pre) return;
     const float inv = 1.0f / sqrtf(row_sum<W>(sum, s_red[1]) / (float)n + a.eps);
 #pragma unroll
-    for (int j = 0; j < V; j++) store4(a.out + r * n, 4 * (lane + 64 * W * j), n, x[j] * inv * pre[j]);
+    for (int j = 0; j < V; j++) store4<FOURS>(a.out + r * n, 4 * (lane + 64 * W * j), n, x[j] * inv * pre[j]);
 }
 
 // Rows that registers do not hold: y is read twice, and x' again where it was
@@ -268,21 +271,21 @@ __global__ __launch_bounds__(1024) void norm_residual_long_kernel(NormResidual a
     float *xo = a.x_out + r * n;
     float inv = 1.0f, sum = 0.0f;
     if (a.post) {
-        for (int i = 4 * threadIdx.x; i < n; i += 4096) sum = sum + squares(load4(y, i, n));
+        for (int i = 4 * threadIdx.x; i < n; i += 4096) sum = sum + squares(load4<false>(y, i, n));
         inv = 1.0f / sqrtf(row_sum<16>(sum, s_red[0]) / (float)n + a.eps);
     }
     sum = 0.0f;
     for (int i = 4 * threadIdx.x; i < n; i += 4096) {
-        float4u t = load4(y, i, n);
-        if (a.post) t = t * inv * load4(a.post, i, n);
-        if (g) t = t * load4(g, i, n);
-        t = load4(x, i, n) + t * a.scale;
+        float4u t = load4<false>(y, i, n);
+        if (a.post) t = t * inv * load4<false>(a.post, i, n);
+        if (g) t = t * load4<false>(g, i, n);
+        t = load4<false>(x, i, n) + t * a.scale;
         sum = sum + squares(t);
-        store4(xo, i, n, t);
+        store4<false>(xo, i, n, t);
     }
     if (!a.pre) return;
     inv = 1.0f / sqrtf(row_sum<16>(sum, s_red[1]) / (float)n + a.eps);
-    for (int i = 4 * threadIdx.x; i < n; i += 4096) store4(a.out + r * n, i, n, load4(xo, i, n) * inv * load4(a.pre, i, n));
+    for (int i = 4 * threadIdx.x; i < n; i += 4096) store4<false>(a.out + r * n, i, n, load4<false>(xo, i, n) * inv * load4<false>(a.pre, i, n));
 }
 
 // Whether two runs of floats share one; a null one shares none.
@@ -417,13 +420,18 @@ int kh_norm_residual_dev(kh_ctx *ctx, const float *x, const float *y, const floa
         (void)hipSetDevice(ctx->device);
         const unsigned g = (unsigned)groups;
         hipStream_t s = ctx->stream;
-        if (n <= 256) norm_residual_kernel<1, 1><<<g, 256, 0, s>>>(a);
-        else if (n <= 512) norm_residual_kernel<1, 2><<<g, 256, 0, s>>>(a);
-        else if (n <= 1024) norm_residual_kernel<1, 4><<<g, 256, 0, s>>>(a);
-        else if (n <= 2048) norm_residual_kernel<4, 2><<<g, 256, 0, s>>>(a);
-        else if (n <= 4096) norm_residual_kernel<4, 4><<<g, 256, 0, s>>>(a);
-        else if (n <= 8192) norm_residual_kernel<16, 2><<<g, 1024, 0, s>>>(a);
-        else norm_residual_long_kernel<<<g, 1024, 0, s>>>(a);
+        auto run = [&](auto fours) {
+            constexpr bool F = decltype(fours)::value;
+            if (n <= 256) norm_residual_kernel<1, 1, F><<<g, 256, 0, s>>>(a);
+            else if (n <= 512) norm_residual_kernel<1, 2, F><<<g, 256, 0, s>>>(a);
+            else if (n <= 1024) norm_residual_kernel<1, 4, F><<<g, 256, 0, s>>>(a);
+            else if (n <= 2048) norm_residual_kernel<4, 2, F><<<g, 256, 0, s>>>(a);
+            else if (n <= 4096) norm_residual_kernel<4, 4, F><<<g, 256, 0, s>>>(a);
+            else norm_residual_kernel<16, 2, F><<<g, 1024, 0, s>>>(a);
+        };
+        if (n > 8192) norm_residual_long_kernel<<<g, 1024, 0, s>>>(a);
+        else if (n % 4) run(std::false_type{});
+        else run(std::true_type{});
         KH_HIP(hipGetLastError());
         return KH_OK;
     });

@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256) void push_kernel(MoveArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; e++)  // magnitudes compare as their bits do, NaN above infinity
                 amax = max(amax, __builtin_bit_cast(int, (float)f[what][j][e]) & 0x7fffffff);
-        for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor(amax, o));
+        amax = dev::max_of_8(amax);
         float inv;
         const float scale = scale_of<ES>(amax, inv);
         const bool finite = amax < 0x7f800000;
@@ -264,10 +264,6 @@ __device__ __forceinline__ unsigned mx_codes(float4u x, int e) {
     const unsigned lo = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, ldexpf(x[0], -e), ldexpf(x[1], -e), 1.0f, 0);
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(lo, ldexpf(x[2], -e), ldexpf(x[3], -e), 1.0f, 1) & 0xffff;
 }
-__device__ __forceinline__ int max8(int v) {
-    for (int o = 1; o < 8; o <<= 1) v = max(v, __shfl_xor(v, o));
-    return v;
-}
 
 // As push_kernel.  A group's 32 dims are one step of the 8 lanes that have a row.
 // V's words of 8 positions that the run fills in part keep the rest of theirs: they
@@ -314,7 +310,7 @@ __global__ __launch_bounds__(256) void push_mx_kernel(MoveArgs a) {
             int amax = 0;
 #pragma unroll
             for (int i = 0; i < 4; i++) amax = max(amax, __builtin_bit_cast(int, (float)f[what][j][i]) & 0x7fffffff);
-            amax = max8(amax);
+            amax = dev::max_of_8(amax);
             finite = finite && amax < 0x7f800000;
             e[j] = mx_exp(amax);
             top = max(top, e[j]);

@@ -68,11 +68,7 @@ __device__ __forceinline__ bool find_seq(const Batch &b, int tile, F count, int 
         Seq mine{0, 0, 0};
         if (base + lane < b.n_seq) mine.load(b, base + lane);
         const int c = count(mine);
-        int sum = c;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int up = __shfl_up(sum, o);
-            if (lane >= o) sum += up;
-        }
+        const int sum = dev::wave_scan(c);
         const int all = __builtin_amdgcn_readlane(sum, 63);
         if (tile < all) {
             const int l = __builtin_ctzll(__ballot(sum > tile));

@@ -7,7 +7,7 @@
 // for itself (two numbers each, in LDS: reading them again costs less than a
 // second launch), then its share of the rows and pages, each found by bisection.
 // The arrays that all of them read, the lengths and the stack's height, are
-// written by the last to finish.  Whether the call can be done is known from
+// written by the last to have read them.  Whether the call can be done is known from
 // the sums: all workgroups find the same, and either all do it or none.
 //
 // What bounds it: trips to memory one behind the other, and the launch.
@@ -20,6 +20,8 @@ namespace pages {
 namespace {
 
 constexpr int THREADS = 256, MAX_SEQ = 4096, ROWS = 4;  // rows a thread takes at a time
+typedef int i4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef long l2 __attribute__((ext_vector_type(2), aligned(8)));
 constexpr int LIMIT = 1 << 30;                          // positions and rows are below it
 
 // kh_page_table's status
@@ -39,14 +41,13 @@ __device__ __forceinline__ int pages_for(int positions, int shift) { return (int
 __device__ __forceinline__ int add(int a, int b) { return (int)min((unsigned)a + (unsigned)b, (unsigned)LIMIT); }
 
 // What a call makes of a sequence: rows (none for a release) and pages given or
-// taken back, from where on in its table.
+// taken back, from column `first` of its table on.
 struct Change {
     int rows, pages, first, bad;
 };
 template <bool STEP>
-__device__ __forceinline__ Change change_of(const Args &a, int s) {
+__device__ __forceinline__ Change change_of(const Args &a, int len, int arg) {
     const int cap = a.max_pages << a.page_shift;
-    int len = a.len[s], arg = a.rows[s];
     Change c{0, 0, 0, DONE};
     if (len < 0 || len > cap) {
         c.bad = BAD_TABLE;
@@ -68,55 +69,73 @@ __device__ __forceinline__ Change change_of(const Args &a, int s) {
     return c;
 }
 
-// The sums before each sequence, in LDS, and over all of them.
+// Of each sequence the sums before it, its length (of a release: the positions it
+// keeps) and what it had before, in LDS; and what all workgroups find alike.
 struct Sums {
-    int rows[MAX_SEQ], pages[MAX_SEQ];
-    int wave_rows[THREADS / 64], wave_pages[THREADS / 64];
+    int rows[MAX_SEQ], pages[MAX_SEQ], len[MAX_SEQ];
+    int wave_rows[THREADS / 64], wave_pages[THREADS / 64], wave_bad[THREADS / 64];
 };
-__device__ __forceinline__ int scan(int v, int lane) {
-    for (int o = 1; o < 64; o <<= 1) {
-        const int up = __shfl_up(v, o);
-        if (lane >= o) v = add(v, up);
-    }
-    return v;
+struct Totals {
+    int rows, pages, bad, n_free;
+};
+// The sums up to and with each lane's.
+template <int CTRL, int ROWS_TO>
+__device__ __forceinline__ int below(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS_TO, 0xf, false);
 }
-// Returns the worst of the sequences' faults, in every thread.
+__device__ __forceinline__ int scan(int v) {
+    v = add(v, below<0x111, 0xf>(v));  // within rows of 16: the lane 1, 2, 4, 8 below
+    v = add(v, below<0x112, 0xf>(v));
+    v = add(v, below<0x114, 0xf>(v));
+    v = add(v, below<0x118, 0xf>(v));
+    v = add(v, below<0x142, 0xa>(v));  // the last of a row to the next one, then of two rows
+    return add(v, below<0x143, 0xc>(v));
+}
+// With n_seq <= THREADS a thread has one sequence, and nothing is read twice.
 template <bool STEP>
-__device__ __forceinline__ int sum_up(const Args &a, Sums &s, int &rows, int &pages) {
+__device__ __forceinline__ Totals sum_up(const Args &a, Sums &s) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int each = (a.n_seq + THREADS - 1) / THREADS, from = threadIdx.x * each, to = min(from + each, a.n_seq);
+    const int each = (a.n_seq + THREADS - 1) / THREADS, from = min((int)threadIdx.x * each, a.n_seq), to = min(from + each, a.n_seq);
+    Totals t{0, 0, DONE, *a.n_free};
     int r = 0, p = 0, bad = DONE;
     for (int i = from; i < to; i++) {
-        const Change c = change_of<STEP>(a, i);
+        const int len = a.len[i], arg = a.rows[i];
+        const Change c = change_of<STEP>(a, len, arg);
         s.rows[i] = r;
         s.pages[i] = p;
+        s.len[i] = STEP ? len : arg;
         r = add(r, c.rows);
         p = add(p, c.pages);
         bad = max(bad, c.bad);
     }
-    const int r_to = scan(r, lane), p_to = scan(p, lane);
+    const int r_to = scan(r), p_to = scan(p);
+    for (int why = BAD_TABLE; why > DONE; why--)
+        if (__ballot(bad == why)) {
+            t.bad = why;
+            break;
+        }
     if (lane == 63) {
         s.wave_rows[wave] = r_to;
         s.wave_pages[wave] = p_to;
+        s.wave_bad[wave] = t.bad;
     }
-    const int worst = __syncthreads_or(bad == BAD_TABLE) ? BAD_TABLE : __syncthreads_or(bad == BAD_ROWS) ? BAD_ROWS : __syncthreads_or(bad == TOO_LONG) ? TOO_LONG : DONE;
-    int r0 = __shfl_up(r_to, 1), p0 = __shfl_up(p_to, 1);
-    if (lane == 0) r0 = p0 = 0;
-    rows = pages = 0;
+    __syncthreads();
+    int r0 = r_to - r, p0 = p_to - p;  // of the wave's lanes before this one, unless a sum has stopped: then nothing is done
     for (int w = 0; w < THREADS / 64; w++) {
         if (w < wave) {
             r0 = add(r0, s.wave_rows[w]);
             p0 = add(p0, s.wave_pages[w]);
         }
-        rows = add(rows, s.wave_rows[w]);
-        pages = add(pages, s.wave_pages[w]);
+        t.rows = add(t.rows, s.wave_rows[w]);
+        t.pages = add(t.pages, s.wave_pages[w]);
+        t.bad = max(t.bad, s.wave_bad[w]);
     }
     for (int i = from; i < to; i++) {
         s.rows[i] = add(s.rows[i], r0);
         s.pages[i] = add(s.pages[i], p0);
     }
     __syncthreads();
-    return worst;
+    return t;
 }
 // The last sequence that starts at i or before it: the one that has item i.
 __device__ __forceinline__ int find(const int *starts, int n, int i) {
@@ -129,18 +148,18 @@ __device__ __forceinline__ int find(const int *starts, int n, int i) {
     return lo;
 }
 
-// Whether this workgroup is the last of the launch to come here.
+// Whether this workgroup is the last of the launch to have read the arrays that are
+// then written; asked early, as nothing waits for the answer but the first wave, whose
+// it is (the others get false).
 __device__ __forceinline__ bool last_one(const Args &a) {
-    __syncthreads();
+    if (threadIdx.x >= 64) return false;
     if (gridDim.x == 1) return true;
-    __shared__ int s_last;
+    int last = 0;
     if (threadIdx.x == 0) {
-        __threadfence();
-        s_last = atomicAdd(&a.status[ARRIVED], 1) == (int)gridDim.x - 1;
-        if (s_last) a.status[ARRIVED] = 0;
+        last = __hip_atomic_fetch_add(&a.status[ARRIVED], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+        if (last) a.status[ARRIVED] = 0;
     }
-    __syncthreads();
-    return s_last;
+    return __builtin_amdgcn_readfirstlane(last) != 0;
 }
 __device__ __forceinline__ void report(const Args &a, int reason) {
     a.status[REASON] = reason;
@@ -149,86 +168,101 @@ __device__ __forceinline__ void report(const Args &a, int reason) {
 
 __global__ __launch_bounds__(THREADS) void step_kernel(Args a) {
     __shared__ Sums s;
-    int rows, need;
-    int reason = sum_up<true>(a, s, rows, need);
-    const int n_free = *a.n_free;
-    if (n_free < 0 || n_free > a.n_pages) reason = BAD_TABLE;
-    else if (reason == DONE && rows > a.n_rows) reason = BAD_ROWS;
-    else if (reason == DONE && need > n_free) reason = SHORT;
-    if (reason != DONE) rows = need = 0;
+    const Totals t = sum_up<true>(a, s);
+    const bool last = last_one(a);
+    int reason = t.bad;
+    if (t.n_free < 0 || t.n_free > a.n_pages) reason = BAD_TABLE;
+    else if (reason == DONE && t.rows > a.n_rows) reason = BAD_ROWS;
+    else if (reason == DONE && t.pages > t.n_free) reason = SHORT;
+    const int rows = reason == DONE ? t.rows : 0, need = reason == DONE ? t.pages : 0;
     const int at = blockIdx.x * THREADS + threadIdx.x, step = gridDim.x * THREADS;
+    const int32_t *top = a.free_pages + t.n_free - 1;
     // pages into the tables, from the stack's top
     for (int i = at; i < need; i += step) {
         const int q = find(s.pages, a.n_seq, i);
-        a.pages[(size_t)q * a.max_pages + pages_for(a.len[q], a.page_shift) + (i - s.pages[q])] = a.free_pages[n_free - 1 - i];
+        a.pages[(size_t)q * a.max_pages + pages_for(s.len[q], a.page_shift) + (i - s.pages[q])] = top[-i];
     }
-    // positions and slots
+    // positions and slots, ROWS rows a thread: of one sequence and one page, or each found by itself
     const int mask = (1 << a.page_shift) - 1;
+    auto page_of = [&](int q, int position) {
+        const int column = position >> a.page_shift, fresh = column - pages_for(s.len[q], a.page_shift);
+        const int page = fresh < 0 ? a.pages[(size_t)q * a.max_pages + column] : top[-s.pages[q] - fresh];
+        return page >= 0 && page < a.n_pages ? (int64_t)page << a.page_shift : (int64_t)-1;
+    };
+    auto end_of = [&](int q) { return q + 1 < a.n_seq ? s.rows[q + 1] : rows; };
     for (int i = at * ROWS; i < a.n_rows; i += step * ROWS) {
-        int q = i < rows ? find(s.rows, a.n_seq, i) : 0;
-        int len = a.len[q], next = q + 1 < a.n_seq ? s.rows[q + 1] : rows, column = -1, page = -1;
+        int position[ROWS];
+        int64_t slot[ROWS];
+        int q = find(s.rows, a.n_seq, min(i, max(rows - 1, 0)));
+        const int p0 = s.len[q] + (i - s.rows[q]);
+        if (i + ROWS <= end_of(q) && i < rows && (p0 & mask) + ROWS <= mask + 1) {
+            const int64_t page = page_of(q, p0);
 #pragma unroll
-        for (int e = 0; e < ROWS; e++) {
-            const int r = i + e;
-            if (r >= a.n_rows) break;
-            int position = -1;
-            int64_t slot = -1;
-            if (r < rows) {
-                if (r >= next) {
-                    do next = ++q + 1 < a.n_seq ? s.rows[q + 1] : rows;
-                    while (r >= next);
-                    len = a.len[q];
-                    column = -1;
-                }
-                position = len + (r - s.rows[q]);
-                const int c = position >> a.page_shift;
-                if (c != column) {
-                    column = c;
-                    const int fresh = c - pages_for(len, a.page_shift);
-                    page = fresh < 0 ? a.pages[(size_t)q * a.max_pages + c] : a.free_pages[n_free - 1 - s.pages[q] - fresh];
-                }
-                slot = (int64_t)page << a.page_shift | (position & mask);
-                if (page < 0 || page >= a.n_pages) slot = -1;
+            for (int e = 0; e < ROWS; e++) {
+                position[e] = p0 + e;
+                slot[e] = page < 0 ? page : page + ((p0 + e) & mask);
             }
-            if (a.position) a.position[r] = position;
-            if (a.slot) a.slot[r] = slot;
+        } else {
+#pragma unroll
+            for (int e = 0; e < ROWS; e++) {
+                position[e] = -1;
+                slot[e] = -1;
+                if (i + e < rows) {
+                    while (i + e >= end_of(q)) q++;
+                    position[e] = s.len[q] + (i + e - s.rows[q]);
+                    slot[e] = page_of(q, position[e]);
+                    if (slot[e] >= 0) slot[e] += position[e] & mask;
+                }
+            }
+        }
+        if (i + ROWS <= a.n_rows) {
+            if (a.position) *reinterpret_cast<i4 *>(a.position + i) = i4{position[0], position[1], position[2], position[3]};
+            if (a.slot) {
+                reinterpret_cast<l2 *>(a.slot + i)[0] = l2{slot[0], slot[1]};
+                reinterpret_cast<l2 *>(a.slot + i)[1] = l2{slot[2], slot[3]};
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < ROWS; e++) {
+                if (a.position && i + e < a.n_rows) a.position[i + e] = position[e];
+                if (a.slot && i + e < a.n_rows) a.slot[i + e] = slot[e];
+            }
         }
     }
     if (blockIdx.x == 0) {
         for (int q = threadIdx.x; q < a.n_seq; q += THREADS) a.row_start[q] = reason == DONE ? s.rows[q] : 0;
         if (threadIdx.x == 0) a.row_start[a.n_seq] = rows;
     }
-    if (!last_one(a)) return;
+    if (!last) return;
     if (reason == DONE)
-        for (int q = threadIdx.x; q < a.n_seq; q += THREADS) a.len[q] = a.len[q] + a.rows[q];
+        for (int q = threadIdx.x; q < a.n_seq; q += 64) a.len[q] = s.len[q] + (end_of(q) - s.rows[q]);
     if (threadIdx.x == 0) {
-        if (reason == DONE) *a.n_free = n_free - need;
+        if (reason == DONE) *a.n_free = t.n_free - need;
         report(a, reason);
     }
 }
 
 __global__ __launch_bounds__(THREADS) void release_kernel(Args a) {
     __shared__ Sums s;
-    int rows, back;
-    int reason = sum_up<false>(a, s, rows, back);
-    const int n_free = *a.n_free;
-    if (n_free < 0 || n_free > a.n_pages || back > a.n_pages - n_free) reason = BAD_TABLE;
-    if (reason != DONE) back = 0;
+    const Totals t = sum_up<false>(a, s);
+    const bool last = last_one(a);
+    int reason = t.bad;
+    if (t.n_free < 0 || t.n_free > a.n_pages || t.pages > a.n_pages - t.n_free) reason = BAD_TABLE;
+    const int back = reason == DONE ? t.pages : 0;
     // the reverse of the order in which a step gives pages
+    int32_t *top = a.free_pages + t.n_free + back - 1;
     for (int i = blockIdx.x * THREADS + threadIdx.x; i < back; i += gridDim.x * THREADS) {
         const int q = find(s.pages, a.n_seq, i);
-        int32_t *entry = &a.pages[(size_t)q * a.max_pages + pages_for(a.rows[q], a.page_shift) + (i - s.pages[q])];
-        a.free_pages[n_free + back - 1 - i] = *entry;
+        int32_t *entry = &a.pages[(size_t)q * a.max_pages + pages_for(s.len[q], a.page_shift) + (i - s.pages[q])];
+        top[-i] = *entry;
         *entry = -1;
     }
-    if (!last_one(a)) return;
+    if (!last) return;
     if (reason == DONE)
-        for (int q = threadIdx.x; q < a.n_seq; q += THREADS) {
-            const int keep = a.rows[q];
-            if (keep >= 0 && keep < a.len[q]) a.len[q] = keep;
-        }
+        for (int q = threadIdx.x; q < a.n_seq; q += 64)
+            if (s.len[q] >= 0) a.len[q] = min(s.len[q], a.len[q]);
     if (threadIdx.x == 0) {
-        if (reason == DONE) *a.n_free = n_free + back;
+        if (reason == DONE) *a.n_free = t.n_free + back;
         report(a, reason);
     }
 }
@@ -323,7 +357,7 @@ int kh_pages_release_dev(kh_ctx *ctx, const kh_page_table *t, const int32_t *kee
         std::lock_guard<std::recursive_mutex> lock(ctx->mu);
         (void)hipSetDevice(ctx->device);
         const size_t most = std::min(t->n_pages, t->n_seq * t->max_pages);
-        release_kernel<<<blocks_for(most / 16, (unsigned)ctx->cu_count), THREADS, 0, ctx->stream>>>(a);
+        release_kernel<<<blocks_for(most / 2, (unsigned)ctx->cu_count), THREADS, 0, ctx->stream>>>(a);
         KH_HIP(hipGetLastError());
         return KH_OK;
     });
