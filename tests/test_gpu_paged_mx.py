@@ -28,7 +28,7 @@ def mx(x):
     finite = np.isfinite(x).all(-1, keepdims=True)
     y = np.where(finite, x, 0).astype(np.float64)
     pad = -hd % 32
-    y = np.concatenate([y, np.zeros(y.shape[:-1] + (pad,))], -1).reshape(y.shape[:-1] + (-1, 32))
+    y = np.concatenate([y, np.zeros(y.shape[:-1] + (pad,))], -1).reshape(y.shape[:-1] + ((hd + pad) // 32, 32))
     amax = np.abs(y).max(-1, keepdims=True)
     e = np.full(amax.shape, -128)
     for k in range(-128, 128):
@@ -41,7 +41,7 @@ def mx(x):
         code += (t > m) if i % 2 == 0 else (t >= m)
     with np.errstate(over="ignore"):
         r = (np.sign(y) * VALUES[code] * np.exp2(e.astype(np.float64))).astype(np.float32)
-    r = r.reshape(r.shape[:-2] + (-1,))[..., :hd]
+    r = r.reshape(r.shape[:-2] + (hd + pad,))[..., :hd]
     return np.where(finite, r, np.float32(np.nan)).astype(np.float32)
 
 
