@@ -152,7 +152,7 @@ def run(g, d, eager, precision):
         for l in range(LAYERS):
             b = {k: v.cpu().numpy() for k, v in d.b[l].items()}
             want = turned(b["qkv"][:m, :(H + KV) * HD].reshape(m, H + KV, HD), d.cos[pos[:m]][:, None], d.sin[pos[:m]][:, None], False)
-            np.testing.assert_array_equal(b["qk"][:m], want.reshape(m, -1))
+            np.testing.assert_array_equal(b["qk"][:m], want.reshape(m, (H + KV) * HD))
             assert (b["qk"][m:] == 7).all() and (b["att"][m:] == 7).all()  # rows that no sequence has
             new_k, new_v = want[:, H:], b["qkv"][:m, (H + KV) * HD:].reshape(m, KV, HD)
             at = 0
