@@ -283,7 +283,7 @@ typedef struct kh_paged kh_paged;
  * refused; they never lead out of the cache or the rows: positions below zero
  * or past max_pages, and pages outside 0 .. n_pages - 1, are not written, are
  * seen by no row and read as zero.  A slot given to two rows of one push holds
- * either's elements, mixed.  max_len (0: what max_pages hold) is the longest
+ * either's elements, mixed (KH_MXFP4: the bits of their codes).  max_len (0: what max_pages hold) is the longest
  * len, for choosing how work is split alone: any value gives the same results
  * to rounding. */
 typedef struct kh_batch {

@@ -370,6 +370,10 @@ int kh_rope_rows_dev(kh_ctx *ctx, const float *cos_t, const float *sin_t, size_t
         const bool in_place = x == out && a.x_stride == a.out_stride;
         if (!in_place && overlap(x, (m - 1) * a.x_stride + width, out, (m - 1) * a.out_stride + width))
             return fail(KH_EINVAL, "kh_rope_rows_dev: out is x, or apart from it");
+        const size_t rows_out = (m - 1) * a.out_stride + width;
+        if (overlap(cos_t, max_pos * half, out, rows_out) || overlap(sin_t, max_pos * half, out, rows_out) ||
+            overlap(reinterpret_cast<const float *>(position), m, out, rows_out))
+            return fail(KH_EINVAL, "kh_rope_rows_dev: out is apart from the tables and positions");
         const int vec = half % 4 ? 1 : 4;
         const size_t items = m * n_vec * (half / vec);
         a.items = (unsigned)items;

@@ -266,8 +266,8 @@ __device__ __forceinline__ unsigned mx_codes(float4u x, int e) {
 }
 
 // As push_kernel.  A group's 32 dims are one step of the 8 lanes that have a row.
-// V's words of 8 positions that the run fills in part keep the rest of theirs: they
-// are loaded with the rows.
+// Words of V's codes, 8 positions each, that the run fills in part keep the rest of
+// theirs, whoever writes that at the same time: bits cleared and set by atomics.
 template <int D>
 __global__ __launch_bounds__(256) void push_mx_kernel(MoveArgs a) {
     constexpr int G = D / 32, ROW = D / 2 + 16, VROW = D + 4;
@@ -294,13 +294,6 @@ __global__ __launch_bounds__(256) void push_mx_kernel(MoveArgs a) {
     const int lo = max(t.first - t.p0, 0), hi = min(t.first + t.n - t.p0, TILE);  // the tile's new positions
     // word i of V's tile: [dim / 64][position / 8][dim % 16][dim / 16 % 4]
     unsigned *v_words = reinterpret_cast<unsigned *>(t.block + mx_v_off(D, a.page, in_page, 0));
-    unsigned old[D / 64], keep[D / 64];
-#pragma unroll
-    for (int j = 0; j < D / 64; j++) {
-        const int p = 8 * (threadIdx.x >> 6), from = max(lo - p, 0), to = min(hi - p, 8);
-        keep[j] = from < to ? ~(0xffffffffu >> (32 - 4 * (to - from)) << (4 * from)) : 0xffffffffu;
-        if (keep[j] && ~keep[j]) old[j] = v_words[threadIdx.x + 256 * j];
-    }
 #pragma unroll
     for (int what = 0; what < 2; what++) {
         int e[G], top = -128;
@@ -346,14 +339,22 @@ __global__ __launch_bounds__(256) void push_mx_kernel(MoveArgs a) {
             *reinterpret_cast<int4 *>(t.block + mx_k_off(a.page, in_page + pos, unit * 32)) =
                 *reinterpret_cast<const int4 *>(s_k + pos * ROW + unit * 16);
     }
+    const int from = max(lo - 8 * (int)(threadIdx.x >> 6), 0), to = min(hi - 8 * (int)(threadIdx.x >> 6), 8);
+    if (from >= to) return;
+    const unsigned keep = ~(0xffffffffu >> (32 - 4 * (to - from)) << (4 * from));
 #pragma unroll
     for (int j = 0; j < D / 64; j++) {
-        if (!~keep[j]) continue;
         const int i = threadIdx.x, dim = 64 * j + (i >> 2 & 15) + 16 * (i & 3), p = 8 * (i >> 6);
         unsigned w = 0;
 #pragma unroll
         for (int k = 0; k < 8; k++) w |= (unsigned)s_v[(p + k) * VROW + dim] << (4 * k);
-        v_words[i + 256 * j] = keep[j] ? (w & ~keep[j]) | (old[j] & keep[j]) : w;
+        unsigned *word = v_words + i + 256 * j;
+        if (!keep) {
+            *word = w;
+        } else {
+            atomicAnd(word, keep);
+            atomicOr(word, w & ~keep);
+        }
     }
 }
 

@@ -59,9 +59,12 @@ def test_a_tables_batch():
     assert (b.n_seq, b.n_rows, b.len, b.pages, b.row_start, b.max_pages, b.max_len) == (4, 7, AT + 4, AT + 8, AT + 12, 8, 100)
 
 
+FAR = AT + (1 << 20)
+
+
 def rope(**kw):
-    a = dict(cos=AT, sin=AT, half=32, max_pos=10, x=AT, position=AT, m=2, n_vec=1, out=AT, interleaved=False, x_stride=0,
-             out_stride=0)
+    a = dict(cos=2 * FAR, sin=3 * FAR, half=32, max_pos=10, x=AT, position=4 * FAR, m=2, n_vec=1, out=AT, interleaved=False,
+             x_stride=0, out_stride=0)
     a.update(kw)
     K.rope_rows_dev(NoDevice, a["cos"], a["sin"], a["half"], a["max_pos"], a["x"], a["position"], a["m"], a["n_vec"], a["out"],
                     a["interleaved"], a["x_stride"], a["out_stride"])
@@ -73,7 +76,8 @@ def rope(**kw):
     ({"m": (1 << 30) + 1}, "2\\^30"), ({"max_pos": (1 << 30) + 1}, "2\\^30"), ({"half": 1 << 20, "n_vec": 1 << 10}, "2\\^30"),
     ({"x_stride": 63}, "less than a row"), ({"out_stride": 63}, "less than a row"), ({"x_stride": 1 << 62}, "too large"),
     ({"out": AT + 4}, "apart"), ({"out": AT + 16 * 4, "m": 2}, "apart"), ({"x_stride": 128}, "apart"),
-    ({"m": 1 << 30, "n_vec": 4, "out": AT + (1 << 42)}, "too many rows")])
+    ({"cos": AT}, "tables"), ({"sin": AT + 508}, "tables"), ({"position": AT - 4}, "positions"),
+    ({"m": 1 << 30, "n_vec": 4, "out": 1 << 60}, "too many rows")])
 def test_rotations_that_are_refused(kw, word):
     with pytest.raises(K.KvadError, match=word):
         rope(**kw)
@@ -87,9 +91,6 @@ def test_empty_calls_do_nothing():
     norm(n=0)
     assert LIB.kh_rope_rows_dev(None, AT, AT, 1, 1, AT, 0, AT, 0, 1, 0, AT, 0) == -1
     assert LIB.kh_norm_residual_dev(None, AT, AT, None, None, 0, 1.0, None, 0, 1, 0.0, AT, None) == -1
-
-
-FAR = AT + (1 << 20)
 
 
 def norm(**kw):
