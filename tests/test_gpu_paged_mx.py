@@ -108,6 +108,24 @@ def test_single_positions_fill_words_of_eight(ctx, hd):
         np.testing.assert_array_equal(got, mx(np.concatenate(x)))
 
 
+@pytest.mark.parametrize("precision", [MX, "i8"])
+def test_one_page_by_several_runs_of_a_push(ctx, precision):
+    # a sequence's rows given as runs that end and start within words of eight
+    import torch
+
+    p = Pool(ctx, np.random.default_rng(21), precision, 2, 128, 64, [64])
+    k, v = p.rows(61), p.rows(61)
+    ends = [3, 4, 5, 13, 24, 27, 40, 41, 61]
+    b = device_batch(ends, np.repeat(p.pages, len(ends), 0), rows=list(np.diff([0] + ends)))
+    dk, dv = torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda()
+    torch.cuda.synchronize()
+    p.cache.push_dev(0, b, dk.data_ptr(), dv.data_ptr())
+    ctx.synchronize()
+    got = p.cache.read(0, p.batch([61], [61]))
+    np.testing.assert_array_equal(got[0], T.rounded(precision, k))
+    np.testing.assert_array_equal(got[1], T.rounded(precision, v))
+
+
 def test_bytes_of_a_cache(ctx):
     for hd, d in ((64, 64), (80, 128), (128, 128), (256, 256)):
         cache = K.PagedCache(ctx, 3, 2, hd, 5, page_size=64, precision=K.MXFP4)
