@@ -1180,15 +1180,41 @@ int launch_d(int d, const Args &a, const AttnPlan &p, unsigned blocks, size_t it
 }
 
 size_t up_to(size_t n, size_t m) { return (n + m - 1) / m; }
+// Waves that join a row's splits (merge_kernel): they take 16 each, one alone 8, a
+// trip to memory.
+int join_waves(size_t splits, size_t items, size_t cus) { return splits > 8 && items <= cus ? 4 : 1; }
 
 // Splits of few_rows, bound by memory: a workgroup for each CU.  Each gets as
 // many tiles as take as long as joining the splits does (a launch, 4 us): 16, or
 // fewer large ones; and where all splits together save a wave less turns than
 // that, there are none.
 size_t few_splits(const kh_paged *kv, size_t blocks, size_t pos_tiles, size_t cus) {
-    const size_t least = std::min(std::max(4096 / ((kv->es == MX ? 1 : 2 * kv->es) * kv->d), 4), 16);
+    const size_t least = std::min(std::max(2048 / (kv->es * kv->d), 4), 16);
     const size_t splits = std::min(up_to(cus, blocks), up_to(pos_tiles, least));
     return up_to(pos_tiles, 4) < up_to(up_to(pos_tiles, splits), 4) + least / 4 ? 1 : splits;
+}
+// The same of 4-bit rows, whose tiles are so small that a CU takes more than one
+// workgroup's at a time with a gain: the splits whose busiest CU ends first.  A turn
+// of the four waves takes 0.85 us (128 dims), of two workgroups on a CU 1.45, of four
+// 2.65; the join as many_splits counts it, and 1.2 for each trip to memory after its
+// first (14 heads of 64, 32768 positions: 64 splits 10.6 us, 128 11.1).  Up to a workgroup a CU without splits:
+// beyond, the CUs are filled by others' sequences.  Of 32 heads on 8 of 128, up to
+// 4000 positions: 5 sequences 13.6 us against 15.7 with few_splits' rule, 12 16.8
+// against 22.1, 20 22.2 against 27.5.
+size_t mx_few_splits(const kh_paged *kv, size_t blocks, size_t pos_tiles, size_t cus, size_t items) {
+    if (blocks > cus) return 1;
+    const double dims = (kv->d + 32) / 160.0, join = 8e-6 / 2.4 * (double)items * (kv->d + 2);
+    size_t splits = 1;
+    double least = 0.0;
+    for (size_t s = 1; s <= std::min(4 * cus / blocks, up_to(pos_tiles, 4)); s++) {
+        const double each = 0.25 + 0.6 * (double)up_to(blocks * s, cus);
+        const double trips = (double)up_to(s, join_waves(s, items, cus) > 1 ? 64 : 8);
+        const double us = (double)up_to(up_to(pos_tiles, s), 4) * each * dims + (s > 1 ? 1.3 + 1.2 * trips + join * (double)s : 0.0);
+        if (s > 1 && us >= least) continue;
+        splits = s;
+        least = us;
+    }
+    return splits;
 }
 // Splits of many_rows, bound by arithmetic: those whose slowest CU ends first.
 // A wave's turn takes 1 us (128 dims, f16 or i8; f32 2), those of two workgroups
@@ -1258,6 +1284,7 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
         const int forced = env_int("KVAD_PAGED_SPLITS", 0);
         size_t splits = 1;
         if (forced > 0) splits = std::min((size_t)forced, pos_tiles);
+        else if (p.tile_rows <= 16 && kv->es == MX) splits = mx_few_splits(kv, blocks, pos_tiles, cus, (size_t)b.n_rows * n_head);
         else if (p.tile_rows <= 16) splits = few_splits(kv, blocks, pos_tiles, cus);
         else splits = many_splits(kv, blocks, pos_tiles, cus, resident, (size_t)b.n_rows * n_head);
         splits = std::min(splits, (size_t)1024);
@@ -1272,7 +1299,7 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
             if (p.tile_rows <= 16) p.split_tiles = 4 * (int)up_to(p.split_tiles, 4);
             p.splits = (int)up_to(pos_tiles, p.split_tiles);
             p.ws_bytes = p.splits > 1 ? each * p.splits : 0;
-            p.join_waves = p.splits > 8 && (size_t)b.n_rows * n_head <= cus ? 4 : 1;
+            p.join_waves = join_waves(p.splits, (size_t)b.n_rows * n_head, cus);
         }
     }
     const size_t all = blocks * p.splits;
