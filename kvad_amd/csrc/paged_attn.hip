@@ -7,10 +7,12 @@
 // is cut into two f16 pieces, hi + lo, 22 bits of significand: enough that the
 // result is as near the 64-bit one as f32 arithmetic is (the operands of a row
 // share a power-of-two scale, so f16's exponents are wide enough).  Cache rows
-// of f16, and i8 codes, are one exact f16 each: two products a tile, q's or the
-// weights' pieces against them; f32 rows are two pieces and three products (lo
-// by lo is below the 22 bits).  The f32 matrix cores run at a sixteenth of the
-// f16 rate.
+// of f16, i8 codes, and 4-bit codes times their factor, are one exact f16 each:
+// two products a tile, q's or the weights' pieces against them; f32 rows are two
+// pieces and three products (lo by lo is below the 22 bits).  The f32 matrix cores
+// run at a sixteenth of the f16 rate.  Two 4-bit codes become f16, times a factor
+// (K's: a lane's unit has one), in one instruction; V's factors, one a position,
+// are a product more.  The row's scale is a score's or a weight's, as the others'.
 //
 // A wave takes rows of one KV head (query tokens x the head's group, flattened:
 // each K and V byte is read once for the whole group) and 32 positions at a
@@ -27,13 +29,15 @@
 // both, and their sums meet in the scores (by a lane move) and at the end.
 //
 // What bounds them.  few_rows: HBM (64 sequences of up to 4000 i8 positions, 8
-// heads of 128: 74 us for 362 MB, 4.9 TB/s, a large copy's rate), or for one
+// heads of 128: 70 us for 362 MB, 5.1 TB/s, a large copy's rate; in 4 bits 44 us
+// for 203 MB, 4.6 TB/s: of 32 long ones, a workgroup a CU, 5.6), or for one
 // short sequence the trips to memory and the joining launch.  many_rows: the
 // matrix cores, 47% at work, behind 6 vector instructions a product (a wave
 // issues one in 8 cycles, so two waves a SIMD, all that 256 registers allow,
 // just fill it): 512 tokens behind 8000, f16, 32 heads of 128: 141 us, 490
 // TFLOP/s of the scores and values or 980 of the products run for them, where a
-// large bf16 product of the library reaches 1200.
+// large bf16 product of the library reaches 1200; in 4 bits 132 to 139 us, 262
+// vector instructions and 32 products a tile, 112 of them for the codes.
 #include <algorithm>
 #include <utility>
 
@@ -1199,8 +1203,8 @@ size_t few_splits(const kh_paged *kv, size_t blocks, size_t pos_tiles, size_t cu
 // 2.65; the join as many_splits counts it, and 1.2 for each trip to memory after its
 // first (14 heads of 64, 32768 positions: 64 splits 10.6 us, 128 11.1).  Up to a workgroup a CU without splits:
 // beyond, the CUs are filled by others' sequences.  Of 32 heads on 8 of 128, up to
-// 4000 positions: 5 sequences 13.6 us against 15.7 with few_splits' rule, 12 16.8
-// against 22.1, 20 22.2 against 27.5.
+// 4000 positions: 5 sequences 14.0 us against 15.7 with few_splits' rule, 12 17.0
+// against 22.1, 20 22.4 against 27.5.
 size_t mx_few_splits(const kh_paged *kv, size_t blocks, size_t pos_tiles, size_t cus, size_t items) {
     if (blocks > cus) return 1;
     const double dims = (kv->d + 32) / 160.0, join = 8e-6 / 2.4 * (double)items * (kv->d + 2);
