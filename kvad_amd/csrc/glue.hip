@@ -116,7 +116,7 @@ typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));  // rows 
 // Rows at positions of their own: row r of x holds n_vec vectors of 2 * half
 // first, at position[r]; a row whose position is outside of the tables is left
 // alone.  VEC pairs a thread, one trip to memory for the position and one for
-// the rest; bound by HBM (5600 rows of 40 heads of 128: 42.6 us for 219 MB, 5.1
+// the rest; bound by HBM (5300 rows of 40 heads of 128: 42.6 us for 219 MB, 5.1
 // TB/s), or by the launch for a few rows (48 of 16 heads of 64: 2.5 us).
 struct RopeRows {
     const float *cos_t, *sin_t, *x;
