@@ -253,7 +253,7 @@ __global__ __launch_bounds__(256) void read_kernel(MoveArgs a) {
 // The exponent of a group's step from the bits of its largest magnitude: amax is
 // 3.5 to 7 steps, so that the largest is cut by 1 of 7 at the most.  Not under
 // -128, amax's under 7 2^-128 being subnormal or nearly so.
-__device__ __forceinline__ int mx_exp(int amax_bits) { return max(((amax_bits + 0x200000) >> 23) - 129, -128); }
+__device__ __forceinline__ int mx_exp(int amax_bits) { return max((int)(((unsigned)amax_bits + 0x200000u) >> 23) - 129, -128); }
 // The exponent of a row's scale from the largest of its groups' exponents: the
 // factors, 2^12 down to f16's least normal 2^-14, keep the codes times them under 2^15.
 __device__ __forceinline__ int mx_row_exp(int top) { return max(top - 12, -126); }

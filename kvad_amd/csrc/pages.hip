@@ -250,7 +250,7 @@ __global__ __launch_bounds__(THREADS) void release_kernel(Args a) {
     const Totals t = sum_up<false>(a, s);
     const bool last = last_one(a);
     int reason = t.bad;
-    if (t.n_free < 0 || t.n_free > a.n_pages || t.pages > a.n_pages - t.n_free) reason = BAD_TABLE;
+    if (t.n_free < 0 || t.n_free > a.n_pages || t.pages > a.n_pages - t.n_free || t.pages >= LIMIT) reason = BAD_TABLE;
     const int back = reason == DONE ? t.pages : 0;
     // the reverse of the order in which a step gives pages
     int32_t *top = a.free_pages + t.n_free + back - 1;

@@ -330,6 +330,13 @@ def test_block_ends(dctx, n, post, gate, pre):
     np.testing.assert_array_equal(dx.cpu().numpy().reshape(m, n), got_x)
     if pre:
         np.testing.assert_array_equal(dy.cpu().numpy().reshape(m, n), got)
+    # and the other way round
+    dx.copy_(dev(x).flatten())
+    dy.copy_(dev(y).flatten())
+    call(dy, dx)
+    np.testing.assert_array_equal(dy.cpu().numpy().reshape(m, n), got_x)
+    if pre:
+        np.testing.assert_array_equal(dx.cpu().numpy().reshape(m, n), got)
 
 
 def test_block_ends_of_rows_that_are_not_finite_leave_the_others(dctx):
