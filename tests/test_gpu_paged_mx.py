@@ -266,6 +266,20 @@ def test_the_longest_sequences_go_first(ctx, precision, n_seq, kv, ragged):
     p2.check([1] * n_seq, kv, q=q, got=p2.cache.attend(0, K.Batch.host(same, p2.pages, None, n_rows=n_seq), kv, q))
 
 
+@pytest.mark.parametrize("splits", ["", "3"])
+@pytest.mark.parametrize("H, kv, hd, counts, lens", [
+    (8, 2, 128, [1] * 9, [1, 40, 700, 33, 64, 5, 900, 2, 31]), (8, 2, 64, [0, 4, 0, 0, 1, 0, 0, 3], [9, 70, 0, 30, 300, 32, 1, 500]),
+    (40, 2, 64, [0, 0, 3, 0], [5, 3, 130, 60]), (24, 1, 256, [1, 0, 2], [90, 7, 64]), (4, 4, 128, [0] * 70 + [40, 9], [20] * 70 + [300, 9])])
+def test_ragged_batches_of_few_rows(ctx, monkeypatch, H, kv, hd, counts, lens, splits):
+    # no more rows than sequences, of a row each or of some with many
+    monkeypatch.setenv("KVAD_PAGED_SPLITS", splits)
+    p = Pool(ctx, np.random.default_rng(hd + H), MX, kv, hd, 32, lens)
+    p.push([n - c for n, c in zip(lens, counts)])
+    p.push(counts)
+    p.check(counts, H)
+    p.check(counts, H, window=50, sinks=2)
+
+
 @pytest.mark.parametrize("size", [-80, -95, -105, -112, -120, 93])
 def test_values_of_one_size(ctx, form, size):  # noqa: F811
     T.test_values_of_one_size(ctx, form, MX, size)
