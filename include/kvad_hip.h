@@ -362,7 +362,7 @@ typedef struct kh_page_table {
     int32_t *free_pages; /* [n_pages]: a stack, its top at n_free[0] - 1 */
     int32_t *n_free;     /* [1] */
     int32_t *status;     /* [4]: why the last call was refused (0: it was not),
-                            how many have been, and two of the library's own */
+                            how many have been, and two that calls leave alone */
 } kh_page_table;
 /* What a refused call leaves in status[0]. */
 #define KH_PAGES_SHORT 1     /* fewer free pages than the step needs */

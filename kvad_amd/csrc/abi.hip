@@ -200,6 +200,7 @@ int kh_free(kh_ctx *ctx) {
         if (ctx->io.ptr) (void)hipFree(ctx->io.ptr);
         if (ctx->moe.ptr) (void)hipFree(ctx->moe.ptr);
         if (ctx->gemm.ptr) (void)hipFree(ctx->gemm.ptr);
+        free_counter(ctx);
         if (ctx->own) (void)hipStreamDestroy(ctx->own);
     }
     delete ctx;

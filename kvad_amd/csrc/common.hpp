@@ -88,6 +88,7 @@ struct kh_ctx {
     kh::Workspace io;        // staging for host-pointer calls
     kh::Workspace moe;       // mixture-of-experts intermediates
     kh::Workspace gemm;      // split-K partials
+    int pages_counter = -1;  // of page table calls outside of graphs (pages.hip)
 };
 
 struct kh_weight {
@@ -379,6 +380,9 @@ void gemm_split_reserve(kh_ctx *ctx);
 // The split-K workspace for `bytes` of partials, or null where it does not
 // hold them (or was not allocated before a capture).
 float *split_partials(kh_ctx *ctx, size_t bytes);
+
+// The counter of a context's page table calls given back (pages.hip), its work done.
+void free_counter(kh_ctx *ctx);
 // y[M][N] (+)= the ks planes of part added in order (+ bias).
 int launch_split_reduce(kh_ctx *ctx, const float *part, int ks, int M, int N, const float *bias, int accumulate,
                         float *y);

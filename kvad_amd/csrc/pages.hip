@@ -28,7 +28,7 @@ typedef long l2 __attribute__((ext_vector_type(2), aligned(8)));
 constexpr int LIMIT = 1 << 30;                          // positions and rows are below it
 
 // kh_page_table's status
-enum { REASON, REFUSED, ARRIVED = 3 };
+enum { REASON, REFUSED };
 enum { DONE, SHORT, TOO_LONG, BAD_ROWS, BAD_TABLE };
 
 struct Args {
@@ -37,7 +37,15 @@ struct Args {
     int32_t *position;
     int64_t *slot;
     int n_seq, max_pages, page_shift, n_pages, n_rows;
+    int counter;  // of arrived, where there are several workgroups
 };
+
+// Workgroups of a launch that have read what its last one writes: a counter for each
+// launch that may run beside others, zero between them.  The library's own, zero from
+// the start whatever the caller's arrays hold, and never freed: a captured graph may
+// outlive its context.
+constexpr int COUNTERS = 1 << 14;
+__device__ int arrived[COUNTERS];
 
 __device__ __forceinline__ int pages_for(int positions, int shift) { return (int)(((unsigned)positions + (1u << shift) - 1) >> shift); }
 // a sum that stops at LIMIT: of operands up to LIMIT, whatever their order
@@ -159,8 +167,8 @@ __device__ __forceinline__ bool last_one(const Args &a) {
     if (gridDim.x == 1) return true;
     int last = 0;
     if (threadIdx.x == 0) {
-        last = __hip_atomic_fetch_add(&a.status[ARRIVED], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
-        if (last) a.status[ARRIVED] = 0;
+        last = __hip_atomic_fetch_add(&arrived[a.counter], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+        if (last) arrived[a.counter] = 0;
     }
     return __builtin_amdgcn_readfirstlane(last) != 0;
 }
@@ -300,15 +308,45 @@ int check(kh_ctx *ctx, const kh_page_table *t, Args &a, const char *what) {
     int shift = 0;
     while (((size_t)1 << shift) < t->page_size) shift++;
     a = Args{t->len, t->pages, t->row_start, t->free_pages, t->n_free, t->status, nullptr, nullptr, nullptr,
-             (int)t->n_seq, (int)t->max_pages, shift, (int)t->n_pages, 0};
+             (int)t->n_seq, (int)t->max_pages, shift, (int)t->n_pages, 0, 0};
     return KH_OK;
 }
 unsigned blocks_for(size_t items, unsigned most) {
     return (unsigned)std::min<size_t>(std::max<size_t>((items + THREADS - 1) / THREADS, 1), most);
 }
 
+// Which of the counters are taken: up to `used`, but for those given back.
+std::mutex counters_mu;
+int counters_used = 0, counters_back[COUNTERS], n_back = 0;
+int take_counter() {
+    std::lock_guard<std::mutex> lock(counters_mu);
+    if (n_back) return counters_back[--n_back];
+    return counters_used < COUNTERS ? counters_used++ : -1;
+}
+// The launch's counter, if it needs one: the context's, whose work is on one stream, or
+// of a captured call, which may be replayed on any, its own for good.  With none left
+// one workgroup does it all.
+unsigned count_with(kh_ctx *ctx, unsigned blocks, Args &a) {
+    if (blocks == 1) return 1;
+    if (capturing(ctx->stream)) {
+        a.counter = take_counter();
+    } else {
+        if (ctx->pages_counter < 0) ctx->pages_counter = take_counter();
+        a.counter = ctx->pages_counter;
+    }
+    return a.counter < 0 ? 1 : blocks;
+}
+
 }  // namespace
 }  // namespace pages
+
+void free_counter(kh_ctx *ctx) {
+    if (ctx->pages_counter < 0) return;
+    std::lock_guard<std::mutex> lock(pages::counters_mu);
+    pages::counters_back[pages::n_back++] = ctx->pages_counter;
+    ctx->pages_counter = -1;
+}
+
 }  // namespace kh
 
 using namespace kh;
@@ -343,7 +381,7 @@ int kh_pages_step_dev(kh_ctx *ctx, const kh_page_table *t, const int32_t *rows, 
         a.slot = slot;
         std::lock_guard<std::recursive_mutex> lock(ctx->mu);
         (void)hipSetDevice(ctx->device);
-        const unsigned blocks = blocks_for(n_rows / ROWS, 2 * (unsigned)ctx->cu_count);
+        const unsigned blocks = count_with(ctx, blocks_for(n_rows / ROWS, 2 * (unsigned)ctx->cu_count), a);
         step_kernel<<<blocks, THREADS, 0, ctx->stream>>>(a);
         KH_HIP(hipGetLastError());
         return KH_OK;
@@ -360,7 +398,8 @@ int kh_pages_release_dev(kh_ctx *ctx, const kh_page_table *t, const int32_t *kee
         std::lock_guard<std::recursive_mutex> lock(ctx->mu);
         (void)hipSetDevice(ctx->device);
         const size_t most = std::min(t->n_pages, t->n_seq * t->max_pages);
-        release_kernel<<<blocks_for(most / 2, (unsigned)ctx->cu_count), THREADS, 0, ctx->stream>>>(a);
+        const unsigned blocks = count_with(ctx, blocks_for(most / 2, (unsigned)ctx->cu_count), a);
+        release_kernel<<<blocks, THREADS, 0, ctx->stream>>>(a);
         KH_HIP(hipGetLastError());
         return KH_OK;
     });

@@ -209,6 +209,83 @@ def test_a_captured_step_takes_each_replays_rows(dctx):
         assert pos.cpu().tolist() == t.position and slot.cpu().tolist() == t.slot
 
 
+@pytest.mark.parametrize("held", [77, -1, 2 ** 31 - 1])
+def test_a_status_that_was_never_cleared(dctx, held):
+    # a table that the caller filled, as init does but for the status: steps and
+    # releases of one workgroup and of several advance it all the same
+    t = Tables(dctx, 64, 40, 32, 1500)
+    rng = np.random.default_rng(2)
+    for n_rows, most in ((4000, 60), (900, 13), (2500, 39), (4000, 60)):
+        t.dev["status"].fill_(held)
+        rows = [int(r) for r in rng.integers(0, most, 64)]
+        r, pos = dev(np.array(rows, np.int32)), torch.zeros(n_rows, dtype=torch.int32, device="cuda")
+        t.t.step_dev(dctx, r.data_ptr(), n_rows, pos.data_ptr())
+        t.expect(rows, n_rows)
+        assert t.dev["status"].tolist() == [0, held, held, held] and pos.cpu().tolist() == t.position
+        t.dev["status"].zero_()
+        t.check()
+        t.dev["status"].fill_(held)
+        keep = [n // 2 if s % 3 else -1 for s, n in enumerate(t.len)]
+        k = dev(np.array(keep, np.int32))
+        t.t.release_dev(dctx, k.data_ptr())
+        assert t.dev["status"].tolist() == [0, held, held, held]
+        t.dev["status"].zero_()
+        for s in reversed(range(64)):
+            if 0 <= keep[s] < t.len[s]:
+                for j in reversed(range(t.pages_of(keep[s]), t.pages_of(t.len[s]))):
+                    t.free.append(t.pages[s][j])
+                    t.pages[s][j] = -1
+                t.len[s] = keep[s]
+        t.check()
+
+
+def test_tables_stepped_beside_each_other():
+    # two tables' captured steps of several workgroups, replayed on two streams at
+    # once, and a third table's calls on another context meanwhile
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    ctxs = [K.Context(0) for _ in range(2)]
+    n_rows, keep = 6000, torch.full((64,), -1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    try:
+        tables, rows, graphs = [], [], []
+        for i, s in enumerate(streams):
+            c = ctxs[i // 2]
+            c.set_stream(s.cuda_stream)
+            with torch.cuda.stream(s):
+                tables.append(Tables(c, 64, 100, 32, 4000 + i))
+                rows.append(torch.zeros(64, dtype=torch.int32, device="cuda"))
+            torch.cuda.synchronize()
+            if i < 2:  # both of one context's
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=s):
+                    tables[i].t.release_dev(c, keep.data_ptr())
+                    tables[i].t.step_dev(c, rows[i].data_ptr(), n_rows)
+                graphs.append(g)
+        rng = np.random.default_rng(3)
+        for _ in range(8):
+            new = [[int(r) for r in rng.integers(0, 90, 64)] for _ in streams]
+            for r, n in zip(rows, new):
+                r.copy_(torch.tensor(n))
+            torch.cuda.synchronize()
+            for _ in range(3):
+                for g, s in zip(graphs, streams):
+                    with torch.cuda.stream(s):
+                        g.replay()
+                tables[2].t.release_dev(ctxs[1], keep.data_ptr())
+                tables[2].t.step_dev(ctxs[1], rows[2].data_ptr(), n_rows)
+            torch.cuda.synchronize()
+            for t, n in zip(tables, new):
+                for _ in range(3):
+                    t.expect(n, n_rows)
+                t.check()
+        del g, graphs
+    finally:
+        torch.cuda.synchronize()
+        for c in ctxs:
+            c.set_stream(None)
+            c.close()
+
+
 # ---- rotation --------------------------------------------------------------------
 
 def turned(x, c, s, interleaved):
