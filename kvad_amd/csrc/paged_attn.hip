@@ -1013,35 +1013,46 @@ constexpr int waves_for(int es, int d, int rows, bool ahead = false) {
     return regs <= 128 ? 4 : regs <= 172 ? 3 : regs <= 250 ? 2 : 1;
 }
 
-// find_seq of up to 64 sequences, the longest of them first: where there are more
-// workgroups than CUs, the last to start, or to have a CU's memory to themselves,
-// are then short ones (64 sequences of 1333 to 4000, 8 KV heads of 128: 4-bit rows
-// 47 us against 44, i8 73.8 against 70.3).  Each lane adds up the tiles of
-// those before its own.  False too for sequences of about one length, which stay as
-// they come: sorting takes 0.5 us.
+// find_seq of up to 64 sequences, those whose rows see the most positions first: where
+// there are more workgroups than CUs, the last to start, or to have a CU's memory to
+// themselves, are then short ones (64 sequences of 1333 to 4000, 8 KV heads of 128:
+// 4-bit rows 47 us against 44, i8 73.4 against 68.7).  Each lane adds up the tiles of
+// those before its own.  Sequences that see about as many stay as they come, as a
+// window makes them, and so does a prompt's chunk before others' single rows, whose
+// tiles take longer (3 chunks and 40 single rows, window 512, i8: 30.2 us, and sorted
+// by length 36.4).  Prompts beside single rows come out alike in any order they are
+// given in (900 rows and 40 sequences of 500 to 4000, i8: 66.7 us; as they come 84.4
+// with the prompt first and 60.4 with it last; f32 181 and 178, as they come 260 and 216).
 template <typename F>
-__device__ __forceinline__ bool find_longest_first(const Batch &b, int tile, F count, int &seq, Seq &s, int &local, int &n) {
+__device__ __forceinline__ bool find_longest_first(const Args &a, int tile, F count, int &seq, Seq &s, int &local, int &n) {
     const int lane = threadIdx.x & 63;
-    const bool has = lane < b.n_seq;
     Seq mine{0, 0, 0};
-    if (has) mine.load(b, lane);
-    const int len0 = __builtin_amdgcn_readfirstlane(mine.len), tiles = has ? count(mine) : 0;
-    if (!__ballot(has && abs(mine.len - len0) > len0 / 8)) return false;
-    const int key = min(mine.len, 1 << 24) << 6 | (63 - lane);  // all different, those of lanes that have none last
+    if (lane < a.b.n_seq) mine.load(a.b, lane);
+    const int tiles = count(mine);
+    int seen = min(mine.len, a.window);
+    seen += min(mine.len - seen, a.sinks);
+    const unsigned long long some = __ballot(tiles > 0);
+    const int seen0 = __builtin_amdgcn_readlane(seen, some ? __builtin_ctzll(some) : 0);
     int first = 0;
-    if (b.row_start) {
-#pragma unroll
-        for (int j = 0; j < 64; j++)
-            first += __builtin_amdgcn_readlane(key, j) > key ? __builtin_amdgcn_readlane(tiles, j) : 0;
+    if (!__ballot(tiles > 0 && abs(seen - seen0) > seen0 / 8)) {
+        first = dev::wave_scan(tiles) - tiles;
     } else {
+        const int key = min(seen, 1 << 24) << 6 | (63 - lane);  // all different, those of lanes that have none last
+        if (a.b.row_start) {
 #pragma unroll
-        for (int j = 0; j < 64; j++) first += __builtin_amdgcn_readlane(key, j) > key;
-        first *= tiles;
+            for (int j = 0; j < 64; j++)
+                first += __builtin_amdgcn_readlane(key, j) > key ? __builtin_amdgcn_readlane(tiles, j) : 0;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 64; j++) first += __builtin_amdgcn_readlane(key, j) > key;
+            first *= tiles;
+        }
     }
     const unsigned long long here = __ballot(tile >= first && tile - first < tiles);
-    seq = here ? __builtin_ctzll(here) : 0;
+    if (!here) return false;  // past the last tile
+    seq = __builtin_ctzll(here);
     n = __builtin_amdgcn_readlane(tiles, seq);
-    local = here ? tile - __builtin_amdgcn_readlane(first, seq) : n;  // past the last tile: no rows
+    local = tile - __builtin_amdgcn_readlane(first, seq);
     s = mine.of_lane(seq);
     return true;
 }
@@ -1067,8 +1078,8 @@ void attn_kernel(Args a) {
     Seq seq;
     int local, tiles;
     auto count = [&](const Seq &q) { return (q.n * a.group + ROWS - 1) / ROWS; };
-    if (a.longest_first && find_longest_first(a.b, tile, count, w.seq, seq, local, tiles)) {
-        if (local >= tiles) return;
+    if (a.longest_first) {
+        if (!find_longest_first(a, tile, count, w.seq, seq, local, tiles)) return;
     } else if (a.b.row_start) {
         if (!find_seq(a.b, tile, count, w.seq, seq, local, tiles)) return;
     } else {
@@ -1315,7 +1326,11 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
     p.ahead = kv->es == MX && p.tile_rows <= 16 && all <= cus;
     const int ahead = env_int("KVAD_PAGED_AHEAD", -1);  // for experiments, and for tests of both
     if (ahead >= 0) p.ahead = ahead && kv->es == MX && p.tile_rows <= 16;
-    p.longest_first = p.splits == 1 && b.n_seq > 1 && b.n_seq <= 64 && all > cus;
+    // Not through a window that is short beside the longest: it makes most sequences
+    // alike, and finding that out is 0.2 to 0.6 us (64 of 3000 to 12000, 8 KV heads of
+    // 128, window 256, i8: 12.0 against 11.7).
+    const bool alike = window != INT32_MAX && (size_t)window < max_len / 4;
+    p.longest_first = p.splits == 1 && b.n_seq > 1 && b.n_seq <= 64 && all > cus && !alike;
     return p;
 }
 

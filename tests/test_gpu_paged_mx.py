@@ -372,3 +372,25 @@ def test_lengths_and_pages_that_lead_nowhere(ctx, form):  # noqa: F811
         assert not k.any() and not v.any() and bool(torch.isfinite(out).all()) and not out[6:].any()
         for a, c in zip(before, p.cache.read(0, p.batch([96, 64]))):
             np.testing.assert_array_equal(a, c)
+
+
+@pytest.mark.parametrize("precision", [MX, "i8", "f16", "f32"])
+@pytest.mark.parametrize("chunk", [1, 3, 45])
+@pytest.mark.parametrize("window, sinks", [(30, 0), (40, 3), (100, 1), (10, 150), (149, 0), (1 << 30, 1)])
+def test_sequences_by_what_their_rows_see(ctx, precision, chunk, window, sinks):
+    # more workgroups than CUs, windows that make all sequences alike, some or none,
+    # in front of them a chunk behind little, sequences without rows among them
+    rng = np.random.default_rng(chunk + window % 1000)
+    lens = [chunk + 4] + [int(n) for n in rng.integers(1, 150, 63)]
+    counts = [chunk] + [int(n > 9) for n in lens[1:]]
+    counts[5] = lens[7] = counts[7] = 0
+    p = Pool(ctx, rng, precision, 8, 64, 32, lens)
+    p.push([n - c for n, c in zip(lens, counts)])
+    p.push(counts)
+    p.check(counts, 16, window=window, sinks=sinks)
+    ones = [1] * 40
+    p2 = Pool(ctx, rng, precision, 8, 64, 32, [max(n, 1) for n in lens[:40]])
+    p2.push([max(n, 1) for n in lens[:40]])
+    q = (rng.standard_normal((40, 16, 64)) * 1.5).astype(np.float32)
+    b = K.Batch.host([len(k) for k in p2.k], p2.pages, None, n_rows=40)
+    p2.check(ones, 16, window=window, sinks=sinks, q=q, got=p2.cache.attend(0, b, 16, q, window=window, sinks=sinks))
