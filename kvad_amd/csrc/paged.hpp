@@ -107,7 +107,7 @@ struct AttnPlan {
     int split_tiles;   // 32-position tiles a split
     int join_waves;    // that join a row's splits
     bool ahead;        // of 4-bit rows: few_rows with two tiles' registers
-    bool longest_first;  // workgroups go to the sequences by their length
+    int longest_first;   // workgroups go to the sequences by what their rows see (0: as they come)
     size_t ws_bytes;   // of partials
 };
 AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head, size_t max_len, int window, int sinks,

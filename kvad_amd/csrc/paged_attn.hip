@@ -1016,39 +1016,46 @@ constexpr int waves_for(int es, int d, int rows, bool ahead = false) {
 // find_seq of up to 64 sequences, those whose rows see the most positions first: where
 // there are more workgroups than CUs, the last to start, or to have a CU's memory to
 // themselves, are then short ones (64 sequences of 1333 to 4000, 8 KV heads of 128:
-// 4-bit rows 47 us against 44, i8 73.4 against 68.7).  Each lane adds up the tiles of
-// those before its own.  Sequences that see about as many stay as they come, as a
-// window makes them, and so does a prompt's chunk before others' single rows, whose
-// tiles take longer (3 chunks and 40 single rows, window 512, i8: 30.2 us, and sorted
-// by length 36.4).  Prompts beside single rows come out alike in any order they are
-// given in (900 rows and 40 sequences of 500 to 4000, i8: 66.7 us; as they come 84.4
-// with the prompt first and 60.4 with it last; f32 181 and 178, as they come 260 and 216).
-template <typename F>
+// 4-bit rows 47 us against 44, i8 72 against 67).  By levels of what a row sees, found
+// bit by bit, and as they come within one: ranking all 64 takes each wave 0.5 us, as
+// much as one of many_rows' turns (a prompt of 900 behind 40 sequences of 500 to 4000,
+// 32 heads on 8, i8: 62 us, ranked 66.5, as they come 60.5, or 84 with the prompt in
+// front).  Few rows go before many that see as much, whose workgroups are more than
+// places and fill what the others leave (a prompt of 3000 beside 63 single rows behind
+// 3000 to 4000, 12 heads on 2, f16: 98 us, by length 126).  Sequences that see about as
+// many stay as they come, as a window makes them (3 chunks and 40 single rows, window
+// 512, i8: 30.2 us, and with the single rows in front 36.4).
+constexpr int LEVELS = 64;  // that find_longest_first tells apart, of the longest sequence
+template <int ROWS, typename F>
 __device__ __forceinline__ bool find_longest_first(const Args &a, int tile, F count, int &seq, Seq &s, int &local, int &n) {
     const int lane = threadIdx.x & 63;
     Seq mine{0, 0, 0};
     if (lane < a.b.n_seq) mine.load(a.b, lane);
     const int tiles = count(mine);
+    const bool few = ROWS <= 16 || mine.n * a.group <= FEW;
     int seen = min(mine.len, a.window);
     seen += min(mine.len - seen, a.sinks);
     const unsigned long long some = __ballot(tiles > 0);
     const int seen0 = __builtin_amdgcn_readlane(seen, some ? __builtin_ctzll(some) : 0);
-    int first = 0;
-    if (!__ballot(tiles > 0 && abs(seen - seen0) > seen0 / 8)) {
-        first = dev::wave_scan(tiles) - tiles;
-    } else {
-        const int key = min(seen, 1 << 24) << 6 | (63 - lane);  // all different, those of lanes that have none last
-        if (a.b.row_start) {
+    // the level that the tile is in, and how many tiles those above have
+    int level = 0, above = 0, mine_level = 0;
+    if (__ballot(tiles > 0 && abs(seen - seen0) > seen0 / 8)) {
+        mine_level = min((seen >> (a.longest_first - 1)) + (few && a.window == INT32_MAX), LEVELS - 1);
+        level = LEVELS - 1;
 #pragma unroll
-            for (int j = 0; j < 64; j++)
-                first += __builtin_amdgcn_readlane(key, j) > key ? __builtin_amdgcn_readlane(tiles, j) : 0;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 64; j++) first += __builtin_amdgcn_readlane(key, j) > key;
-            first *= tiles;
+        for (int step = LEVELS / 2; step > 0; step /= 2) {
+            const bool over = mine_level > level - step;
+            const int sum = a.b.row_start ? __builtin_amdgcn_readlane(dev::wave_scan(over ? tiles : 0), 63)
+                                          : __builtin_popcountll(__ballot(over && tiles > 0)) * a.tiles_per;
+            if (sum <= tile) {
+                level -= step;
+                above = sum;
+            }
         }
     }
-    const unsigned long long here = __ballot(tile >= first && tile - first < tiles);
+    const int there = mine_level == level ? tiles : 0;
+    const int first = above + dev::wave_scan(there) - there;
+    const unsigned long long here = __ballot(tile >= first && tile - first < there);
     if (!here) return false;  // past the last tile
     seq = __builtin_ctzll(here);
     n = __builtin_amdgcn_readlane(tiles, seq);
@@ -1079,7 +1086,7 @@ void attn_kernel(Args a) {
     int local, tiles;
     auto count = [&](const Seq &q) { return (q.n * a.group + ROWS - 1) / ROWS; };
     if (a.longest_first) {
-        if (!find_longest_first(a, tile, count, w.seq, seq, local, tiles)) return;
+        if (!find_longest_first<ROWS>(a, tile, count, w.seq, seq, local, tiles)) return;
     } else if (a.b.row_start) {
         if (!find_seq(a.b, tile, count, w.seq, seq, local, tiles)) return;
     } else {
@@ -1330,7 +1337,11 @@ AttnPlan plan_attn(int cu_count, const kh_paged *kv, const Batch &b, int n_head,
     // alike, and finding that out is 0.2 to 0.6 us (64 of 3000 to 12000, 8 KV heads of
     // 128, window 256, i8: 12.0 against 11.7).
     const bool alike = window != INT32_MAX && (size_t)window < max_len / 4;
-    p.longest_first = p.splits == 1 && b.n_seq > 1 && b.n_seq <= 64 && all > cus && !alike;
+    p.longest_first = 0;
+    if (p.splits == 1 && b.n_seq > 1 && b.n_seq <= 64 && all > cus && !alike) {
+        p.longest_first = 1;
+        while ((pos_tiles * TILE) >> (p.longest_first - 1) >= (size_t)LEVELS - 1) p.longest_first++;
+    }
     return p;
 }
 
@@ -1356,7 +1367,7 @@ int launch_attn(kh_ctx *ctx, const AttnCall &c, const AttnPlan &p) {
     a.tiles_per = p.per;
     a.splits = p.splits;
     a.split_tiles = p.split_tiles;
-    a.longest_first = p.longest_first;
+    a.longest_first = p.longest_first;  // 1 + the bits that leave LEVELS of what a row sees
     a.window = c.window;
     a.sinks = c.sinks;
     a.scale = c.scale;

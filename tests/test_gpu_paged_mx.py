@@ -394,3 +394,24 @@ def test_sequences_by_what_their_rows_see(ctx, precision, chunk, window, sinks):
     q = (rng.standard_normal((40, 16, 64)) * 1.5).astype(np.float32)
     b = K.Batch.host([len(k) for k in p2.k], p2.pages, None, n_rows=40)
     p2.check(ones, 16, window=window, sinks=sinks, q=q, got=p2.cache.attend(0, b, 16, q, window=window, sinks=sinks))
+
+
+@pytest.mark.parametrize("precision", [MX, "i8"])
+@pytest.mark.parametrize("n_seq, kv", [(2, 160), (17, 40), (63, 8), (64, 8)])
+def test_sequences_of_every_length_by_levels(ctx, form, precision, n_seq, kv):  # noqa: F811
+    # lengths over three orders, several of a level and of a length, few rows and
+    # many, a hint of the longest that is far too small
+    rng = np.random.default_rng(n_seq)
+    lens = [int(n) for n in np.exp(rng.uniform(0, np.log(600), n_seq))]
+    lens[0], lens[-1] = 600, 1
+    lens[n_seq // 2] = lens[n_seq // 3] = 300
+    counts = [min(n, int(rng.choice([0, 1, 1, 1, 3, 40]))) for n in lens]
+    counts[0], counts[-1] = 1, 1
+    p = Pool(ctx, rng, precision, kv, 64, 32, lens)
+    p.push([n - c for n, c in zip(lens, counts)])
+    p.push(counts)
+    q = (rng.standard_normal((sum(counts), kv, 64)) * 1.5).astype(np.float32)
+    p.check(counts, kv, q=q)
+    b = p.batch(counts)
+    b.max_len = 2
+    p.check(counts, kv, q=q, got=p.cache.attend(0, b, kv, q))
