@@ -264,7 +264,7 @@ int kh_mla_attend_dev(kh_ctx *ctx, size_t n_head, const float *q_lat, const floa
  *           two 2^e for each 32 dims of the head's row from its first on: 3.5 2^e
  *           <= amax < 7 2^e, the nearest of them, of two as near the one of even
  *           code; e not under -128, nor more than 26 under the row's largest.
- *           4.25 bits a value, and 32 a row
+ *           4.25 bits a dim as it is kept, and 32 a row
  * A value that rounds past f32's range reads back as infinity: KH_F16 from
  * 2^128 - 2^116 on, KH_MXFP4 from 1.75 2^127 on, KH_I8 the largest floats alone.  A row with a NaN or an
  * infinity in it reads back as NaN (KH_F32: as it is), and makes the attention
@@ -353,7 +353,10 @@ int kh_paged_attend_ws(const kh_paged *kv, const kh_batch *b, size_t n_head, siz
  * and where each new row goes.  All arrays are the caller's device memory, read
  * and written when the work runs, and a kh_batch over len, pages and row_start
  * is what the cache's calls take.  n_seq is up to 4096, page_size as the
- * cache's.  Calls on one table are made on one stream, one behind the other. */
+ * cache's.  Calls on one table are made on one stream, one behind the other.  A
+ * table that the caller fills, instead of kh_pages_init_dev, gives each sequence a
+ * page of 0 .. n_pages - 1 for every page_size positions of its len: a release puts
+ * on the stack what stands there. */
 typedef struct kh_page_table {
     size_t n_seq, max_pages, page_size, n_pages;
     int32_t *len;        /* [n_seq]: positions each sequence holds */

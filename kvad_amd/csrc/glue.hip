@@ -265,7 +265,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_residual_kernel(No
 }
 
 // Rows that registers do not hold: y is read twice, and x' again where it was
-// written, each element by the thread that wrote it.
+// written, each element by the thread that wrote it.  Bound by memory and by the loops'
+// loads, of which a thread has few in flight (512 rows of 16384, norms on both sides and
+// a gate a row: 39.2 us for the 168 MB that have to move, 4.3 TB/s; 1025 of 8193, three
+// steps of which the last is nearly empty, 45 us, where 8192 are held and take 37; 32 of
+// 16384 8.2 us).
 __global__ __launch_bounds__(1024) void norm_residual_long_kernel(NormResidual a) {
     __shared__ float s_red[2][16];
     const size_t r = blockIdx.x;

@@ -5,8 +5,9 @@
 // Both kernels move each byte once and are bound by HBM, or by the launch for
 // a few rows (20001 positions of 8 heads of 128 read from i8: 43 us for 206 MB,
 // 4.8 TB/s, a large copy's rate; 4500 rows written in 13 us, 3.5 TB/s; 48 single
-// rows 3.7 us; 3900 rows in 4 bits 8 us a way, 4.0 TB/s).  A workgroup takes the 32 positions of one layout tile, one KV
-// head, K and V: a cache unit of V runs over positions and a row over dims, so
+// rows 3.7 us; 3900 rows in 4 bits 8.0 us in and 7.8 out at the least of a trace, 4.0
+// TB/s, 9.6 and 8.6 in the mean).  A workgroup takes the 32 positions of one layout
+// tile, one KV head, K and V: a cache unit of V runs over positions and a row over dims, so
 // the tile is turned in LDS, and both sides go in whole lines: rows of
 // head_dim floats, and 16-byte units 32 to 256 in a run.
 #include <cmath>

@@ -10,10 +10,13 @@
 // written by the last to have read them.  Whether the call can be done is known from
 // the sums: all workgroups find the same, and either all do it or none.
 //
-// What bounds it: trips to memory one behind the other (lengths, then pages, then
-// what is written), and the launch: 64 sequences of a decode step 4.1 us, their
-// release 3.4; 137000 new rows of 33 sequences, 4300 pages, 6.4 us, their release 3.5.
-// The bytes alone would take 0.3.
+// What bounds it: trips to memory one behind the other (lengths; a step's row counts,
+// which the compiler loads behind the check of the length; of several workgroups the
+// count of those that have read, which the first wave of each waits for; pages; what
+// is written), and the launch.  Alone on an idle device, mean and least of a trace: 64
+// sequences of a decode step 4.5 and 4.2 us, their release 3.6 and 3.3; 137000 new rows
+// of 33 sequences, 4300 pages, 6.9 and 5.8, their release 4.7 and 4.4.  The bytes alone
+// would take 0.3.
 #include <algorithm>
 
 #include "common.hpp"
@@ -67,7 +70,6 @@ __device__ __forceinline__ Change change_of(const Args &a, int len, int arg) {
             c.bad = BAD_ROWS;
         } else if (arg > cap - len) {
             c.bad = TOO_LONG;
-            c.rows = arg;
         } else {
             c.rows = arg;
             c.first = pages_for(len, a.page_shift);
@@ -80,8 +82,8 @@ __device__ __forceinline__ Change change_of(const Args &a, int len, int arg) {
     return c;
 }
 
-// Of each sequence the sums before it, its length (of a release: the positions it
-// keeps) and what it had before, in LDS; and what all workgroups find alike.
+// Of each sequence the sums before it and its length (of a release: the positions it
+// keeps), in LDS; and what all workgroups find alike.
 struct Sums {
     int rows[MAX_SEQ], pages[MAX_SEQ], len[MAX_SEQ];
     int wave_rows[THREADS / 64], wave_pages[THREADS / 64], wave_bad[THREADS / 64];
@@ -160,8 +162,8 @@ __device__ __forceinline__ int find(const int *starts, int n, int i) {
 }
 
 // Whether this workgroup is the last of the launch to have read the arrays that are
-// then written; asked early, as nothing waits for the answer but the first wave, whose
-// it is (the others get false).
+// then written; asked as soon as it has.  The first wave waits for the answer, whose it
+// is (the others get false, and go on to their rows and pages).
 __device__ __forceinline__ bool last_one(const Args &a) {
     if (threadIdx.x >= 64) return false;
     if (gridDim.x == 1) return true;
